@@ -259,6 +259,92 @@ V3G_API int v3g_token_bytes(const v3g_tokenizer *t, uint32_t id, const uint8_t *
 V3G_API int v3g_argmax_noalloc(const float *dev_logits, uint32_t rows, uint32_t vocab, uint64_t ld, int32_t *dev_tokens,
                                void *stream);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * Paged 8-bit KV cache, attention over it, and beam search (no counterpart in the reference).
+ *
+ * A cache holds pages of `page` tokens for every layer and KV head.  Codes are bytes biased by 128; the 16
+ * consecutive tokens of a block share one fp32 scale per head: value = (code - 128) * scale.
+ *   k, v             uint8  [n_layers][n_pages][n_kv_heads][page][head_dim]   (16-byte aligned)
+ *   k_scale, v_scale float  [n_layers][n_pages][n_kv_heads][page / 16]
+ * head_dim 64 or 128; page 16, 32, 64, 128 or 256.  A scale below 2^-120 is stored as zero; a block that was given a
+ * NaN or an infinity has the scale NaN and reads as NaN.  The arrays need no initial content: a block's first token
+ * starts its scale.
+ *
+ * A batch names its sequences by device arrays.  Token i of sequence b (packed index q_start[b] + i, of
+ * n_b = q_start[b + 1] - q_start[b]) stands at position kv_len[b] - n_b + i, so kv_len counts the batch's tokens too
+ * and the same arrays serve the append and the attention that follows.  Sequences without tokens are allowed.
+ * Position p of sequence b lives in page page_table[b * table_ld + p / page]; an entry outside [0, n_pages) is no
+ * page: nothing is stored there and attention sees no key there.  The arrays are not read on the host; whatever they
+ * hold, no kernel leaves the cache's and the batch's bounds. */
+enum { V3G_F32 = 0, V3G_F16 = 1, V3G_BF16 = 2 };   /* element types of rows */
+#define V3G_BEAM_MAX 32
+
+typedef struct {
+    uint8_t *k, *v;
+    float *k_scale, *v_scale;
+    uint32_t n_layers, n_pages, n_kv_heads, page, head_dim;
+} v3g_kv_cache_t;
+typedef struct {
+    const int32_t *page_table;        /* device [batch][table_ld], max_pages columns used */
+    uint64_t table_ld;
+    const int32_t *kv_len, *q_start;  /* device [batch], [batch + 1] */
+    uint32_t batch, max_pages, n_tokens;   /* n_tokens >= q_start[batch]: the packed rows */
+} v3g_kv_batch_t;
+typedef struct {
+    const void *data;                 /* device rows: token t, head h at data + t * tok_stride + h * head_stride */
+    int64_t tok_stride, head_stride;  /* in elements; head_dim consecutive elements per row */
+} v3g_rows_t;
+
+/* Append the batch's tokens to `layer`: rotate k at each token's position (rope: device [rope_rows][head_dim], row p
+ * holds head_dim / 2 cosines, then sines; pairs i, i + head_dim / 2; NULL: no rotation), round k and v to 8 bits and
+ * write them to their pages.  Per block and head, s = max(s_old, max |x| / 127) over the block's new rows, s_old
+ * counting only when the block holds earlier tokens; new codes are rint(x / s), earlier codes move to
+ * rint(code * s_old / s) where s grew.  With q (n_q_heads) the rotated queries go to q_out [n_tokens][n_q_heads]
+ * [head_dim] of the same type.  Tokens without a page or a rotation row are dropped (queries without a rotation row
+ * become zero) and set V3G_STATUS_BOUNDS in *dev_status (may be NULL).  A page that is written must belong to one
+ * sequence of the batch. */
+V3G_API int v3g_kv_append(const v3g_kv_cache_t *cache, uint32_t layer, const v3g_kv_batch_t *batch, int dtype, const v3g_rows_t *k,
+                          const v3g_rows_t *v, const v3g_rows_t *q, uint32_t n_q_heads, void *q_out, const float *rope,
+                          uint32_t rope_rows, int32_t *dev_status, void *stream);
+/* Values of tokens [first[b], kv_len[b]) of n_layers layers: batch->q_start holds the packed row where each
+ * sequence's values start, batch->n_tokens all rows; k_out, v_out [n_layers][n_tokens][n_kv_heads][head_dim].  Rows of
+ * no token or no page become zero. */
+V3G_API int v3g_kv_read(const v3g_kv_cache_t *cache, uint32_t layer, uint32_t n_layers, const v3g_kv_batch_t *batch,
+                        const int32_t *dev_first, int dtype, void *k_out, void *v_out, void *stream);
+/* Attention of the batch's query rows (dtype V3G_F16 or V3G_BF16) over `layer`: out [n_tokens][n_q_heads][head_dim] of
+ * the same type, lse [n_tokens][n_q_heads] fp32 (natural logarithm of the sum of exponentials; may be NULL).  Query
+ * heads h n_q_heads / n_kv_heads .. share KV head h.  A token at position p sees keys j <= p with j > p - window or
+ * j < n_sink (window 0: all).  A row that sees no key gives zeros and lse -inf.  max_q and max_kv are the largest token
+ * count and length of a sequence as far as the host knows them (0: unknown): they choose kernels and splits, never
+ * results' validity.  dev_work: v3g_kv_attention_work_size bytes of device memory, 256-byte aligned, with no content
+ * kept between calls. */
+V3G_API size_t v3g_kv_attention_work_size(const v3g_kv_cache_t *cache, const v3g_kv_batch_t *batch, uint32_t n_q_heads,
+                                          uint32_t max_q, uint32_t max_kv, uint32_t window, uint32_t n_sink);
+V3G_API int v3g_kv_attention(const v3g_kv_cache_t *cache, uint32_t layer, const v3g_kv_batch_t *batch, int dtype, const v3g_rows_t *q,
+                             uint32_t n_q_heads, float scale, uint32_t window, uint32_t n_sink, uint32_t max_q, uint32_t max_kv,
+                             void *out, float *lse, void *dev_work, size_t work_bytes, void *stream);
+/* Reorder the caches of groups of `beams` consecutive sequences (1..32; the sequences of a group have equal kv_len):
+ * row g * beams + j continues beam parents[g * beams + j] of its group.  table_out (another buffer) receives the new
+ * page table: the parent's entries for full pages, dst_page (NULL: the row's own entry) for the page still being
+ * filled, into which the parent's tokens of that page are copied in every layer, and the row's own entries beyond.  A
+ * group's pages still being filled may be each other's sources; they must not be another group's.  A parent outside
+ * the group or a missing page leaves the row as it was and sets V3G_STATUS_BOUNDS in *dev_status (may be NULL).
+ * batch->q_start and n_tokens are not used. */
+V3G_API int v3g_kv_reorder(const v3g_kv_cache_t *cache, const v3g_kv_batch_t *batch, uint32_t beams, const int32_t *dev_parents,
+                           const int32_t *dev_dst_page, int32_t *table_out, uint64_t table_out_ld, int32_t *dev_status, void *stream);
+/* One step of beam search: of every group's beams x vocab continuations, scored (logit - logsumexp of the beam's
+ * logits) + scores[beam], the `beams` best in descending order; equal scores go to the lower beam * vocab + token
+ * (different logits of one beam that round to the same score may also come in the order of the logits).
+ * logits [groups * beams] rows ld elements apart (dtype any).  A finished beam (finished may be NULL) has one
+ * continuation: eos_id at its own score.  Continuations scored NaN or -inf are never chosen; slots left over get token
+ * eos_id (0 when eos_id < 0), parent = their own beam, score -inf and count as finished.  NaN logits are skipped.
+ * Outputs [groups][beams]; finished_out: the parent's flag, or token == eos_id.  dev_work:
+ * v3g_beam_select_work_size bytes, 256-byte aligned. */
+V3G_API size_t v3g_beam_select_work_size(uint32_t groups, uint32_t beams, uint32_t vocab);
+V3G_API int v3g_beam_select(const void *dev_logits, int dtype, uint32_t groups, uint32_t beams, uint32_t vocab, uint64_t ld,
+                            const float *dev_scores, const uint8_t *dev_finished, int32_t eos_id, int32_t *tokens, int32_t *parents,
+                            float *scores_out, uint8_t *finished_out, void *dev_work, size_t work_bytes, void *stream);
+
 V3G_API const char *v3g_error_string(int code);
 V3G_API const char *v3g_last_error(void);   /* detail of the last failure on this thread */
 

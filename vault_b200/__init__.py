@@ -15,8 +15,11 @@ def __getattr__(name):
     if name in ("Governor", "VAULTv3ForCausalLM", "VAULTv3State", "sample_topk"):
         from . import model
         return getattr(model, name)
+    if name in ("PagedKVCache", "beam_select", "rope_table"):
+        from . import paged
+        return getattr(paged, name)
     raise AttributeError(name)
 
 
-__all__ = ["Governor", "VAULTv3Config", "VAULTv3ForCausalLM", "VAULTv3State", "VLT3Error", "read_vlt3", "sample_topk",
-           "Tokenizer", "vlt3_config", "write_vlt3"]
+__all__ = ["Governor", "PagedKVCache", "VAULTv3Config", "VAULTv3ForCausalLM", "VAULTv3State", "VLT3Error", "beam_select", "read_vlt3",
+           "rope_table", "sample_topk", "Tokenizer", "vlt3_config", "write_vlt3"]

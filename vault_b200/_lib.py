@@ -41,6 +41,24 @@ class GovRules(C.Structure):
     _fields_ = [("n_rules", C.c_uint32), ("rule_len", C.c_uint32 * 8), ("rules", (C.c_uint8 * 32) * 8)]
 
 
+class KVCache(C.Structure):
+    """v3g_kv_cache_t: a paged 8-bit cache's device arrays and sizes."""
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + \
+               [(n, C.c_uint32) for n in ("n_layers", "n_pages", "n_kv_heads", "page", "head_dim")]
+
+
+class KVBatch(C.Structure):
+    """v3g_kv_batch_t: the sequences of one call."""
+    _fields_ = [("page_table", C.c_void_p), ("table_ld", C.c_uint64), ("kv_len", C.c_void_p), ("q_start", C.c_void_p),
+                ("batch", C.c_uint32), ("max_pages", C.c_uint32), ("n_tokens", C.c_uint32)]
+
+
+class Rows(C.Structure):
+    """v3g_rows_t: strided rows of one operand."""
+    _fields_ = [("data", C.c_void_p), ("tok_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+V3G_F32, V3G_F16, V3G_BF16 = 0, 1, 2
 GOV_STREAM_BYTES = 192   # sizeof(v3g_gov_stream_t)
 
 _P = C.c_void_p
@@ -85,6 +103,17 @@ _SIGS = {
     "v3g_gemm_work_size": (C.c_size_t, [_P, C.c_uint32, C.c_uint32]),
     "v3g_gemm": (C.c_int, [_P, C.c_uint32, _P, C.c_uint32, _P, _P, C.c_size_t, _P]),
     "v3g_argmax_noalloc": (C.c_int, [_P, C.c_uint32, C.c_uint32, C.c_uint64, _P, _P]),
+    "v3g_kv_append": (C.c_int, [C.POINTER(KVCache), C.c_uint32, C.POINTER(KVBatch), C.c_int, C.POINTER(Rows), C.POINTER(Rows),
+                                C.POINTER(Rows), C.c_uint32, _P, _P, C.c_uint32, _P, _P]),
+    "v3g_kv_read": (C.c_int, [C.POINTER(KVCache), C.c_uint32, C.c_uint32, C.POINTER(KVBatch), _P, C.c_int, _P, _P, _P]),
+    "v3g_kv_attention_work_size": (C.c_size_t, [C.POINTER(KVCache), C.POINTER(KVBatch), C.c_uint32, C.c_uint32, C.c_uint32,
+                                                C.c_uint32, C.c_uint32]),
+    "v3g_kv_attention": (C.c_int, [C.POINTER(KVCache), C.c_uint32, C.POINTER(KVBatch), C.c_int, C.POINTER(Rows), C.c_uint32, C.c_float,
+                                   C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, _P, _P, _P, C.c_size_t, _P]),
+    "v3g_kv_reorder": (C.c_int, [C.POINTER(KVCache), C.POINTER(KVBatch), C.c_uint32, _P, _P, _P, C.c_uint64, _P, _P]),
+    "v3g_beam_select_work_size": (C.c_size_t, [C.c_uint32, C.c_uint32, C.c_uint32]),
+    "v3g_beam_select": (C.c_int, [_P, C.c_int, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint64, _P, _P, C.c_int32, _P, _P, _P, _P, _P,
+                                  C.c_size_t, _P]),
     "v3g_error_string": (C.c_char_p, [C.c_int]),
     "v3g_last_error": (C.c_char_p, []),
 }

@@ -1,0 +1,499 @@
+// Paged 8-bit KV cache: append with the position rotation, read-back, and reordering for beam search.
+//
+// All three move bytes and are bound by HBM at large sizes and by launch latency at small ones.
+#include <cfloat>
+
+#include "v3g_internal.h"
+#include "v3g_kv.cuh"
+
+namespace v3g {
+
+// ------------------------------------------------------------------------------------------------------- append
+// One CTA takes the new tokens of one 16-token block of one sequence (all heads, or the blockIdx.y-th share of
+// them), because a scale belongs to a block: the CTA's warps are its only writers, so there are no atomics and the
+// codes are the same every time.  The rotation's cosines and sines of the block's tokens are staged once in shared
+// memory and serve every head.  A warp holds the block's rows of one head in registers between the two uses (the
+// largest magnitude, then the rounding), so each input is read once.
+//
+// x' = rotation of x (pairs i, i + D/2; fp32, each product and sum rounded by itself), s = max(s_old, max |x'| / 127),
+// code = rint(x' * (1 / s)).  A larger s moves the block's earlier codes to rint(code * (s_old / s)).
+constexpr int APPEND_WARPS = 8;
+
+struct AppendArgs {
+    KvView c;
+    const void *k, *v, *q;
+    int64_t k_tok, k_head, v_tok, v_head, q_tok, q_head;   // strides in elements
+    void *q_out;                                           // [tokens][q_heads][D]
+    int q_heads, rope_rows;
+    const float *rope;                                     // [rope_rows][D / 2 cos | D / 2 sin], null: no rotation
+    int32_t *status;
+    bool k_vec, v_vec, q_vec;
+};
+
+// the rotation of the four dims that start at 4 l (l: lane in the row) given the partner half's four values
+template <int D>
+__device__ __forceinline__ float4 rotate4(float4 x, float4 other, const float *cs, int l) {
+    constexpr int HL = D / 8;                              // lanes of a half row
+    const float4 c = *reinterpret_cast<const float4 *>(cs + 4 * (l % HL));
+    float4 s = *reinterpret_cast<const float4 *>(cs + D / 2 + 4 * (l % HL));
+    if (l < HL) s = make_float4(-s.x, -s.y, -s.z, -s.w);   // x1 c - x2 s; x2 c + x1 s
+    return make_float4(__fadd_rn(__fmul_rn(x.x, c.x), __fmul_rn(other.x, s.x)), __fadd_rn(__fmul_rn(x.y, c.y), __fmul_rn(other.y, s.y)),
+                       __fadd_rn(__fmul_rn(x.z, c.z), __fmul_rn(other.z, s.z)), __fadd_rn(__fmul_rn(x.w, c.w), __fmul_rn(other.w, s.w)));
+}
+__device__ __forceinline__ float4 shfl4(float4 x, int mask) {
+    return make_float4(__shfl_xor_sync(0xffffffffu, x.x, mask), __shfl_xor_sync(0xffffffffu, x.y, mask),
+                       __shfl_xor_sync(0xffffffffu, x.z, mask), __shfl_xor_sync(0xffffffffu, x.w, mask));
+}
+__device__ __forceinline__ uint32_t code_byte(float x, float inv) {
+    return (uint32_t)((int)rintf(fminf(fmaxf(__fmul_rn(x, inv), -127.f), 127.f)) + 128);
+}
+__device__ __forceinline__ uint32_t moved_codes(uint32_t w, float ratio) {
+    uint32_t r = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        r |= (uint32_t)((int)rintf(__fmul_rn((float)((int)((w >> (8 * i)) & 255u) - 128), ratio)) + 128) << (8 * i);
+    return r;
+}
+
+// one head's rows [s0, s1) of a block: the rounding described above
+template <typename T, int D>
+__device__ __forceinline__ void append_rows(const T *src, int64_t tok_ld, bool vec, const float *cs, bool turn, int s0, int s1,
+                                            uint8_t *codes, float *scale, int lane) {
+    constexpr int LR = D / 4, RP = 32 / LR, NP = KV_BLOCK / RP;   // lanes of a row, rows of a pass, passes
+    const int l = lane % LR, sub = lane / LR;
+    const float s_old = s0 > 0 ? *scale : 0.f;
+    float4 x[NP];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        const int r = s0 + i * RP + sub;
+        x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < s1) x[i] = kv_load4<T>(src + (int64_t)(r - s0) * tok_ld + 4 * l, vec);
+    }
+    float top = 0.f;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        const int r = s0 + i * RP + sub;
+        if (s0 + i * RP >= s1) break;   // uniform over the warp
+        if (turn) {
+            const float4 o = shfl4(x[i], LR / 2);
+            if (r < s1) x[i] = rotate4<D>(x[i], o, cs + (r - s0) * D, l);
+        }
+        const float a = fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
+        bad |= !(fabsf(x[i].x) <= FLT_MAX && fabsf(x[i].y) <= FLT_MAX && fabsf(x[i].z) <= FLT_MAX && fabsf(x[i].w) <= FLT_MAX);
+        top = fmaxf(top, a);
+    }
+    top = warp_max(top);
+    bad = __any_sync(0xffffffffu, bad) || s_old != s_old;
+    float s = fmaxf(s_old, __fmul_rn(top, 1.f / 127.f));
+    if (s < KV_SCALE_MIN) s = 0.f;
+    if (bad) s = __int_as_float(0x7FC00000);   // the block holds a NaN or an infinity: it reads as NaN
+    const float inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
+    if (s0 > 0 && s != s_old) {
+        const float ratio = s > 0.f ? __fdiv_rn(s_old, s) : 0.f;
+        for (int r = sub; r < s0; r += RP) {
+            uint32_t *p = reinterpret_cast<uint32_t *>(codes + r * D + 4 * l);
+            *p = moved_codes(*p, ratio);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        const int r = s0 + i * RP + sub;
+        if (r < s1) {
+            uint32_t w = 0x80808080u;
+            if (!bad)
+                w = code_byte(x[i].x, inv) | code_byte(x[i].y, inv) << 8 | code_byte(x[i].z, inv) << 16 | code_byte(x[i].w, inv) << 24;
+            *reinterpret_cast<uint32_t *>(codes + r * D + 4 * l) = w;
+        }
+    }
+    __syncwarp();
+    if (lane == 0) *scale = s;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(32 * APPEND_WARPS) k_kv_append(const __grid_constant__ AppendArgs a) {
+    __shared__ __align__(16) float cs[KV_BLOCK * D];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int64_t base;
+    const int b = kv_find(a.c.q_start, a.c.batch, a.c.n_tokens, KV_BLOCK, 1, 2, blockIdx.x, base);
+    int first;
+    const int n = a.c.tokens(b, first);
+    const int p0 = a.c.end(b) - n;                                        // position of the first new token
+    const int blk = (p0 >> 4) + (int)(blockIdx.x - base);                 // arithmetic shift: p0 may be negative
+    const int lo = max(blk * KV_BLOCK, p0), hi = min(blk * KV_BLOCK + KV_BLOCK, p0 + n);
+    if (lo >= hi) return;
+    const int t0 = first + (lo - p0), nt = hi - lo;                       // the block's packed tokens
+    const int s0 = lo - blk * KV_BLOCK;
+    const bool turn = a.rope != nullptr;
+    const int page = a.c.page_of(b, lo);
+    // tokens that the rotation table reaches; the others have no place, and their queries become zero
+    const int placed = lo < 0 ? 0 : (turn ? max(min(a.rope_rows - lo, nt), 0) : nt);
+    if (threadIdx.x == 0 && (page < 0 || placed < nt) && a.status) atomicOr(a.status, STATUS_BOUNDS);
+    if (turn) {
+        const float4 *src = reinterpret_cast<const float4 *>(a.rope + (int64_t)lo * D);
+        for (int i = threadIdx.x; i < placed * D / 4; i += 32 * APPEND_WARPS) reinterpret_cast<float4 *>(cs)[i] = __ldg(src + i);
+        __syncthreads();
+    }
+    const int heads = a.c.heads, step = APPEND_WARPS * gridDim.y, w0 = blockIdx.y * APPEND_WARPS + warp;
+    if (page >= 0 && placed > 0)
+        for (int t = w0; t < 2 * heads; t += step) {
+            const bool is_v = t >= heads;
+            const int h = is_v ? t - heads : t;
+            const int64_t at = a.c.block(page, h, lo);
+            const T *src = is_v ? static_cast<const T *>(a.v) + (int64_t)t0 * a.v_tok + (int64_t)h * a.v_head
+                                : static_cast<const T *>(a.k) + (int64_t)t0 * a.k_tok + (int64_t)h * a.k_head;
+            append_rows<T, D>(src, is_v ? a.v_tok : a.k_tok, is_v ? a.v_vec : a.k_vec, cs, turn && !is_v, s0, s0 + placed,
+                              (is_v ? a.c.v : a.c.k) + at * (KV_BLOCK * D), (is_v ? a.c.vs : a.c.ks) + at, lane);
+        }
+    if (a.q) {   // the queries of the same tokens: rotated, not rounded further than their own type
+        constexpr int LR = D / 4, RP = 32 / LR, U = 4;
+        const int l = lane % LR, sub = lane / LR, rows = nt * a.q_heads;
+        // shares of the warps that hold no K/V row come first
+        const int w1 = (w0 + step - 2 * heads % step) % step;
+        for (int r0 = w1 * RP * U; r0 < rows; r0 += step * RP * U) {
+            float4 x[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int r = r0 + u * RP + sub, tok = r / a.q_heads, h = r - tok * a.q_heads;
+                x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (r < rows)
+                    x[u] = kv_load4<T>(static_cast<const T *>(a.q) + (int64_t)(t0 + tok) * a.q_tok + (int64_t)h * a.q_head + 4 * l, a.q_vec);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int r = r0 + u * RP + sub, tok = r / a.q_heads, h = r - tok * a.q_heads;
+                const float4 o = shfl4(x[u], LR / 2);
+                if (r < rows) {
+                    if (tok >= placed) x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    else if (turn) x[u] = rotate4<D>(x[u], o, cs + tok * D, l);
+                    kv_store4(static_cast<T *>(a.q_out) + ((int64_t)(t0 + tok) * a.q_heads + h) * D + 4 * l, x[u]);
+                }
+            }
+        }
+    }
+}
+
+// --------------------------------------------------------------------------------------------------------- read
+// Values of tokens [first[b], kv_len[b]) of every sequence, of `layers` layers: row row_start[b] + i is token
+// first[b] + i.  A thread takes eight dims of one row of one head; rows without a page read as zero.
+struct ReadArgs {
+    KvView c;                     // layer 0 of the call; q_start holds row_start, n_tokens the rows
+    const int32_t *first;
+    int64_t layer_codes, layer_scales;
+    int layers;
+    void *k, *v;                  // [layers][rows][heads][D]
+};
+
+__device__ __forceinline__ void read8(uint2 w, float s, float4 &lo, float4 &hi) {
+    auto f = [&](uint32_t u, int i) { return __fmul_rn((float)((int)((u >> (8 * i)) & 255u) - 128), s); };
+    lo = make_float4(f(w.x, 0), f(w.x, 1), f(w.x, 2), f(w.x, 3));
+    hi = make_float4(f(w.y, 0), f(w.y, 1), f(w.y, 2), f(w.y, 3));
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(256) k_kv_read(const __grid_constant__ ReadArgs a) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t row = i / (a.c.heads * (D / 8));
+    if (row >= a.c.n_tokens) return;
+    const int rest = (int)(i - row * (a.c.heads * (D / 8))), h = rest / (D / 8), d = rest % (D / 8) * 8;
+    int64_t base;
+    const int b = kv_find(a.c.q_start, a.c.batch, a.c.n_tokens, 1, 1, 0, row, base);
+    const int pos = a.first[b] + (int)(row - base);
+    const bool in = base <= row && row < a.c.q_start[b + 1] && pos >= 0 && pos < a.c.len(b);
+    const int page = in ? a.c.page_of(b, pos) : -1;
+    const int64_t at = page >= 0 ? a.c.block(page, h, pos) : 0;
+    for (int l = blockIdx.y; l < a.layers; l += gridDim.y) {
+#pragma unroll
+        for (int kind = 0; kind < 2; ++kind) {
+            float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
+            if (page >= 0) {
+                const uint8_t *codes = (kind ? a.c.v : a.c.k) + l * a.layer_codes;
+                const float s = (kind ? a.c.vs : a.c.ks)[l * a.layer_scales + at];
+                read8(*reinterpret_cast<const uint2 *>(codes + (at * KV_BLOCK + (pos & 15)) * D + d), s, lo, hi);
+            }
+            T *out = static_cast<T *>(kind ? a.v : a.k) + (((int64_t)l * a.c.n_tokens + row) * a.c.heads + h) * D + d;
+            kv_store4(out, lo);
+            kv_store4(out + 4, hi);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------ reorder
+// Beam j of a group continues beam parents[j]: full pages are shared through the table, the page still being
+// filled is copied (codes and scales of its tokens, every layer).  A thread owns one 16-byte unit of the page and
+// reads it from all of the group's parents before it writes any of the children, so a child's page may be another
+// child's source; groups share no page that is still being filled.
+struct ReorderArgs {
+    KvView c;
+    int64_t layer_codes, layer_scales;
+    int layers, beams;
+    const int32_t *parents, *dst;
+    int32_t *out;
+    int64_t out_ld;
+    int32_t *status;
+};
+
+template <int KB, int D>
+__global__ void __launch_bounds__(256) k_kv_reorder(const __grid_constant__ ReorderArgs a) {
+    __shared__ int src_s[KB], dst_s[KB], par_s[KB];
+    const int g = blockIdx.y, r0 = g * a.beams;
+    const int len = a.c.len(r0), full = len >> a.c.page_shift, tail = len & (a.c.page - 1);
+    if (threadIdx.x < KB) {
+        const int j = threadIdx.x;
+        int par = -1, src = -1, dst = -1;
+        if (j < a.beams) {
+            par = a.parents[r0 + j];
+            if (par < 0 || par >= a.beams) par = -1;
+            if (par >= 0 && tail) {
+                src = a.c.page_of(r0 + par, len);
+                dst = a.dst ? a.dst[r0 + j] : a.c.page_of(r0 + j, len);
+                if (dst >= a.c.n_pages) dst = -1;
+            }
+            if (tail && (src < 0 || dst < 0)) par = src = -1;   // the row stays as it is
+            if (par < 0 && blockIdx.x == 0 && a.status) atomicOr(a.status, STATUS_BOUNDS);
+        }
+        par_s[j] = par;
+        src_s[j] = src == dst || dst < 0 ? -1 : src;
+        dst_s[j] = dst;
+    }
+    __syncthreads();
+    // the table: a column at a time, as the beams' rows of it are exchanged
+    for (int col = blockIdx.x * 256 + threadIdx.x; col < a.c.max_pages; col += gridDim.x * 256)
+#pragma unroll
+        for (int j = 0; j < KB; ++j)
+            if (j < a.beams) {
+                int from = r0 + j;
+                if (col < full && par_s[j] >= 0) from = r0 + par_s[j];
+                int32_t e = a.c.table[(int64_t)from * a.c.table_ld + col];
+                if (col == full && tail && par_s[j] >= 0 && dst_s[j] >= 0) e = dst_s[j];
+                a.out[(int64_t)(r0 + j) * a.out_ld + col] = e;
+            }
+    if (!tail) return;
+    const int upr = tail * (D / 16), blocks = (tail + 15) >> 4;   // 16-byte units and scales of one head's part of the page
+    const int64_t per_head = 2 * (int64_t)(upr + blocks), total = per_head * a.c.heads * a.layers;
+    const int64_t page_codes = (int64_t)a.c.heads * a.c.page * D, page_scales = (int64_t)a.c.heads * a.c.page / 16;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t lh = i / per_head;
+        int u = (int)(i - lh * per_head);
+        const int layer = (int)(lh / a.c.heads), h = (int)(lh - (int64_t)layer * a.c.heads);
+        const bool is_v = u >= upr + blocks;
+        if (is_v) u -= upr + blocks;
+        if (u < upr) {
+            uint8_t *p = (is_v ? a.c.v : a.c.k) + layer * a.layer_codes + (int64_t)h * a.c.page * D + (int64_t)u * 16;
+            uint4 x[KB];
+#pragma unroll
+            for (int j = 0; j < KB; ++j)
+                if (src_s[j] >= 0) x[j] = *reinterpret_cast<const uint4 *>(p + src_s[j] * page_codes);
+#pragma unroll
+            for (int j = 0; j < KB; ++j)
+                if (src_s[j] >= 0) *reinterpret_cast<uint4 *>(p + dst_s[j] * page_codes) = x[j];
+        } else {
+            float *p = (is_v ? a.c.vs : a.c.ks) + layer * a.layer_scales + (int64_t)h * (a.c.page / 16) + (u - upr);
+            float x[KB];
+#pragma unroll
+            for (int j = 0; j < KB; ++j)
+                if (src_s[j] >= 0) x[j] = p[src_s[j] * page_scales];
+#pragma unroll
+            for (int j = 0; j < KB; ++j)
+                if (src_s[j] >= 0) p[dst_s[j] * page_scales] = x[j];
+        }
+    }
+}
+
+// --------------------------------------------------------------------------------------------------------- host
+static bool aligned_to(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+int kv_view(const char *who, const v3g_kv_cache_t *c, uint32_t layer, const v3g_kv_batch_t *b, KvView *out) {
+    const std::string w = who;
+    if (!c || !b) return v3g_fail(V3G_E_ARG, w + ": null cache or batch");
+    if (!c->k || !c->v || !c->k_scale || !c->v_scale || !b->page_table || !b->kv_len || !b->q_start)
+        return v3g_fail(V3G_E_ARG, w + ": null pointer");
+    if (c->head_dim != 64 && c->head_dim != 128) return v3g_fail(V3G_E_UNSUPPORTED, w + ": head_dim must be 64 or 128");
+    if (c->page < 16 || c->page > 256 || (c->page & (c->page - 1)))
+        return v3g_fail(V3G_E_UNSUPPORTED, w + ": the page must hold 16, 32, 64, 128 or 256 tokens");
+    if (c->n_layers == 0 || c->n_pages == 0 || c->n_kv_heads == 0 || c->n_pages > 0x7FFFFFFFu || c->n_kv_heads > 65535u ||
+        c->n_layers > 65535u)
+        return v3g_fail(V3G_E_ARG, w + ": layers, pages and heads must be positive");
+    if (layer >= c->n_layers) return v3g_fail(V3G_E_ARG, w + ": no such layer");
+    if (b->max_pages == 0 || b->table_ld < b->max_pages || b->max_pages > 0x7FFFFFFFu / 256)
+        return v3g_fail(V3G_E_ARG, w + ": the page table needs at least one column and table_ld >= max_pages");
+    if (b->batch > 65535u || b->n_tokens > 0x7FFFFFFFu / 64) return v3g_fail(V3G_E_LIMIT, w + ": at most 65535 sequences and 2^25 tokens");
+    if (!aligned_to(c->k, 16) || !aligned_to(c->v, 16) || !aligned_to(c->k_scale, 4) || !aligned_to(c->v_scale, 4) ||
+        !aligned_to(b->page_table, 4) || !aligned_to(b->kv_len, 4) || !aligned_to(b->q_start, 4))
+        return v3g_fail(V3G_E_ALIGN, w + ": codes need 16-byte alignment");
+    const int64_t scales = (int64_t)c->n_pages * c->n_kv_heads * (c->page / 16), codes = scales * 16 * c->head_dim;
+    out->k = c->k + layer * codes;
+    out->v = c->v + layer * codes;
+    out->ks = c->k_scale + layer * scales;
+    out->vs = c->v_scale + layer * scales;
+    out->n_pages = (int)c->n_pages;
+    out->heads = (int)c->n_kv_heads;
+    out->page = (int)c->page;
+    out->page_shift = 31 - __builtin_clz(c->page);
+    out->table = b->page_table;
+    out->table_ld = (int64_t)b->table_ld;
+    out->max_pages = (int)b->max_pages;
+    out->batch = (int)b->batch;
+    out->n_tokens = (int)b->n_tokens;
+    out->kv_len = b->kv_len;
+    out->q_start = b->q_start;
+    return V3G_OK;
+}
+
+static int launched(const char *who) {
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? V3G_OK : v3g_fail(V3G_E_CUDA, std::string(who) + ": " + cudaGetErrorString(e));
+}
+
+static size_t dtype_bytes(int t) { return t == V3G_F32 ? 4 : 2; }
+
+// four-wide loads of rows: the base and both strides keep 4-element alignment
+static bool rows_vec(const v3g_rows_t &r, int dtype) {
+    return aligned_to(r.data, 4 * dtype_bytes(dtype)) && r.tok_stride % 4 == 0 && r.head_stride % 4 == 0;
+}
+
+template <typename T>
+static void launch_append(const AppendArgs &a, int D, dim3 grid, cudaStream_t st) {
+    if (D == 64) k_kv_append<T, 64><<<grid, 32 * APPEND_WARPS, 0, st>>>(a);
+    else k_kv_append<T, 128><<<grid, 32 * APPEND_WARPS, 0, st>>>(a);
+}
+
+template <typename T>
+static void launch_read(const ReadArgs &a, int D, dim3 grid, cudaStream_t st) {
+    if (D == 64) k_kv_read<T, 64><<<grid, 256, 0, st>>>(a);
+    else k_kv_read<T, 128><<<grid, 256, 0, st>>>(a);
+}
+
+template <int KB>
+static void launch_reorder(const ReorderArgs &a, int D, dim3 grid, cudaStream_t st) {
+    if (D == 64) k_kv_reorder<KB, 64><<<grid, 256, 0, st>>>(a);
+    else k_kv_reorder<KB, 128><<<grid, 256, 0, st>>>(a);
+}
+
+}  // namespace v3g
+
+using namespace v3g;
+
+extern "C" int v3g_kv_append(const v3g_kv_cache_t *cache, uint32_t layer, const v3g_kv_batch_t *batch, int dtype, const v3g_rows_t *k,
+                             const v3g_rows_t *v, const v3g_rows_t *q, uint32_t n_q_heads, void *q_out, const float *rope,
+                             uint32_t rope_rows, int32_t *dev_status, void *stream) {
+    AppendArgs a = {};
+    const int rc = kv_view("v3g_kv_append", cache, layer, batch, &a.c);
+    if (rc != V3G_OK) return rc;
+    if (dtype != V3G_F32 && dtype != V3G_F16 && dtype != V3G_BF16) return v3g_fail(V3G_E_DTYPE, "v3g_kv_append: fp32, fp16 or bf16 rows");
+    if (!k || !v || !k->data || !v->data) return v3g_fail(V3G_E_ARG, "v3g_kv_append: null rows");
+    if (q && (!q->data || !q_out || n_q_heads == 0 || n_q_heads > 65535u)) return v3g_fail(V3G_E_ARG, "v3g_kv_append: q needs heads and q_out");
+    if ((rope && rope_rows == 0) || rope_rows > 0x7FFFFFFFu) return v3g_fail(V3G_E_ARG, "v3g_kv_append: an empty rotation table");
+    const size_t e = dtype_bytes(dtype);
+    if (!aligned_to(k->data, e) || !aligned_to(v->data, e) || (q && (!aligned_to(q->data, e) || !aligned_to(q_out, 16))) ||
+        (rope && !aligned_to(rope, 16)) || !aligned_to(dev_status, 4))
+        return v3g_fail(V3G_E_ALIGN, "v3g_kv_append: q_out and the rotation table need 16-byte alignment, rows that of their type");
+    if (batch->batch == 0 || batch->n_tokens == 0) return V3G_OK;
+    a.k = k->data;
+    a.v = v->data;
+    a.k_tok = k->tok_stride;
+    a.k_head = k->head_stride;
+    a.v_tok = v->tok_stride;
+    a.v_head = v->head_stride;
+    a.k_vec = rows_vec(*k, dtype);
+    a.v_vec = rows_vec(*v, dtype);
+    if (q) {
+        a.q = q->data;
+        a.q_tok = q->tok_stride;
+        a.q_head = q->head_stride;
+        a.q_vec = rows_vec(*q, dtype);
+        a.q_heads = (int)n_q_heads;
+        a.q_out = q_out;
+    }
+    a.rope = rope;
+    a.rope_rows = (int)rope_rows;
+    a.status = dev_status;
+    const uint32_t items = batch->n_tokens / KV_BLOCK + 2 * batch->batch;
+    // heads are shared out over more CTAs while the blocks alone leave SMs idle; past one pass of the warps over
+    // the rows there is nothing left to share
+    const uint32_t passes = (2 * cache->n_kv_heads + (q ? n_q_heads * 2 : 0) + APPEND_WARPS - 1) / APPEND_WARPS;
+    uint32_t ny = 296 / (items ? items : 1);
+    ny = ny < 1 ? 1 : (ny > passes ? passes : ny);
+    const dim3 grid(items, ny);
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (dtype == V3G_F32) launch_append<float>(a, (int)cache->head_dim, grid, st);
+    else if (dtype == V3G_F16) launch_append<__half>(a, (int)cache->head_dim, grid, st);
+    else launch_append<__nv_bfloat16>(a, (int)cache->head_dim, grid, st);
+    return launched("v3g_kv_append");
+}
+
+extern "C" int v3g_kv_read(const v3g_kv_cache_t *cache, uint32_t layer, uint32_t n_layers, const v3g_kv_batch_t *batch,
+                           const int32_t *dev_first, int dtype, void *k_out, void *v_out, void *stream) {
+    ReadArgs a = {};
+    const int rc = kv_view("v3g_kv_read", cache, layer, batch, &a.c);
+    if (rc != V3G_OK) return rc;
+    if (dtype != V3G_F32 && dtype != V3G_F16 && dtype != V3G_BF16) return v3g_fail(V3G_E_DTYPE, "v3g_kv_read: fp32, fp16 or bf16 values");
+    if (!dev_first) return v3g_fail(V3G_E_ARG, "v3g_kv_read: null pointer");
+    if (n_layers == 0 || n_layers > cache->n_layers - layer) return v3g_fail(V3G_E_ARG, "v3g_kv_read: no such layers");
+    if (batch->batch == 0 || batch->n_tokens == 0) return V3G_OK;
+    if (!k_out || !v_out) return v3g_fail(V3G_E_ARG, "v3g_kv_read: null pointer");
+    if (!aligned_to(k_out, 16) || !aligned_to(v_out, 16) || !aligned_to(dev_first, 4))
+        return v3g_fail(V3G_E_ALIGN, "v3g_kv_read: outputs need 16-byte alignment");
+    a.first = dev_first;
+    a.layer_scales = (int64_t)cache->n_pages * cache->n_kv_heads * (cache->page / 16);
+    a.layer_codes = a.layer_scales * 16 * cache->head_dim;
+    a.layers = (int)n_layers;
+    a.k = k_out;
+    a.v = v_out;
+    const int64_t threads = (int64_t)batch->n_tokens * cache->n_kv_heads * (cache->head_dim / 8);
+    const int64_t gx = (threads + 255) / 256;
+    if (gx > 0x7FFFFFFF) return v3g_fail(V3G_E_LIMIT, "v3g_kv_read: too many values");
+    // a thread that takes several layers looks its page up once; few rows spread their layers over the GPU
+    int64_t gy = 2048 / gx;
+    gy = gy < 1 ? 1 : (gy > n_layers ? n_layers : gy);
+    const dim3 grid((uint32_t)gx, (uint32_t)gy);
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (dtype == V3G_F32) launch_read<float>(a, (int)cache->head_dim, grid, st);
+    else if (dtype == V3G_F16) launch_read<__half>(a, (int)cache->head_dim, grid, st);
+    else launch_read<__nv_bfloat16>(a, (int)cache->head_dim, grid, st);
+    return launched("v3g_kv_read");
+}
+
+extern "C" int v3g_kv_reorder(const v3g_kv_cache_t *cache, const v3g_kv_batch_t *batch, uint32_t beams, const int32_t *dev_parents,
+                              const int32_t *dev_dst_page, int32_t *table_out, uint64_t table_out_ld, int32_t *dev_status, void *stream) {
+    ReorderArgs a = {};
+    v3g_kv_batch_t rows;
+    if (batch) {
+        rows = *batch;
+        rows.q_start = rows.kv_len;   // a reorder has no new tokens: any readable array stands for q_start
+        rows.n_tokens = 0;
+    }
+    const int rc = kv_view("v3g_kv_reorder", cache, 0, batch ? &rows : nullptr, &a.c);
+    if (rc != V3G_OK) return rc;
+    if (beams == 0 || beams > V3G_BEAM_MAX) return v3g_fail(V3G_E_LIMIT, "v3g_kv_reorder: 1 to 32 beams");
+    if (batch->batch % beams) return v3g_fail(V3G_E_ARG, "v3g_kv_reorder: the rows are not whole groups of beams");
+    if (batch->batch == 0) return V3G_OK;
+    if (!dev_parents || !table_out) return v3g_fail(V3G_E_ARG, "v3g_kv_reorder: null pointer");
+    if (table_out_ld < batch->max_pages) return v3g_fail(V3G_E_ARG, "v3g_kv_reorder: table_out_ld < max_pages");
+    if (!aligned_to(dev_parents, 4) || !aligned_to(dev_dst_page, 4) || !aligned_to(table_out, 4) || !aligned_to(dev_status, 4))
+        return v3g_fail(V3G_E_ALIGN, "v3g_kv_reorder: misaligned pointer");
+    if (table_out == batch->page_table) return v3g_fail(V3G_E_ARG, "v3g_kv_reorder: table_out must be another buffer than the page table");
+    a.layer_scales = (int64_t)cache->n_pages * cache->n_kv_heads * (cache->page / 16);
+    a.layer_codes = a.layer_scales * 16 * cache->head_dim;
+    a.layers = (int)cache->n_layers;
+    a.beams = (int)beams;
+    a.parents = dev_parents;
+    a.dst = dev_dst_page;
+    a.out = table_out;
+    a.out_ld = (int64_t)table_out_ld;
+    a.status = dev_status;
+    const uint32_t groups = batch->batch / beams;
+    // 16-byte units of a whole page; the part that is filled is known on the device only
+    const int64_t units = (int64_t)cache->n_layers * cache->n_kv_heads * 2 * cache->page * (cache->head_dim / 16);
+    int64_t gx = (units + 255) / 256;
+    const int64_t most = (148 * 8 + groups - 1) / groups;
+    gx = gx > most ? most : gx;
+    const dim3 grid((uint32_t)gx, groups);
+    const cudaStream_t st = (cudaStream_t)stream;
+    const int D = (int)cache->head_dim;
+    if (beams <= 4) launch_reorder<4>(a, D, grid, st);
+    else if (beams <= 8) launch_reorder<8>(a, D, grid, st);
+    else if (beams <= 16) launch_reorder<16>(a, D, grid, st);
+    else launch_reorder<32>(a, D, grid, st);
+    return launched("v3g_kv_reorder");
+}

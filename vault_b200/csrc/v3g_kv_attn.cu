@@ -1,0 +1,490 @@
+// Attention over the paged 8-bit cache: few query rows per KV head (decode steps, short chunks).
+//
+// o_r = sum_j softmax_j(scale q_r . k_j) v_j over the visible keys of row r.  A decode step reads every visible key and
+// value once, 2 D bytes per key and KV head against 4 D G flops (G query heads share them), so HBM bounds it; the
+// kernel's work is to keep loads in flight and to spread one sequence over many SMs.
+//
+// * A CTA (4 warps) takes up to 8 NT rows (token, query head of one KV head) and a contiguous share of the visible
+//   16-key blocks; each warp takes every fourth of them with its own running maximum and sum, so the loop has no
+//   barrier.  A block of one head is 16 D consecutive bytes of codes; a warp loads K and V straight to registers, the
+//   next block's while it computes.
+// * S^T[key, row] = K Q^T on mma.sync m16n8k16 with the 16 keys as M: a lane's bytes of a key row are its fragment when
+//   the head dims are taken in that order (the contraction does not care), so no shared memory is used.  Codes become
+//   fp16 integers exactly (byte permute to 1024 + c, minus 1152).  fp16 queries enter as they are, bf16 queries as fp16
+//   after an exact power of two per row that puts the largest magnitude in [2^13, 2^14).
+// * The K scale of the block multiplies the scores, the V scale the probabilities: P' = p vs / ref with ref a power of
+//   two that follows the largest V scale seen, so P' keeps fp16's 11 bits whatever the scales are.  Sums, maxima and
+//   the accumulators are fp32.  The maximum is raised only when a score exceeds it by 8 (P' then stays below 2^12).
+// * O^T[d, row] = V^T P'^T: V's bytes of four keys are interleaved into fragments, P' is transposed with movmatrix.
+//   Splits of one row are joined by a second kernel in split order, so results do not depend on timing.
+#include <cfloat>
+#include <cmath>
+#include <type_traits>
+
+#include "v3g_internal.h"
+#include "v3g_kv.cuh"
+#include "v3g_kv_attn.cuh"
+
+namespace v3g {
+
+constexpr int DEC_WARPS = 4;
+constexpr int DEC_MIN_BLOCKS = 2 * DEC_WARPS;   // blocks of a split at least: fewer leave warps idle
+
+__device__ __forceinline__ uint32_t magic_half2(uint32_t w, uint32_t sel) {   // two code bytes -> fp16 integers
+    const uint32_t v = __byte_perm(w, 0x64646464u, sel);
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&v), __float2half2_rn(1152.f));
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float ex2(float x) {   // 2^x, 0 for -inf
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+template <int BYTES>
+struct Bytes;
+template <>
+struct Bytes<16> {
+    uint32_t w[4];
+    __device__ __forceinline__ void load(const uint8_t *p) {
+        const uint4 u = ldg_stream16(p);
+        w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+    }
+};
+template <>
+struct Bytes<8> {
+    uint32_t w[2];
+    __device__ __forceinline__ void load(const uint8_t *p) {
+        const uint2 u = ldg_stream8(p);
+        w[0] = u.x, w[1] = u.y;
+    }
+};
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 3) k_kv_decode(const __grid_constant__ KvAttnArgs a) {
+    constexpr int ROWS = 8 * NT, NCH = D / 64, VB = D / 8, MT = D / 16, OS = D + 4;
+    __shared__ float sm_m[DEC_WARPS][ROWS], sm_l[DEC_WARPS][ROWS];
+    __shared__ __align__(16) float sm_o[DEC_WARPS][ROWS][OS];
+    griddep_launch();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    int idx = blockIdx.x;
+    const int rt0 = idx % a.row_tiles;
+    idx /= a.row_tiles;
+    const int split = idx % a.splits;
+    idx /= a.splits;
+    const int h = idx % a.c.heads, b = idx / a.c.heads;
+    int first;
+    const int n = a.c.tokens(b, first);
+    if (n * a.group > a.max_rows) return;                                    // the many-row kernel's
+    const int p0 = a.c.end(b) - n;
+    for (int rt = rt0; rt * ROWS < n * a.group; rt += a.row_tiles) {
+        const int r0 = rt * ROWS, rn = min(n * a.group - r0, ROWS);
+        const int pmin = p0 + r0 / a.group, pmax = p0 + (r0 + rn - 1) / a.group;
+        int sb, ws;                                                          // blocks [0, sb) and [ws, ws + nb - sb)
+        const int nb = kv_visible(a, pmin, pmax, KV_BLOCK, sb, ws);
+        const int per = max((nb + a.splits - 1) / a.splits, DEC_MIN_BLOCKS);
+        const int lo = split * per, hi = min(nb, lo + per);
+
+        // queries: row g of each n tile, dims 64 c + 16 t .. + 15
+        uint32_t qf[NT][NCH][8];
+        float qs[NT][2], m[NT][2], l[NT][2];
+        int rpos[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int r = r0 + 8 * nt + g, tok = r / a.group, qh = h * a.group + r - tok * a.group;
+            float x[NCH][16], top = 0.f;
+#pragma unroll
+            for (int c = 0; c < NCH; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (8 * nt + g < rn)
+                        v = kv_load4<T>(static_cast<const T *>(a.q) + (int64_t)(first + tok) * a.q_tok + (int64_t)qh * a.q_head + 64 * c +
+                                            16 * t + 4 * i, a.q_vec);
+                    x[c][4 * i] = v.x, x[c][4 * i + 1] = v.y, x[c][4 * i + 2] = v.z, x[c][4 * i + 3] = v.w;
+                    top = fmaxf(fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+                }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int up = kv_row_exponent<T>(top);
+            const float f = __int_as_float((up + 127) << 23), fi = __int_as_float((127 - up) << 23) * a.scale_log2;
+#pragma unroll
+            for (int c = 0; c < NCH; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) qf[nt][c][i] = pack_half2(x[c][2 * i] * f, x[c][2 * i + 1] * f);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                qs[nt][i] = __shfl_sync(0xffffffffu, fi, (2 * t + i) * 4);
+                const int rr = 8 * nt + 2 * t + i;
+                rpos[nt][i] = rr < rn ? p0 + (r0 + rr) / a.group : -1;
+                m[nt][i] = -INFINITY;
+                l[nt][i] = 0.f;
+            }
+        }
+        float acc[MT][NT][4], ref = 0.f, inv_ref = 0.f;
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[j][nt][i] = 0.f;
+
+        for (int base = lo + warp; base < hi; base += 32 * DEC_WARPS) {
+            // lane i looks up the warp's i-th block from here: page, scales
+            int64_t my_at = -1;
+            float my_ks = 0.f, my_vs = 0.f;
+            {
+                const int vi = base + DEC_WARPS * lane;
+                if (vi < hi) {
+                    const int pos = (vi < sb ? vi : vi - sb + ws) * KV_BLOCK, pg = a.c.page_of(b, pos);
+                    if (pg >= 0) {
+                        my_at = a.c.block(pg, h, pos);
+                        my_ks = a.c.ks[my_at];
+                        my_vs = a.c.vs[my_at];
+                    }
+                }
+            }
+            const int cnt = min(32, (hi - base + DEC_WARPS - 1) / DEC_WARPS);
+            Bytes<16> kr[NCH][2];
+            Bytes<VB> vr[4];
+            auto load_k = [&](int64_t at) {
+                if (at < 0) return;
+                const uint8_t *p = a.c.k + at * (KV_BLOCK * D) + g * D + 16 * t;
+#pragma unroll
+                for (int c = 0; c < NCH; ++c) {
+                    kr[c][0].load(p + 64 * c);
+                    kr[c][1].load(p + 8 * D + 64 * c);
+                }
+            };
+            auto load_v = [&](int64_t at) {
+                if (at < 0) return;
+                const uint8_t *p = a.c.v + at * (KV_BLOCK * D) + 2 * t * D + g * VB;
+                vr[0].load(p);
+                vr[1].load(p + D);
+                vr[2].load(p + 8 * D);
+                vr[3].load(p + 9 * D);
+            };
+            int64_t at = __shfl_sync(0xffffffffu, my_at, 0);
+            load_k(at);
+            load_v(at);
+            for (int it = 0; it < cnt; ++it) {
+                const int64_t next = it + 1 < cnt ? __shfl_sync(0xffffffffu, my_at, it + 1) : -1;
+                const float ks = __shfl_sync(0xffffffffu, my_ks, it), vs = __shfl_sync(0xffffffffu, my_vs, it);
+                if (at < 0) {   // no page: no key is visible
+                    load_k(next);
+                    load_v(next);
+                    at = next;
+                    continue;
+                }
+                float s[NT][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+                for (int c = 0; c < NCH; ++c)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t a0 = magic_half2(kr[c][0].w[i], 0x4140u), a2 = magic_half2(kr[c][0].w[i], 0x4342u);
+                        const uint32_t a1 = magic_half2(kr[c][1].w[i], 0x4140u), a3 = magic_half2(kr[c][1].w[i], 0x4342u);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) mma16816(s[nt], a0, a1, a2, a3, qf[nt][c][2 * i], qf[nt][c][2 * i + 1]);
+                    }
+                load_k(next);
+                const int vi = base + DEC_WARPS * it, j0 = (vi < sb ? vi : vi - sb + ws) * KV_BLOCK;
+                const bool whole = j0 + KV_BLOCK - 1 <= pmin &&
+                                   (a.window == 0 || j0 > pmax - a.window || j0 + KV_BLOCK - 1 < a.n_sink);
+                bool raise = false;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float f = ks * qs[nt][i];
+                        s[nt][i] *= f;
+                        s[nt][2 + i] *= f;
+                        if (!whole) {
+                            if (!kv_sees(a, rpos[nt][i], j0 + g)) s[nt][i] = -INFINITY;
+                            if (!kv_sees(a, rpos[nt][i], j0 + g + 8)) s[nt][2 + i] = -INFINITY;
+                        }
+                        raise |= fmaxf(s[nt][i], s[nt][2 + i]) > m[nt][i] + 8.f;
+                    }
+                if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            float mx = fmaxf(s[nt][i], s[nt][2 + i]);
+                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                            mx = fmaxf(mx, m[nt][i]);
+                            const float al = ex2(m[nt][i] - (mx == -INFINITY ? 0.f : mx));
+                            m[nt][i] = mx;
+                            l[nt][i] *= al;
+#pragma unroll
+                            for (int j = 0; j < MT; ++j) {
+                                acc[j][nt][i] *= al;
+                                acc[j][nt][2 + i] *= al;
+                            }
+                        }
+                }
+                if (vs > 16.f * ref) {   // uniform over the warp
+                    const float nr = kv_scale_ref(vs), al = ref / nr;
+                    ref = nr;
+                    inv_ref = 1.f / nr;
+#pragma unroll
+                    for (int j = 0; j < MT; ++j)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) acc[j][nt][i] *= al;
+                }
+                const float w = vs * inv_ref;
+                uint32_t pb[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float pw[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float mi = m[nt][i & 1];
+                        const float p = ex2(s[nt][i] - (mi == -INFINITY ? 0.f : mi));
+                        l[nt][i & 1] += p;
+                        pw[i] = s[nt][i] == -INFINITY ? 0.f : p * w;   // a hidden key counts for nothing, whatever its block's scale
+                    }
+                    pb[nt][0] = movmatrix(pack_half2(pw[0], pw[1]));
+                    pb[nt][1] = movmatrix(pack_half2(pw[2], pw[3]));
+                }
+#pragma unroll
+                for (int j = 0; j < MT; ++j) {
+                    const uint32_t sel = j & 1 ? 0x7362u : 0x5140u;
+                    const uint32_t x = __byte_perm(vr[0].w[j / 2], vr[1].w[j / 2], sel), y = __byte_perm(vr[2].w[j / 2], vr[3].w[j / 2], sel);
+                    const uint32_t a0 = magic_half2(x, 0x4140u), a1 = magic_half2(x, 0x4342u);
+                    const uint32_t a2 = magic_half2(y, 0x4140u), a3 = magic_half2(y, 0x4342u);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma16816(acc[j][nt], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+                }
+                load_v(next);
+                at = next;
+            }
+        }
+        // join the warps: rows' maxima first, then the scaled accumulators in warp order
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], o);
+                if (g == 0) {
+                    sm_m[warp][8 * nt + 2 * t + i] = m[nt][i];
+                    sm_l[warp][8 * nt + 2 * t + i] = l[nt][i];
+                }
+            }
+        __syncthreads();
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int r = 8 * nt + 2 * t + i;
+                float mx = sm_m[0][r];
+#pragma unroll
+                for (int w = 1; w < DEC_WARPS; ++w) mx = fmaxf(mx, sm_m[w][r]);
+                const float f = exp2f(m[nt][i] - (mx == -INFINITY ? 0.f : mx)) * ref;
+#pragma unroll
+                for (int j = 0; j < MT; ++j)
+                    *reinterpret_cast<float2 *>(&sm_o[warp][r][VB * g + 2 * j]) = make_float2(acc[j][nt][i] * f, acc[j][nt][2 + i] * f);
+            }
+        __syncthreads();
+        for (int i = threadIdx.x; i < rn * (D / 4); i += 32 * DEC_WARPS) {
+            const int r = i / (D / 4), d = i % (D / 4) * 4;
+            float mx = sm_m[0][r], ls = 0.f;
+#pragma unroll
+            for (int w = 1; w < DEC_WARPS; ++w) mx = fmaxf(mx, sm_m[w][r]);
+            const float mu = mx == -INFINITY ? 0.f : mx;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < DEC_WARPS; ++w) {
+                ls += sm_l[w][r] * exp2f(sm_m[w][r] - mu);
+                const float4 x = *reinterpret_cast<const float4 *>(&sm_o[w][r][d]);
+                o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
+            }
+            const int rr = r0 + r, tok = rr / a.group;
+            const int64_t row = (int64_t)(first + tok) * a.c.heads * a.group + h * a.group + rr - tok * a.group;
+            if (a.splits > 1) {
+                if (d == 0) a.part_ml[row * a.splits + split] = make_float2(mx, ls);
+                if (lo < hi) *reinterpret_cast<float4 *>(a.part_o + (row * a.splits + split) * D + d) = o;
+            } else {
+                const float inv = ls == 0.f ? 0.f : 1.f / ls;   // no visible key: zeros
+                kv_store4(static_cast<T *>(a.out) + row * D + d, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+                if (a.lse && d == 0) a.lse[row] = ls == 0.f ? -INFINITY : (mx + log2f(ls)) * 0.69314718f;
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// joins the splits of one row (a warp each, in split order)
+template <typename T, int D>
+__global__ void __launch_bounds__(128) k_kv_join(const __grid_constant__ KvAttnArgs a) {
+    griddep_wait();
+    const int lane = threadIdx.x & 31, qh = a.c.heads * a.group;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (row >= (int64_t)a.c.n_tokens * qh) return;
+    const int tok = (int)(row / qh);
+    int64_t base;
+    const int b = kv_find(a.c.q_start, a.c.batch, a.c.n_tokens, 1, 1, 0, tok, base);
+    int first;
+    const int n = a.c.tokens(b, first);
+    if (tok < first || tok >= first + n || n * a.group > a.max_rows) return;   // no sequence's, or the many-row kernel's
+    float mx = -INFINITY, ls = 0.f;
+    for (int s = lane; s < a.splits; s += 32) mx = fmaxf(mx, a.part_ml[row * a.splits + s].x);
+    mx = warp_max(mx);
+    const float mu = mx == -INFINITY ? 0.f : mx;
+    constexpr int W = D / 32;
+    float o[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) o[i] = 0.f;
+    bool poison = false;
+    for (int s0 = 0; s0 < a.splits; s0 += 32) {
+        float f = 0.f, lw = 0.f;
+        if (s0 + lane < a.splits) {
+            const float2 ml = a.part_ml[row * a.splits + s0 + lane];
+            f = exp2f(ml.x - mu);
+            lw = ml.y * f;
+            if (ml.y != ml.y) poison = true;
+        }
+        ls += warp_sum(lw);
+        const int cnt = min(32, a.splits - s0);
+#pragma unroll 8
+        for (int s = 0; s < cnt; ++s) {
+            const float fs = __shfl_sync(0xffffffffu, f, s);
+            if (fs == 0.f) continue;
+            const float *p = a.part_o + (row * a.splits + s0 + s) * D + W * lane;
+#pragma unroll
+            for (int i = 0; i < W; ++i) o[i] += fs * p[i];
+        }
+    }
+    poison = __any_sync(0xffffffffu, poison);
+    const float inv = poison ? __int_as_float(0x7FC00000) : (ls == 0.f ? 0.f : 1.f / ls);
+    T *out = static_cast<T *>(a.out) + row * D + W * lane;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+        if constexpr (std::is_same<T, __half>::value) out[i] = __float2half_rn(o[i] * inv);
+        else out[i] = __float2bfloat16_rn(o[i] * inv);
+    }
+    if (a.lse && lane == 0) a.lse[row] = poison ? inv : (ls == 0.f ? -INFINITY : (mx + log2f(ls)) * 0.69314718f);
+}
+
+// ----------------------------------------------------------------------------------------------------------- host
+struct KvAttnPlan {
+    int nt, row_tiles, splits;
+    size_t part_o, bytes;
+};
+
+// rows of the longest sequence as the host knows it, and the splits that fill the SMs once: every CTA slot (4 per
+// SM) gets a share of the keys, none less than DEC_MIN_BLOCKS blocks
+static KvAttnPlan kv_plan(const v3g_kv_cache_t *c, const v3g_kv_batch_t *b, uint32_t q_heads, uint32_t max_q, uint32_t max_kv,
+                          uint32_t window, uint32_t n_sink) {
+    KvAttnPlan p = {};
+    const uint64_t group = q_heads / c->n_kv_heads;
+    uint64_t tokens = max_q ? max_q : (b->n_tokens + b->batch - 1) / b->batch;
+    if (tokens == 0) tokens = 1;
+    if (tokens > b->n_tokens) tokens = b->n_tokens;
+    const uint64_t rows = tokens * group;
+    p.nt = rows > 8 ? 2 : 1;
+    uint64_t tiles = (rows + 8 * p.nt - 1) / (8 * p.nt);
+    const uint64_t seq = (uint64_t)b->batch * c->n_kv_heads;
+    while (tiles > 1 && tiles * seq > 0x1000000u) tiles = (tiles + 1) / 2;   // a tile loop serves the rest
+    p.row_tiles = (int)tiles;
+    uint64_t keys = (uint64_t)b->max_pages * c->page;
+    if (max_kv && max_kv < keys) keys = max_kv;
+    if (window && window + n_sink + tokens + 2 * KV_BLOCK < keys) keys = window + n_sink + tokens + 2 * KV_BLOCK;
+    const uint64_t blocks = (keys + KV_BLOCK - 1) / KV_BLOCK, ctas = seq * tiles;
+    uint64_t splits = 148 * 4 / (ctas ? ctas : 1);
+    const uint64_t most = (blocks + DEC_MIN_BLOCKS - 1) / DEC_MIN_BLOCKS;
+    splits = splits > most ? most : splits;
+    splits = splits > 128 ? 128 : splits;
+    p.splits = splits < 1 ? 1 : (int)splits;
+    if (p.splits > 1) {
+        const size_t n = (size_t)b->n_tokens * q_heads * p.splits;
+        p.part_o = (n * sizeof(float2) + 255) & ~(size_t)255;
+        p.bytes = p.part_o + n * c->head_dim * sizeof(float);
+    }
+    return p;
+}
+
+template <typename T, int D>
+static cudaError_t launch_decode(const KvAttnArgs &a, int nt, cudaStream_t st) {
+    const dim3 grid((uint32_t)((uint64_t)a.c.batch * a.c.heads * a.splits * a.row_tiles));
+    cudaError_t e;
+    if (nt == 1) e = launch_k(false, k_kv_decode<T, D, 1>, grid, 32 * DEC_WARPS, 0, st, a);
+    else e = launch_k(false, k_kv_decode<T, D, 2>, grid, 32 * DEC_WARPS, 0, st, a);
+    if (e != cudaSuccess || a.splits == 1) return e;
+    const int64_t rows = (int64_t)a.c.n_tokens * a.c.heads * a.group;
+    return launch_k(true, k_kv_join<T, D>, dim3((uint32_t)((rows + 3) / 4)), 128, 0, st, a);
+}
+
+}  // namespace v3g
+
+using namespace v3g;
+
+static bool attention_shape(const v3g_kv_cache_t *c, const v3g_kv_batch_t *b, uint32_t q_heads) {
+    return c && b && c->n_kv_heads && q_heads && q_heads % c->n_kv_heads == 0 && q_heads <= 65535u && b->batch && b->n_tokens &&
+           b->max_pages && c->page >= 16;
+}
+
+extern "C" size_t v3g_kv_attention_work_size(const v3g_kv_cache_t *cache, const v3g_kv_batch_t *batch, uint32_t n_q_heads,
+                                             uint32_t max_q, uint32_t max_kv, uint32_t window, uint32_t n_sink) {
+    if (!attention_shape(cache, batch, n_q_heads)) return 0;
+    return kv_plan(cache, batch, n_q_heads, max_q, max_kv, window, n_sink).bytes;
+}
+
+extern "C" int v3g_kv_attention(const v3g_kv_cache_t *cache, uint32_t layer, const v3g_kv_batch_t *batch, int dtype, const v3g_rows_t *q,
+                                uint32_t n_q_heads, float scale, uint32_t window, uint32_t n_sink, uint32_t max_q, uint32_t max_kv,
+                                void *out, float *lse, void *dev_work, size_t work_bytes, void *stream) {
+    KvAttnArgs a = {};
+    const int rc = kv_view("v3g_kv_attention", cache, layer, batch, &a.c);
+    if (rc != V3G_OK) return rc;
+    if (dtype != V3G_F16 && dtype != V3G_BF16) return v3g_fail(V3G_E_DTYPE, "v3g_kv_attention: fp16 or bf16 queries");
+    if (n_q_heads == 0 || n_q_heads % cache->n_kv_heads || n_q_heads > 65535u)
+        return v3g_fail(V3G_E_ARG, "v3g_kv_attention: the query heads must be a multiple of the KV heads");
+    if (!std::isfinite(scale)) return v3g_fail(V3G_E_ARG, "v3g_kv_attention: scale must be finite");
+    if (batch->batch == 0 || batch->n_tokens == 0) return V3G_OK;
+    if (!q || !q->data || !out) return v3g_fail(V3G_E_ARG, "v3g_kv_attention: null pointer");
+    if (reinterpret_cast<uintptr_t>(q->data) % 2 || reinterpret_cast<uintptr_t>(out) % 16 || reinterpret_cast<uintptr_t>(lse) % 4)
+        return v3g_fail(V3G_E_ALIGN, "v3g_kv_attention: out needs 16-byte alignment");
+    if ((uint64_t)batch->n_tokens * n_q_heads > 0x7FFFFFFFu) return v3g_fail(V3G_E_LIMIT, "v3g_kv_attention: too many query rows");
+    if (window > 0x40000000u) window = 0;   // past every position
+    if (n_sink > 0x40000000u) n_sink = 0x40000000u;
+    const KvAttnPlan p = kv_plan(cache, batch, n_q_heads, max_q, max_kv, window, n_sink);
+    if (p.bytes && (!dev_work || work_bytes < p.bytes)) return v3g_fail(V3G_E_SIZE, "v3g_kv_attention: workspace too small");
+    if (p.bytes && reinterpret_cast<uintptr_t>(dev_work) % 256) return v3g_fail(V3G_E_ALIGN, "v3g_kv_attention: the workspace needs 256-byte alignment");
+    if ((uint64_t)batch->batch * cache->n_kv_heads * p.splits * p.row_tiles > 0x7FFFFFFFu)
+        return v3g_fail(V3G_E_LIMIT, "v3g_kv_attention: too many sequences and heads");
+    a.q = q->data;
+    a.q_tok = q->tok_stride;
+    a.q_head = q->head_stride;
+    a.q_vec = reinterpret_cast<uintptr_t>(q->data) % 8 == 0 && q->tok_stride % 4 == 0 && q->head_stride % 4 == 0;
+    a.group = (int)(n_q_heads / cache->n_kv_heads);
+    a.scale_log2 = scale * 1.44269504f;
+    a.window = (int)window;
+    a.n_sink = (int)n_sink;
+    a.out = out;
+    a.lse = lse;
+    a.splits = p.splits;
+    a.row_tiles = p.row_tiles;
+    a.max_rows = 0x7FFFFFFF;
+    a.part_ml = static_cast<float2 *>(dev_work);
+    a.part_o = reinterpret_cast<float *>(static_cast<uint8_t *>(dev_work) + p.part_o);
+    const cudaStream_t st = (cudaStream_t)stream;
+    cudaError_t e;
+    if (dtype == V3G_F16) e = cache->head_dim == 64 ? launch_decode<__half, 64>(a, p.nt, st) : launch_decode<__half, 128>(a, p.nt, st);
+    else e = cache->head_dim == 64 ? launch_decode<__nv_bfloat16, 64>(a, p.nt, st) : launch_decode<__nv_bfloat16, 128>(a, p.nt, st);
+    return e == cudaSuccess ? V3G_OK : v3g_fail(V3G_E_CUDA, std::string("v3g_kv_attention: ") + cudaGetErrorString(e));
+}

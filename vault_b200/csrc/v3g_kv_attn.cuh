@@ -1,0 +1,62 @@
+// What the attention kernels over the paged 8-bit cache share: arguments, visibility, operand scaling.
+#pragma once
+#include <type_traits>
+
+#include "v3g_kv.cuh"
+
+namespace v3g {
+
+struct KvAttnArgs {
+    KvView c;
+    const void *q;
+    int64_t q_tok, q_head;     // strides in elements
+    bool q_vec;                // four-element loads of q are aligned
+    int group;                 // query heads per KV head
+    float scale_log2;          // scale x log2(e)
+    int window, n_sink;        // window 0: every earlier key
+    void *out;                 // [tokens][query heads][D]
+    float *lse;                // [tokens][query heads], or null
+    int splits, row_tiles;
+    int max_rows;              // sequences with more rows (tokens x group) are another kernel's
+    float2 *part_ml;           // [row][split] maximum (log2 units) and sum
+    float *part_o;             // [row][split][D]
+};
+
+// a row at position p sees key j; negative positions see nothing
+__device__ __forceinline__ bool kv_sees(const KvAttnArgs &a, int p, int j) {
+    return j <= p && (a.window == 0 || j > p - a.window || j < a.n_sink);
+}
+
+// Key blocks of `unit` keys that rows at positions pmin..pmax can see: [0, sinks) and [first, first + count - sinks);
+// returns count.  Keys past the page table's reach do not exist.
+__device__ __forceinline__ int kv_visible(const KvAttnArgs &a, int pmin, int pmax, int unit, int &sinks, int &first) {
+    const int64_t cap = (int64_t)a.c.max_pages << a.c.page_shift;
+    const int end = (int)min((int64_t)pmax + 1, cap);
+    sinks = first = 0;
+    if (end <= 0) return 0;
+    const int last = (end + unit - 1) / unit;
+    if (a.window == 0) return last;
+    first = min(max(pmin - a.window + 1, 0) / unit, last);
+    sinks = (min(a.n_sink, end) + unit - 1) / unit;
+    if (first <= sinks) {
+        sinks = first = 0;
+        return last;
+    }
+    return sinks + last - first;
+}
+
+// power of two that brings a row of largest magnitude top into fp16's range without losing bits (fp16 rows: 1)
+template <typename T>
+__device__ __forceinline__ int kv_row_exponent(float top) {
+    if constexpr (sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value) return 0;
+    const int e = (int)((__float_as_uint(top) >> 23) & 255u) - 127;
+    return min(13 - e, 100);
+}
+
+// the power of two at or above a V scale, inside a range whose inverse is a normal number
+__device__ __forceinline__ float kv_scale_ref(float vs) {
+    const uint32_t e = ((__float_as_uint(vs) + 0x7FFFFFu) >> 23) & 255u;
+    return __uint_as_float(min(max(e, 7u), 247u) << 23);
+}
+
+}  // namespace v3g
