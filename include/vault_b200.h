@@ -268,7 +268,7 @@ V3G_API int v3g_argmax_noalloc(const float *dev_logits, uint32_t rows, uint32_t 
  *   k_scale, v_scale float  [n_layers][n_pages][n_kv_heads][page / 16]
  * head_dim 64 or 128; page 16, 32, 64, 128 or 256.  A scale below 2^-120 is stored as zero; a block that was given a
  * NaN or an infinity has the scale NaN and reads as NaN.  The arrays need no initial content: a block's first token
- * starts its scale.
+ * starts its scale.  Scales are not negative.
  *
  * A batch names its sequences by device arrays.  Token i of sequence b (packed index q_start[b] + i, of
  * n_b = q_start[b + 1] - q_start[b]) stands at position kv_len[b] - n_b + i, so kv_len counts the batch's tokens too
@@ -316,13 +316,14 @@ V3G_API int v3g_kv_read(const v3g_kv_cache_t *cache, uint32_t layer, uint32_t n_
  * heads h n_q_heads / n_kv_heads .. share KV head h.  A token at position p sees keys j <= p with j > p - window or
  * j < n_sink (window 0: all).  A row that sees no key gives zeros and lse -inf.  max_q and max_kv are the largest token
  * count and length of a sequence as far as the host knows them (0: unknown): they choose kernels and splits, never
- * results' validity.  dev_work: v3g_kv_attention_work_size bytes of device memory, 256-byte aligned, with no content
+ * results' validity.  *dev_status (may be NULL) gets V3G_STATUS_TIMEOUT if a bounded wait inside a kernel ran out (the
+ * output is then invalid).  dev_work: v3g_kv_attention_work_size bytes of device memory, 256-byte aligned, with no content
  * kept between calls. */
 V3G_API size_t v3g_kv_attention_work_size(const v3g_kv_cache_t *cache, const v3g_kv_batch_t *batch, uint32_t n_q_heads,
                                           uint32_t max_q, uint32_t max_kv, uint32_t window, uint32_t n_sink);
 V3G_API int v3g_kv_attention(const v3g_kv_cache_t *cache, uint32_t layer, const v3g_kv_batch_t *batch, int dtype, const v3g_rows_t *q,
                              uint32_t n_q_heads, float scale, uint32_t window, uint32_t n_sink, uint32_t max_q, uint32_t max_kv,
-                             void *out, float *lse, void *dev_work, size_t work_bytes, void *stream);
+                             void *out, float *lse, int32_t *dev_status, void *dev_work, size_t work_bytes, void *stream);
 /* Reorder the caches of groups of `beams` consecutive sequences (1..32; the sequences of a group have equal kv_len):
  * row g * beams + j continues beam parents[g * beams + j] of its group.  table_out (another buffer) receives the new
  * page table: the parent's entries for full pages, dst_page (NULL: the row's own entry) for the page still being

@@ -37,7 +37,7 @@ def append(c=None, b=None, layer=0, dtype=1, k=None, v=None, q=None, heads=0, q_
 
 def attention(c=None, b=None, layer=0, dtype=1, q=None, heads=4, scale=0.1, out=P, lse=None, work=P, size=1 << 40, max_q=0, max_kv=0):
     return _lib.lib().v3g_kv_attention(c or cache(), layer, b or batch(), dtype, q or rows(), heads, scale, 0, 0, max_q, max_kv, out, lse,
-                                       work, size, None)
+                                       None, work, size, None)
 
 
 @pytest.mark.parametrize("code,change", [(E_ARG, dict(k=None)), (E_ARG, dict(v_scale=None)), (E_UNSUPPORTED, dict(head_dim=96)),

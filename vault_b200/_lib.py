@@ -109,7 +109,7 @@ _SIGS = {
     "v3g_kv_attention_work_size": (C.c_size_t, [C.POINTER(KVCache), C.POINTER(KVBatch), C.c_uint32, C.c_uint32, C.c_uint32,
                                                 C.c_uint32, C.c_uint32]),
     "v3g_kv_attention": (C.c_int, [C.POINTER(KVCache), C.c_uint32, C.POINTER(KVBatch), C.c_int, C.POINTER(Rows), C.c_uint32, C.c_float,
-                                   C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, _P, _P, _P, C.c_size_t, _P]),
+                                   C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, _P, _P, _P, _P, C.c_size_t, _P]),
     "v3g_kv_reorder": (C.c_int, [C.POINTER(KVCache), C.POINTER(KVBatch), C.c_uint32, _P, _P, _P, C.c_uint64, _P, _P]),
     "v3g_beam_select_work_size": (C.c_size_t, [C.c_uint32, C.c_uint32, C.c_uint32]),
     "v3g_beam_select": (C.c_int, [_P, C.c_int, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint64, _P, _P, C.c_int32, _P, _P, _P, _P, _P,

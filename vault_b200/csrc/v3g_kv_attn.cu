@@ -317,8 +317,8 @@ __global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 3) k_kv_decode(c
             const int rr = r0 + r, tok = rr / a.group;
             const int64_t row = (int64_t)(first + tok) * a.c.heads * a.group + h * a.group + rr - tok * a.group;
             if (a.splits > 1) {
-                if (d == 0) a.part_ml[row * a.splits + split] = make_float2(mx, ls);
-                if (lo < hi) *reinterpret_cast<float4 *>(a.part_o + (row * a.splits + split) * D + d) = o;
+                if (d == 0) a.part_ml[row * a.part_stride + split] = make_float2(mx, ls);
+                if (lo < hi) *reinterpret_cast<float4 *>(a.part_o + (row * a.part_stride + split) * D + d) = o;
             } else {
                 const float inv = ls == 0.f ? 0.f : 1.f / ls;   // no visible key: zeros
                 kv_store4(static_cast<T *>(a.out) + row * D + d, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
@@ -341,9 +341,12 @@ __global__ void __launch_bounds__(128) k_kv_join(const __grid_constant__ KvAttnA
     const int b = kv_find(a.c.q_start, a.c.batch, a.c.n_tokens, 1, 1, 0, tok, base);
     int first;
     const int n = a.c.tokens(b, first);
-    if (tok < first || tok >= first + n || n * a.group > a.max_rows) return;   // no sequence's, or the many-row kernel's
+    if (tok < first || tok >= first + n) return;   // no sequence's
+    const int splits = n * a.group > a.max_rows ? a.pf_splits : a.splits;
+    if (splits <= 1) return;                       // the row is finished
+    const float2 *ml = a.part_ml + row * a.part_stride;
     float mx = -INFINITY, ls = 0.f;
-    for (int s = lane; s < a.splits; s += 32) mx = fmaxf(mx, a.part_ml[row * a.splits + s].x);
+    for (int s = lane; s < splits; s += 32) mx = fmaxf(mx, ml[s].x);
     mx = warp_max(mx);
     const float mu = mx == -INFINITY ? 0.f : mx;
     constexpr int W = D / 32;
@@ -351,21 +354,21 @@ __global__ void __launch_bounds__(128) k_kv_join(const __grid_constant__ KvAttnA
 #pragma unroll
     for (int i = 0; i < W; ++i) o[i] = 0.f;
     bool poison = false;
-    for (int s0 = 0; s0 < a.splits; s0 += 32) {
+    for (int s0 = 0; s0 < splits; s0 += 32) {
         float f = 0.f, lw = 0.f;
-        if (s0 + lane < a.splits) {
-            const float2 ml = a.part_ml[row * a.splits + s0 + lane];
-            f = exp2f(ml.x - mu);
-            lw = ml.y * f;
-            if (ml.y != ml.y) poison = true;
+        if (s0 + lane < splits) {
+            const float2 x = ml[s0 + lane];
+            f = exp2f(x.x - mu);
+            lw = x.y * f;
+            if (x.y != x.y) poison = true;
         }
         ls += warp_sum(lw);
-        const int cnt = min(32, a.splits - s0);
+        const int cnt = min(32, splits - s0);
 #pragma unroll 8
         for (int s = 0; s < cnt; ++s) {
             const float fs = __shfl_sync(0xffffffffu, f, s);
             if (fs == 0.f) continue;
-            const float *p = a.part_o + (row * a.splits + s0 + s) * D + W * lane;
+            const float *p = a.part_o + (row * a.part_stride + s0 + s) * D + W * lane;
 #pragma unroll
             for (int i = 0; i < W; ++i) o[i] += fs * p[i];
         }
@@ -382,37 +385,63 @@ __global__ void __launch_bounds__(128) k_kv_join(const __grid_constant__ KvAttnA
 }
 
 // ----------------------------------------------------------------------------------------------------------- host
+// Sequences of at most this many rows go to the few-row kernel when a batch has longer ones too.
+constexpr int DEC_MAX_ROWS = 64;
+constexpr size_t PART_BYTES_MAX = (size_t)64 << 20;   // partial results stay in L2
+
 struct KvAttnPlan {
-    int nt, row_tiles, splits;
+    bool few, many;              // kernels that run
+    int nt, row_tiles, splits, pf_splits, part_stride, max_rows;
     size_t part_o, bytes;
 };
 
-// rows of the longest sequence as the host knows it, and the splits that fill the SMs once: every CTA slot (4 per
-// SM) gets a share of the keys, none less than DEC_MIN_BLOCKS blocks
 static KvAttnPlan kv_plan(const v3g_kv_cache_t *c, const v3g_kv_batch_t *b, uint32_t q_heads, uint32_t max_q, uint32_t max_kv,
                           uint32_t window, uint32_t n_sink) {
     KvAttnPlan p = {};
-    const uint64_t group = q_heads / c->n_kv_heads;
-    uint64_t tokens = max_q ? max_q : (b->n_tokens + b->batch - 1) / b->batch;
-    if (tokens == 0) tokens = 1;
-    if (tokens > b->n_tokens) tokens = b->n_tokens;
-    const uint64_t rows = tokens * group;
-    p.nt = rows > 8 ? 2 : 1;
-    uint64_t tiles = (rows + 8 * p.nt - 1) / (8 * p.nt);
-    const uint64_t seq = (uint64_t)b->batch * c->n_kv_heads;
-    while (tiles > 1 && tiles * seq > 0x1000000u) tiles = (tiles + 1) / 2;   // a tile loop serves the rest
-    p.row_tiles = (int)tiles;
+    const uint64_t group = q_heads / c->n_kv_heads, seq = (uint64_t)b->batch * c->n_kv_heads;
+    const uint64_t mean = (b->n_tokens + b->batch - 1) / b->batch;
+    uint64_t longest = max_q && max_q < b->n_tokens ? max_q : b->n_tokens;   // as the host knows it: a hint
+    if (longest < mean) longest = mean;
+    p.few = true;
+    p.max_rows = 0x7FFFFFFF;
+    if (longest * group > DEC_MAX_ROWS) {
+        p.many = true;
+        p.few = longest * b->batch > b->n_tokens;                            // else all are of that length
+        p.max_rows = p.few ? DEC_MAX_ROWS : 0;
+    }
     uint64_t keys = (uint64_t)b->max_pages * c->page;
     if (max_kv && max_kv < keys) keys = max_kv;
-    if (window && window + n_sink + tokens + 2 * KV_BLOCK < keys) keys = window + n_sink + tokens + 2 * KV_BLOCK;
-    const uint64_t blocks = (keys + KV_BLOCK - 1) / KV_BLOCK, ctas = seq * tiles;
-    uint64_t splits = 148 * 4 / (ctas ? ctas : 1);
-    const uint64_t most = (blocks + DEC_MIN_BLOCKS - 1) / DEC_MIN_BLOCKS;
-    splits = splits > most ? most : splits;
-    splits = splits > 128 ? 128 : splits;
-    p.splits = splits < 1 ? 1 : (int)splits;
-    if (p.splits > 1) {
-        const size_t n = (size_t)b->n_tokens * q_heads * p.splits;
+    // splits that fill the SMs once: 4 CTA slots per SM and DEC_MIN_BLOCKS blocks a share for few rows
+    auto seen = [&](uint64_t tokens) {
+        const uint64_t w = (uint64_t)window + n_sink + tokens + 2 * KV_BLOCK;
+        return window && w < keys ? w : keys;
+    };
+    const uint64_t room = PART_BYTES_MAX / (((uint64_t)b->n_tokens * q_heads) * (c->head_dim + 2) * 4);
+    p.splits = p.pf_splits = p.row_tiles = 1;
+    if (p.few) {
+        const uint64_t tokens = p.many ? (longest * group < DEC_MAX_ROWS ? longest : (DEC_MAX_ROWS + group - 1) / group) : longest;
+        const uint64_t rows = tokens * group;
+        p.nt = rows > 8 ? 2 : 1;
+        uint64_t tiles = (rows + 8 * p.nt - 1) / (8 * p.nt);
+        while (tiles > 1 && tiles * seq > 0x1000000u) tiles = (tiles + 1) / 2;   // a tile loop serves the rest
+        p.row_tiles = (int)tiles;
+        const uint64_t blocks = (seen(tokens) + KV_BLOCK - 1) / KV_BLOCK, most = (blocks + DEC_MIN_BLOCKS - 1) / DEC_MIN_BLOCKS;
+        uint64_t s = 148 * 4 / (seq * tiles);
+        s = s > most ? most : s;
+        s = s > room ? room : s;
+        p.splits = s < 1 ? 1 : (s > 128 ? 128 : (int)s);
+    }
+    if (p.many) {
+        const uint64_t ctas = (longest * group + 255) / 256 * c->n_kv_heads * (p.few ? 1 : b->batch);
+        const uint64_t most = (seen(longest) + 1023) / 1024;                    // eight key tiles a share at least
+        uint64_t s = 148 / ctas;
+        s = s > most ? most : s;
+        s = s > room ? room : s;
+        p.pf_splits = s < 1 ? 1 : (s > 128 ? 128 : (int)s);
+    }
+    p.part_stride = p.splits > p.pf_splits ? p.splits : p.pf_splits;
+    if (p.part_stride > 1) {
+        const size_t n = (size_t)b->n_tokens * q_heads * p.part_stride;
         p.part_o = (n * sizeof(float2) + 255) & ~(size_t)255;
         p.bytes = p.part_o + n * c->head_dim * sizeof(float);
     }
@@ -420,12 +449,15 @@ static KvAttnPlan kv_plan(const v3g_kv_cache_t *c, const v3g_kv_batch_t *b, uint
 }
 
 template <typename T, int D>
-static cudaError_t launch_decode(const KvAttnArgs &a, int nt, cudaStream_t st) {
-    const dim3 grid((uint32_t)((uint64_t)a.c.batch * a.c.heads * a.splits * a.row_tiles));
-    cudaError_t e;
-    if (nt == 1) e = launch_k(false, k_kv_decode<T, D, 1>, grid, 32 * DEC_WARPS, 0, st, a);
-    else e = launch_k(false, k_kv_decode<T, D, 2>, grid, 32 * DEC_WARPS, 0, st, a);
-    if (e != cudaSuccess || a.splits == 1) return e;
+static cudaError_t launch_attention_kernels(const KvAttnArgs &a, const KvAttnPlan &p, int dtype, cudaStream_t st) {
+    cudaError_t e = cudaSuccess;
+    if (p.many) e = launch_kv_prefill(a, dtype, D, a.max_rows + 1, st);
+    if (e == cudaSuccess && p.few) {
+        const dim3 grid((uint32_t)((uint64_t)a.c.batch * a.c.heads * a.splits * a.row_tiles));
+        if (p.nt == 1) e = launch_k(false, k_kv_decode<T, D, 1>, grid, 32 * DEC_WARPS, 0, st, a);
+        else e = launch_k(false, k_kv_decode<T, D, 2>, grid, 32 * DEC_WARPS, 0, st, a);
+    }
+    if (e != cudaSuccess || a.part_stride == 1) return e;
     const int64_t rows = (int64_t)a.c.n_tokens * a.c.heads * a.group;
     return launch_k(true, k_kv_join<T, D>, dim3((uint32_t)((rows + 3) / 4)), 128, 0, st, a);
 }
@@ -447,7 +479,7 @@ extern "C" size_t v3g_kv_attention_work_size(const v3g_kv_cache_t *cache, const 
 
 extern "C" int v3g_kv_attention(const v3g_kv_cache_t *cache, uint32_t layer, const v3g_kv_batch_t *batch, int dtype, const v3g_rows_t *q,
                                 uint32_t n_q_heads, float scale, uint32_t window, uint32_t n_sink, uint32_t max_q, uint32_t max_kv,
-                                void *out, float *lse, void *dev_work, size_t work_bytes, void *stream) {
+                                void *out, float *lse, int32_t *dev_status, void *dev_work, size_t work_bytes, void *stream) {
     KvAttnArgs a = {};
     const int rc = kv_view("v3g_kv_attention", cache, layer, batch, &a.c);
     if (rc != V3G_OK) return rc;
@@ -457,7 +489,8 @@ extern "C" int v3g_kv_attention(const v3g_kv_cache_t *cache, uint32_t layer, con
     if (!std::isfinite(scale)) return v3g_fail(V3G_E_ARG, "v3g_kv_attention: scale must be finite");
     if (batch->batch == 0 || batch->n_tokens == 0) return V3G_OK;
     if (!q || !q->data || !out) return v3g_fail(V3G_E_ARG, "v3g_kv_attention: null pointer");
-    if (reinterpret_cast<uintptr_t>(q->data) % 2 || reinterpret_cast<uintptr_t>(out) % 16 || reinterpret_cast<uintptr_t>(lse) % 4)
+    if (reinterpret_cast<uintptr_t>(q->data) % 2 || reinterpret_cast<uintptr_t>(out) % 16 || reinterpret_cast<uintptr_t>(lse) % 4 ||
+        reinterpret_cast<uintptr_t>(dev_status) % 4)
         return v3g_fail(V3G_E_ALIGN, "v3g_kv_attention: out needs 16-byte alignment");
     if ((uint64_t)batch->n_tokens * n_q_heads > 0x7FFFFFFFu) return v3g_fail(V3G_E_LIMIT, "v3g_kv_attention: too many query rows");
     if (window > 0x40000000u) window = 0;   // past every position
@@ -479,12 +512,18 @@ extern "C" int v3g_kv_attention(const v3g_kv_cache_t *cache, uint32_t layer, con
     a.lse = lse;
     a.splits = p.splits;
     a.row_tiles = p.row_tiles;
-    a.max_rows = 0x7FFFFFFF;
+    a.max_rows = p.max_rows;
+    a.pf_splits = p.pf_splits;
+    a.part_stride = p.part_stride;
+    a.status = dev_status;
     a.part_ml = static_cast<float2 *>(dev_work);
     a.part_o = reinterpret_cast<float *>(static_cast<uint8_t *>(dev_work) + p.part_o);
     const cudaStream_t st = (cudaStream_t)stream;
     cudaError_t e;
-    if (dtype == V3G_F16) e = cache->head_dim == 64 ? launch_decode<__half, 64>(a, p.nt, st) : launch_decode<__half, 128>(a, p.nt, st);
-    else e = cache->head_dim == 64 ? launch_decode<__nv_bfloat16, 64>(a, p.nt, st) : launch_decode<__nv_bfloat16, 128>(a, p.nt, st);
+    if (dtype == V3G_F16)
+        e = cache->head_dim == 64 ? launch_attention_kernels<__half, 64>(a, p, dtype, st) : launch_attention_kernels<__half, 128>(a, p, dtype, st);
+    else
+        e = cache->head_dim == 64 ? launch_attention_kernels<__nv_bfloat16, 64>(a, p, dtype, st)
+                                  : launch_attention_kernels<__nv_bfloat16, 128>(a, p, dtype, st);
     return e == cudaSuccess ? V3G_OK : v3g_fail(V3G_E_CUDA, std::string("v3g_kv_attention: ") + cudaGetErrorString(e));
 }

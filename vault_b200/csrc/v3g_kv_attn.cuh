@@ -16,10 +16,14 @@ struct KvAttnArgs {
     int window, n_sink;        // window 0: every earlier key
     void *out;                 // [tokens][query heads][D]
     float *lse;                // [tokens][query heads], or null
-    int splits, row_tiles;
-    int max_rows;              // sequences with more rows (tokens x group) are another kernel's
-    float2 *part_ml;           // [row][split] maximum (log2 units) and sum
-    float *part_o;             // [row][split][D]
+    // sequences of at most max_rows rows (tokens x group) are the few-row kernel's, the others the many-row kernel's
+    int max_rows;
+    int splits, row_tiles;     // few rows: key shares, row tiles in the grid
+    int pf_splits;             // many rows: key shares
+    int part_stride;           // shares that a row has room for
+    float2 *part_ml;           // [row][share] maximum (log2 units) and sum
+    float *part_o;             // [row][share][D]
+    int32_t *status;           // V3G_STATUS_TIMEOUT when a bounded wait ran out, or null
 };
 
 // a row at position p sees key j; negative positions see nothing
@@ -58,5 +62,8 @@ __device__ __forceinline__ float kv_scale_ref(float vs) {
     const uint32_t e = ((__float_as_uint(vs) + 0x7FFFFFu) >> 23) & 255u;
     return __uint_as_float(min(max(e, 7u), 247u) << 23);
 }
+
+// the many-row kernel over every sequence of at least min_rows rows (v3g_kv_prefill.cu)
+cudaError_t launch_kv_prefill(const KvAttnArgs &a, int dtype, int head_dim, int min_rows, cudaStream_t st);
 
 }  // namespace v3g

@@ -91,8 +91,9 @@ class PagedKVCache:
         bits = int(self.status_word.item())
         if bits:
             self.status_word.zero_()
-            raise RuntimeError(f"device status bits {bits:#x}: a token without a page or a rotation row was dropped, or a "
-                               "beam's parent or page does not exist")
+            raise RuntimeError(f"device status bits {bits:#x}: " +
+                               ("a token without a page or a rotation row was dropped, or a beam's parent or page does not exist"
+                                if bits & _lib.V3G_STATUS_BOUNDS else "a kernel gave up waiting, its output is invalid"))
 
     # ---- arguments
     def _stream(self) -> int:
@@ -198,7 +199,7 @@ class PagedKVCache:
             work = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
             self._call(L.v3g_kv_attention, "v3g_kv_attention", self._ref, self._layer(layer), batch, dt, qr, heads,
                        self.head_dim ** -0.5 if scale is None else float(scale), window, n_sink, max_q, max_kv, out.data_ptr(),
-                       None if lse is None else lse.data_ptr(), None if work is None else work.data_ptr(), size)
+                       None if lse is None else lse.data_ptr(), self.status_word.data_ptr(), None if work is None else work.data_ptr(), size)
         return (out, lse) if return_lse else out
 
     def read(self, page_table: torch.Tensor, first: torch.Tensor, kv_len: torch.Tensor, row_start: torch.Tensor, n_rows: int,
