@@ -9,12 +9,16 @@
 //   warps 8-11       converters: codes from their pages to fp16 operands (exact: permute to 1024 + c, minus 1152), two
 //                    stages each of K and V.  Both are stored [key][d] with the 128-byte swizzle, K read as a K-major
 //                    operand, V as an MN-major one, so neither is transposed
-//   warp 12          tensor memory and the MMAs: S = Q K^T (128 x 128), O += P' V (P' from tensor memory)
+//   warps 12, 13     the MMAs of tile 0 / 1: S = Q K^T, O += P' V (P' from tensor memory); warp 12 holds tensor memory
+//   warp 14          the tiles' pages and scales
 //
-// The two tiles alternate, so one tile's softmax runs under the other's MMAs: in issue order PV0(j), QK0(j+1), PV1(j),
-// QK1(j+1).  tcgen05 operations of one thread run in order, so QK(j+1) may overwrite P'(j), and a full S(j) says that
-// PV(j-1) is done: a row whose maximum grew by more than 8 (else its old one stays; P' is then below 2^12) rescales its
-// O in tensor memory right there.
+// A step is 64 keys of one tile: S = Q K^T into one of the tile's two score buffers, softmax, P' over the same columns,
+// O += P' V.  A tile's issuer runs PV(u), QK(u + 2): while these run, the tile's softmax works on the other buffer, so neither
+// waits for a round trip.  tcgen05 operations of one thread run in order, so QK(u + 2) may overwrite P'(u).  Each tile has
+// an issuer in another quarter of the SM, because an issuing warp slows the softmax warps of its quarter (one issuer for
+// both tiles: 718 us for the 8,192-token prompt, 32/8 heads; two: 693).  The offset m of a row's exponents is its maximum when m was set, plus 3; it stays until a score passes it
+// by 11 (P' is then below 2^15).  Only then the warp rescales its O in tensor memory, after a wait for PV(u - 1): with a
+// margin of 8 from the maximum itself, some row of the 32 did so at every second step on scores of standard deviation 3.
 //
 // K scales multiply the scores; a V scale vs enters the exponent, P' = 2^(s - m + log2(vs / ref)), ref a power of two
 // that follows the largest vs, and the row sum takes P' ref / vs.  vs / ref is held at or above 2^-40, where P' rounds to
@@ -30,19 +34,23 @@
 namespace v3g {
 
 constexpr int PF_ROWS = 256, PF_KEYS = 128, PF_THREADS = 512;
-constexpr int PF_SCALES = 4;   // ring of scale sets: the converters are at most two tiles ahead of the softmax
+// Ring of the tiles' places and scales.  Its writer is at most PF_AHEAD tiles past the converters' loads; they load tile t + 1
+// after tile t - 2's PV, which needed every softmax warp to be through with that tile's scales, so a slot is written again
+// only after its last reader.
+constexpr int PF_RING = 8, PF_AHEAD = 5;
 
 template <int D>
 struct PfSmem {
     static constexpr int OP = 128 * D * 2;                      // one 128 x D fp16 operand
-    static constexpr int Q = 0, K = 2 * OP, V = 4 * OP, SC = 6 * OP, BAR = SC + PF_SCALES * 128, END = BAR + 192, BYTES = END + 1024;
+    static constexpr int Q = 0, K = 2 * OP, V = 4 * OP, SC = 6 * OP, BAR = SC + PF_RING * 192, END = BAR + 384, BYTES = END + 1024;
 };
 
-struct PfScales {   // of one key tile: per 16-key block
+struct alignas(16) PfPlaces {   // of one key tile, per 16-key block
     float ks[8], lv[8], iv[8];   // K scale, log2 of the V scale, its inverse
-    uint32_t valid, pad[7];      // bit i: block i has a page
+    int64_t at[8];               // index of the block in the layer
+    uint32_t valid, pad[7];      // bit i: block i has a page and some row sees it
 };
-static_assert(sizeof(PfScales) == 128, "scale ring slot");
+static_assert(sizeof(PfPlaces) == 192, "ring slot");
 
 #define TC_REGS8(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7])
 #define TC_IN8(r, o) "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7])
@@ -82,6 +90,28 @@ __device__ __forceinline__ uint64_t v_desc(uint32_t saddr) {
     return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(16384u >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | ((uint64_t)1u << 46) |
            ((uint64_t)2u << 61);
 }
+__device__ __forceinline__ bool elect_one() {   // one lane of the converged warp
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+    return p;
+}
+// two fp32 operations at once
+__device__ __forceinline__ uint64_t f2_pack(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void f2_unpack(uint64_t x, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x)); }
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 __device__ __forceinline__ float pf_ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -106,6 +136,20 @@ __device__ __forceinline__ uint4 pf_convert8(uint32_t a, uint32_t b) {   // eigh
 
 // a whole warp's bounded wait: one answer for all its lanes
 __device__ __forceinline__ bool pf_wait(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity)); }
+// The same for warps that are ahead of their consumers: they sleep between looks and leave their issue slots to others.
+__device__ __forceinline__ bool pf_wait_idle(uint32_t bar, uint32_t parity) {
+    for (uint32_t i = 0; i < tc::WAIT_LIMIT; ++i) {
+        uint32_t done;
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+            : "=r"(done)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (__all_sync(0xffffffffu, done)) return true;
+        __nanosleep(40);
+    }
+    return false;
+}
 
 // visible keys of 32 consecutive ones from kb, as a bit mask, for a row at position p
 __device__ __forceinline__ uint32_t pf_mask(const KvAttnArgs &a, int p, int kb, uint32_t pages) {
@@ -146,37 +190,46 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
     auto KEMPTY = [&](int s) { return bars + 8u * (3 + s); };
     auto VFULL = [&](int s) { return bars + 8u * (5 + s); };
     auto VEMPTY = [&](int s) { return bars + 8u * (7 + s); };
-    auto SFULL = [&](int t) { return bars + 8u * (9 + t); };
-    auto PFULL = [&](int t) { return bars + 8u * (11 + t); };
-    auto OFULL = [&](int t) { return bars + 8u * (13 + t); };
-    auto SCFULL = [&](int s) { return bars + 8u * (15 + s); };
-    const uint32_t DRAIN = bars + 8u * 19;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + SM::BAR + 160);
-    PfScales *scales = reinterpret_cast<PfScales *>(smem + SM::SC);
+    auto SFULL = [&](int t, int half) { return bars + 8u * (9 + 2 * t + half); };
+    auto PFULL = [&](int t, int half) { return bars + 8u * (13 + 2 * t + half); };
+    auto ODONE = [&](int t) { return bars + 8u * (17 + t); };
+    auto OFULL = [&](int t) { return bars + 8u * (19 + t); };
+    auto ATFULL = [&](int s) { return bars + 8u * (21 + s); };
+    auto ATEMPTY = [&](int s) { return bars + 8u * (29 + s); };
+    const uint32_t DRAIN = bars + 8u * 37, GO = bars + 8u * 38;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + SM::BAR + 8 * 39);
+    PfPlaces *places = reinterpret_cast<PfPlaces *>(smem + SM::SC);
     if (threadIdx.x == 0) {
         tc::mbar_init(QFULL, 4 * tiles);
         for (int s = 0; s < 2; ++s) {
             tc::mbar_init(KFULL(s), 4);
-            tc::mbar_init(KEMPTY(s), 1);
+            tc::mbar_init(KEMPTY(s), tiles);
             tc::mbar_init(VFULL(s), 4);
-            tc::mbar_init(VEMPTY(s), 1);
-            tc::mbar_init(SFULL(s), 1);
-            tc::mbar_init(PFULL(s), 4);
+            tc::mbar_init(VEMPTY(s), tiles);
+            for (int half = 0; half < 2; ++half) {
+                tc::mbar_init(SFULL(s, half), 1);
+                tc::mbar_init(PFULL(s, half), 4);
+            }
+            tc::mbar_init(ODONE(s), 1);
             tc::mbar_init(OFULL(s), 1);
         }
-        for (int s = 0; s < PF_SCALES; ++s) tc::mbar_init(SCFULL(s), 1);
-        tc::mbar_init(DRAIN, 1);
+        for (int s = 0; s < PF_RING; ++s) {
+            tc::mbar_init(ATFULL(s), 1);
+            tc::mbar_init(ATEMPTY(s), 4);
+        }
+        tc::mbar_init(DRAIN, tiles);
+        tc::mbar_init(GO, 4);   // used once
         tc::mbar_fence_init();
     }
     if (warp == 12) tc::tmem_alloc(tc::smem_addr(tmem_slot), 512);
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
-    bool ok = true;
+    constexpr uint32_t tmem = 0;   // all 512 columns are this CTA's: S0 0, S1 128, O0 256, O1 384
+    bool ok = *tmem_slot == tmem;
 
     if (warp < 8) {   // ------------------------------------------------------------------------------- softmax
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
         const int tile = warp >> 2, row = 32 * (warp & 3) + lane;
         const int r = r0 + 128 * tile + row, tok = r / a.group;
         const bool live = 128 * tile + row < rn;
@@ -187,25 +240,29 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
             float qf;
             {
                 const T *src = static_cast<const T *>(a.q) + (int64_t)(first + tok) * a.q_tok + (int64_t)qh * a.q_head;
+                float4 x[D / 4];   // all loads in flight at once
                 float top = 0.f;
-                if (live)
-                    for (int i = 0; i < D; i += 4) {
-                        const float4 v = kv_load4<T>(src + i, a.q_vec);
-                        top = fmaxf(fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
-                    }
+#pragma unroll
+                for (int i = 0; i < D / 4; ++i) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (live && a.q_vec) {
+#pragma unroll
+                    for (int i = 0; i < D / 4; ++i) x[i] = kv_load4<T>(src + 4 * i, true);
+                } else if (live) {
+#pragma unroll
+                    for (int i = 0; i < D / 4; ++i) x[i] = kv_load4<T>(src + 4 * i, false);
+                }
+#pragma unroll
+                for (int i = 0; i < D / 4; ++i)
+                    top = fmaxf(fmaxf(top, fmaxf(fabsf(x[i].x), fabsf(x[i].y))), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
                 const int up = kv_row_exponent<T>(top);
                 const float f = __int_as_float((up + 127) << 23) * (a.scale_log2 < 0.f ? -1.f : 1.f);
                 qf = __int_as_float((127 - up) << 23) * fabsf(a.scale_log2);
                 uint8_t *dst = smem + SM::Q + tile * SM::OP + row * 128;
-#pragma unroll 4
+#pragma unroll
                 for (int c = 0; c < D / 8; ++c) {
-                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-                    if (live) {
-                        x = kv_load4<T>(src + 8 * c, a.q_vec);
-                        y = kv_load4<T>(src + 8 * c + 4, a.q_vec);
-                    }
+                    const float4 u = x[2 * c], v = x[2 * c + 1];
                     *reinterpret_cast<uint4 *>(dst + (c >> 3) * 16384 + (((c & 7) ^ (row & 7)) << 4)) =
-                        make_uint4(pf_half2(x.x * f, x.y * f), pf_half2(x.z * f, x.w * f), pf_half2(y.x * f, y.y * f), pf_half2(y.z * f, y.w * f));
+                        make_uint4(pf_half2(u.x * f, u.y * f), pf_half2(u.z * f, u.w * f), pf_half2(v.x * f, v.y * f), pf_half2(v.z * f, v.w * f));
                 }
                 tc::fence_proxy_async();
                 __syncwarp();
@@ -215,102 +272,125 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
             const int tn = min(rn - 128 * tile, 128);
             const int pmin = p0 + (r0 + 128 * tile) / a.group, pmax = p0 + (r0 + 128 * tile + tn - 1) / a.group;
             float m = -INFINITY, l = 0.f, eref = -126.f;   // eref: log2 of ref
-            for (int j = 0; j < nk && ok; ++j) {
-                ok = pf_wait(SCFULL(j & (PF_SCALES - 1)), (j / PF_SCALES) & 1) && pf_wait(SFULL(tile), j & 1);
-                if (!ok) break;
+            uint32_t s[64];
+            float f[4], wv[4], ivs[4];   // of the step's four blocks: score factor, log2 of the V scale, its inverse
+            uint32_t valid = 0;
+            // What step u starts with: its scales (written before the K that its scores come from) and its scores, their
+            // loads under way.
+            auto fetch = [&](int u) {
+                const PfPlaces &at = places[(u >> 1) & (PF_RING - 1)];
+                if (!(ok = pf_wait(SFULL(tile, u & 1), (u >> 1) & 1))) return;
                 tc::tc_fence_after();
-                uint32_t s[128];
+                tmem_ld32(tS + 64 * (u & 1), s);
+                tmem_ld32(tS + 64 * (u & 1) + 32, s + 32);
+                const float4 k4 = *reinterpret_cast<const float4 *>(at.ks + 4 * (u & 1)), l4 = *reinterpret_cast<const float4 *>(at.lv + 4 * (u & 1)),
+                             i4 = *reinterpret_cast<const float4 *>(at.iv + 4 * (u & 1));
+                valid = at.valid >> (4 * (u & 1)) & 15u;
+                f[0] = k4.x, f[1] = k4.y, f[2] = k4.z, f[3] = k4.w;
+                wv[0] = l4.x, wv[1] = l4.y, wv[2] = l4.z, wv[3] = l4.w;
+                ivs[0] = i4.x, ivs[1] = i4.y, ivs[2] = i4.z, ivs[3] = i4.w;
+            };
+            auto step = [&](int u) {
+                const int j = u >> 1, half = u & 1, k0 = key0(j) + 64 * half;
+                const bool whole = valid == 15u && k0 + 63 <= pmin && (a.window == 0 || k0 > pmax - a.window || k0 + 63 < a.n_sink);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld32(tS + 32 * c, s + 32 * c);
-                const PfScales &sc = scales[j & (PF_SCALES - 1)];
-                const int k0 = key0(j);
-                const uint32_t valid = sc.valid;
-                const bool whole = valid == 0xFFu && k0 + PF_KEYS - 1 <= pmin &&
-                                   (a.window == 0 || k0 > pmax - a.window || k0 + PF_KEYS - 1 < a.n_sink);
-                float f[8], lv[8];
-                float vmax = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    f[i] = sc.ks[i] * qf;
-                    lv[i] = sc.lv[i];
-                    vmax = fmaxf(vmax, lv[i]);
-                }
+                for (int i = 0; i < 4; ++i) f[i] *= qf;
+                const float vmax = fmaxf(fmaxf(wv[0], wv[1]), fmaxf(wv[2], wv[3]));
                 tc::tmem_ld_wait();
 #pragma unroll
-                for (int i = 0; i < 128; ++i) asm volatile("" : "+r"(s[i]));   // no use moves above the wait
-                if (!whole)
+                for (int i = 0; i < 64; ++i) asm volatile("" : "+r"(s[i]));   // no use moves above the wait
+                auto rest = [&](auto masked) {   // twice in the code, so that whole steps carry no tests
+                    constexpr bool MASKED = decltype(masked)::value;
+                    uint32_t see[2] = {~0u, ~0u};
+                    if constexpr (MASKED) {
+                        see[0] = pf_mask(a, p, k0, valid);
+                        see[1] = pf_mask(a, p, k0 + 32, valid >> 2);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const uint32_t see = pf_mask(a, p, k0 + 32 * c, valid >> (2 * c));
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (!(see >> i & 1u)) s[32 * c + i] = 0xFF800000u;
+                        for (int i = 0; i < 64; ++i)
+                            if (!(see[i >> 5] >> (i & 31) & 1u)) s[i] = 0xFF800000u;
                     }
-                float mx = -INFINITY;
+                    float mx = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    float g = __uint_as_float(s[16 * i]);
+                    for (int i = 0; i < 4; ++i) {
+                        float g = __uint_as_float(s[16 * i]);
 #pragma unroll
-                    for (int e = 1; e < 16; ++e) g = fmaxf(g, __uint_as_float(s[16 * i + e]));
-                    mx = fmaxf(mx, g * f[i]);
-                }
-                float al = 1.f;
-                bool change = false;
-                if (mx > m + 8.f) {
-                    al = pf_ex2(m - mx);
-                    m = mx;
-                    l *= al;
-                    change = true;
-                }
-                if (vmax > eref + 4.f) {   // the same in every thread of the CTA
-                    const float e = fminf(fmaxf(ceilf(vmax), -120.f), 120.f);
-                    al *= pf_ex2(eref - e);
-                    change = true;
-                    eref = e;
-                }
-                if (__any_sync(0xffffffffu, change) && j > 0) {
+                        for (int e = 1; e < 16; ++e) g = fmaxf(g, __uint_as_float(s[16 * i + e]));
+                        mx = fmaxf(mx, g * f[i]);
+                    }
+                    float al = 1.f;
+                    bool change = false;
+                    if (mx > m + 11.f) {
+                        al = pf_ex2(m - (mx + 3.f));
+                        m = mx + 3.f;
+                        l *= al;
+                        change = true;
+                    }
+                    if (vmax > eref + 4.f) {   // the same in every thread of the CTA
+                        const float e = fminf(fmaxf(ceilf(vmax), -120.f), 120.f);
+                        al *= pf_ex2(eref - e);
+                        change = true;
+                        eref = e;
+                    }
+                    if (__any_sync(0xffffffffu, change) && u > 0) {   // O as it stands after the step before this one
+                        if (!(ok = pf_wait(ODONE(tile), (u - 1) & 1))) return;
+                        tc::tc_fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < D / 16; ++c) {
-                        uint32_t o[16];
-                        tc::tmem_ld16(tO + 16 * c, o);
-                        tc::tmem_ld_wait();
+                        for (int c = 0; c < D / 16; ++c) {
+                            uint32_t o[16];
+                            tc::tmem_ld16(tO + 16 * c, o);
+                            tc::tmem_ld_wait();
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(o[i]));
+                            for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(o[i]));
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
-                        tmem_st16(tO + 16 * c, o);
-                    }
-                }
-                const float mu = m == -INFINITY ? 0.f : m, ref = pf_ex2(eref);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t pk[16], see = ~0u;
-                    if (!whole) see = pf_mask(a, p, k0 + 32 * c, valid >> (2 * c));
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const int i = 2 * c + u;
-                        const float w = lv[i] - eref, cw = (w < -40.f ? -40.f : w) - mu;   // a NaN scale stays one
-                        float sum = 0.f;
-#pragma unroll
-                        for (int e = 0; e < 16; e += 2) {
-                            float x = pf_ex2(fmaf(__uint_as_float(s[16 * i + e]), f[i], cw));
-                            float y = pf_ex2(fmaf(__uint_as_float(s[16 * i + e + 1]), f[i], cw));
-                            if (!whole) {
-                                x = see >> (16 * u + e) & 1u ? x : 0.f;
-                                y = see >> (16 * u + e + 1) & 1u ? y : 0.f;
-                            }
-                            sum += x + y;
-                            pk[8 * u + e / 2] = pf_half2(x, y);
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
+                            tmem_st16(tO + 16 * c, o);
                         }
-                        l = fmaf(sum, fminf(sc.iv[i] * ref, 0x1p40f), l);
                     }
-                    tmem_st16(tS + 16 * c, pk);
-                }
+                    const float mu = m == -INFINITY ? 0.f : m, ref = pf_ex2(eref);
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int h2 = 0; h2 < 2; ++h2) {
+                            const int i = 2 * c + h2;
+                            const float w = wv[i] - eref, cw = (w < -40.f ? -40.f : w) - mu;   // a NaN scale stays one
+                            const uint64_t f2 = f2_pack(f[i], f[i]), c2 = f2_pack(cw, cw);
+                            uint64_t sum2 = 0;   // two zeros
+#pragma unroll
+                            for (int e = 0; e < 16; e += 2) {
+                                float x, y;
+                                f2_unpack(f2_fma(f2_pack(__uint_as_float(s[16 * i + e]), __uint_as_float(s[16 * i + e + 1])), f2, c2), x, y);
+                                x = pf_ex2(x);
+                                y = pf_ex2(y);
+                                if constexpr (MASKED) {
+                                    x = see[c] >> (16 * h2 + e) & 1u ? x : 0.f;
+                                    y = see[c] >> (16 * h2 + e + 1) & 1u ? y : 0.f;
+                                }
+                                sum2 = f2_add(sum2, f2_pack(x, y));
+                                pk[8 * h2 + e / 2] = pf_half2(x, y);
+                            }
+                            float sum, odd;
+                            f2_unpack(sum2, sum, odd);
+                            l = fmaf(sum + odd, fminf(ivs[i] * ref, 0x1p40f), l);
+                        }
+                        tmem_st16(tS + 64 * half + 16 * c, pk);
+                    }
+                };
+                if (whole) rest(std::false_type());
+                else rest(std::true_type());
+                if (!ok) return;
+                if (u + 1 < 2 * nk) fetch(u + 1);   // long there: its wait and loads pass under the stores
+                if (!ok) return;
                 tmem_st_wait();
                 tc::tc_fence_before();
                 __syncwarp();
-                if (lane == 0) tc::mbar_arrive(PFULL(tile));
-            }
+                if (lane == 0) {
+                    tc::mbar_arrive(PFULL(tile, half));
+                    if (u == 0 && tile == 0) tc::mbar_arrive(GO);
+                }
+            };
+            if (nk > 0) fetch(0);
+            for (int u = 0; u < 2 * nk && ok; ++u) step(u);
             const int64_t out_row = (int64_t)(first + tok) * a.c.heads * a.group + qh;
             float inv = 0.f;
             if (nk > 0 && ok) {
@@ -346,51 +426,21 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
             }
         }
     } else if (warp < 12) {   // ----------------------------------------------------------------------- converters
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
         constexpr int CH = D / 16, RP = 128 / CH, NL = 128 / RP;   // 16-byte pieces of a key, keys of a pass, passes
         const int ct = threadIdx.x - 256, ch = ct % CH, kr = ct / CH;
-        uint4 x[NL];
-        uint32_t valid = 0;
-        // item i: K of tile i / 2 when i is even, V when odd; its codes to registers
-        auto load = [&](int i) {
-            const int k0 = key0(i >> 1);
-            const uint8_t *codes = i & 1 ? a.c.v : a.c.k;
-            int pg = -1;
-            if (lane < 8) {   // blocks that no row of the CTA sees count as blocks without a page
-                const int kb = k0 + 16 * lane;
-                if (kb <= phi && (a.window == 0 || kb + 15 > plo - a.window || kb < a.n_sink)) pg = a.c.page_of(b, kb);
-            }
-            valid = __ballot_sync(0xffffffffu, pg >= 0) & 0xFFu;
+        uint4 xk[NL], xv[NL];   // a tile's codes, a tile ahead of their conversion
+        auto load = [&](uint4 *x, const uint8_t *codes, int j) {
+            const PfPlaces &sc = places[j & (PF_RING - 1)];
+            const uint32_t valid = sc.valid;
 #pragma unroll
             for (int u = 0; u < NL; ++u) {
-                const int key = u * RP + kr, pos = k0 + key;
-                const int page = __shfl_sync(0xffffffffu, pg, key >> 4);
+                const int key = u * RP + kr;
                 x[u] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-                if (page >= 0) x[u] = ldg_stream16(codes + (a.c.block(page, h, pos) * KV_BLOCK + (pos & 15)) * D + 16 * ch);
-            }
-            if (!(i & 1) && warp == 8 && lane < 8) {   // the tile's scales travel with its K
-                PfScales &sc = scales[(i >> 1) & (PF_SCALES - 1)];
-                float ks = 0.f, vs = 0.f;
-                if (pg >= 0) {
-                    const int64_t at = a.c.block(pg, h, k0 + 16 * lane);
-                    ks = a.c.ks[at];
-                    vs = a.c.vs[at];
-                }
-                sc.ks[lane] = ks;
-                sc.lv[lane] = log2f(vs);
-                sc.iv[lane] = 1.f / vs;
-                if (lane == 0) sc.valid = valid;
-            }
-            if (!(i & 1) && warp == 8) {
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive(SCFULL((i >> 1) & (PF_SCALES - 1)));
+                if (valid >> (key >> 4) & 1u) x[u] = ldg_stream16(codes + (sc.at[key >> 4] * KV_BLOCK + (key & 15)) * D + 16 * ch);
             }
         };
-        if (nk > 0) load(0);
-        for (int i = 0; i < 2 * nk && ok; ++i) {
-            const int j = i >> 1, s = j & 1;
-            if (j >= 2 && !(ok = pf_wait(i & 1 ? VEMPTY(s) : KEMPTY(s), ((j >> 1) - 1) & 1))) break;
-            uint8_t *op = smem + (i & 1 ? SM::V : SM::K) + s * SM::OP;
+        auto store = [&](const uint4 *x, uint8_t *op) {
 #pragma unroll
             for (int u = 0; u < NL; ++u) {
                 const int key = u * RP + kr;
@@ -404,57 +454,103 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
             }
             tc::fence_proxy_async();
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(i & 1 ? VFULL(s) : KFULL(s));
-            if (i + 1 < 2 * nk) load(i + 1);
+        };
+        if (nk > 0 && (ok = pf_wait_idle(ATFULL(0), 0))) {
+            load(xk, a.c.k, 0);
+            load(xv, a.c.v, 0);
+            if (lane == 0) tc::mbar_arrive(ATEMPTY(0));
+        }
+        for (int j = 0; j < nk && ok; ++j) {
+            const int s = j & 1, t = (j + 1) & (PF_RING - 1);
+            if (j >= 2 && !(ok = pf_wait_idle(KEMPTY(s), ((j >> 1) - 1) & 1))) break;
+            store(xk, smem + SM::K + s * SM::OP);
+            if (lane == 0) tc::mbar_arrive(KFULL(s));
+            if (j + 1 < nk) {
+                if (!(ok = pf_wait_idle(ATFULL(t), ((j + 1) / PF_RING) & 1))) break;
+                load(xk, a.c.k, j + 1);
+            }
+            if (j >= 2 && !(ok = pf_wait_idle(VEMPTY(s), ((j >> 1) - 1) & 1))) break;
+            store(xv, smem + SM::V + s * SM::OP);
+            if (lane == 0) tc::mbar_arrive(VFULL(s));
+            if (j + 1 < nk) {
+                load(xv, a.c.v, j + 1);
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(ATEMPTY(t));
+            }
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-        if (warp == 12 && nk > 0) {   // ------------------------------------------------------------- MMA issuer
-            constexpr uint32_t id_qk = tc::idesc_f16(128, PF_KEYS), id_pv = tc::idesc_f16(128, D) | (1u << 16);
-            auto qk = [&](int t, int j) {
-                if (lane == 0) {
-                    const uint32_t sq = tc::smem_addr(smem + SM::Q + t * SM::OP), sk = tc::smem_addr(smem + SM::K + (j & 1) * SM::OP);
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        if (warp == 14) {   // ------------------------------------------------------ pages, some tiles ahead
+            for (int j = 0; j < nk && ok; ++j) {
+                const int s = j & (PF_RING - 1), kb = key0(j) + 16 * lane;
+                int pg = -1;
+                // blocks that no row of the CTA sees count as blocks without a page
+                if (lane < 8 && kb <= phi && (a.window == 0 || kb + 15 > plo - a.window || kb < a.n_sink)) pg = a.c.page_of(b, kb);
+                const uint32_t valid = __ballot_sync(0xffffffffu, pg >= 0);
+                float ks = 0.f, vs = 0.f;
+                int64_t at = 0;
+                if (pg >= 0) {
+                    at = a.c.block(pg, h, kb);
+                    ks = a.c.ks[at];
+                    vs = a.c.vs[at];
+                }
+                if (j >= PF_AHEAD && !(ok = pf_wait_idle(ATEMPTY((j - PF_AHEAD) & (PF_RING - 1)), ((j - PF_AHEAD) / PF_RING) & 1))) break;
+                if (lane < 8) {
+                    places[s].ks[lane] = ks;
+                    places[s].lv[lane] = log2f(vs);
+                    places[s].iv[lane] = 1.f / vs;
+                    places[s].at[lane] = at;
+                }
+                if (lane == 8) places[s].valid = valid;
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(ATFULL(s));
+            }
+        } else if (warp < 12 + tiles && nk > 0) {   // ------------------------------------------------- MMA issuers
+            constexpr uint32_t id_qk = tc::idesc_f16(128, 64), id_pv = tc::idesc_f16(128, D) | (1u << 16);
+            constexpr uint32_t OPD = SM::OP >> 4;   // one operand further in a descriptor
+            const int t = warp - 12;
+            const uint64_t dq = tc::sw128_desc(tc::smem_addr(smem + SM::Q + t * SM::OP)), dk = tc::sw128_desc(tc::smem_addr(smem + SM::K)),
+                           dv = v_desc<D>(tc::smem_addr(smem + SM::V));
+            const bool one = elect_one();
+            auto qk = [&](int j, int half) {   // scores of 64 keys
+                if (one) {
+                    const uint64_t k = dk + (j & 1) * OPD + half * 512;
 #pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        const uint32_t o = (k >> 2) * 16384 + (k & 3) * 32;
-                        tc::mma_f16(tmem + 128u * t, tc::sw128_desc(sq + o), tc::sw128_desc(sk + o), id_qk, k > 0);
-                    }
-                    tc::mma_commit(SFULL(t));
+                    for (int i = 0; i < D / 16; ++i)
+                        tc::mma_f16(128u * t + 64u * half, dq + (i >> 2) * 1024 + (i & 3) * 2, k + (i >> 2) * 1024 + (i & 3) * 2, id_qk, i > 0);
+                    tc::mma_commit(SFULL(t, half));
+                    if (half) tc::mma_commit(KEMPTY(j & 1));   // the last of this tile to read it
                 }
                 __syncwarp();
             };
             ok = pf_wait(QFULL, 0) && pf_wait(KFULL(0), 0);
+            // Tile 1 begins when tile 0 has its first P', so that the two do not start at the exponentials together
+            if (t == 1) ok = ok && pf_wait(GO, 0);
             tc::tc_fence_after();
             if (ok) {
-                for (int t = 0; t < tiles; ++t) qk(t, 0);
-                if (lane == 0) tc::mma_commit(KEMPTY(0));
-                __syncwarp();
+                qk(0, 0);
+                qk(0, 1);
             }
-            for (int j = 0; j < nk && ok; ++j) {
-                for (int t = 0; t < tiles && ok; ++t) {
-                    ok = pf_wait(PFULL(t), j & 1) && (t > 0 || pf_wait(VFULL(j & 1), (j >> 1) & 1));
-                    if (!ok) break;
-                    tc::tc_fence_after();
-                    if (lane == 0) {
-                        const uint32_t sv = tc::smem_addr(smem + SM::V + (j & 1) * SM::OP);
+            for (int u = 0; u < 2 * nk && ok; ++u) {
+                const int j = u >> 1, half = u & 1;
+                if (half == 0)
+                    ok = (j + 1 == nk || pf_wait(KFULL((j + 1) & 1), ((j + 1) >> 1) & 1)) && pf_wait(VFULL(j & 1), (j >> 1) & 1);
+                if (!(ok = ok && pf_wait(PFULL(t, half), j & 1))) break;
+                tc::tc_fence_after();
+                if (one) {
+                    const uint64_t v = dv + (j & 1) * OPD + half * 512;
 #pragma unroll
-                        for (int k = 0; k < PF_KEYS / 16; ++k)
-                            mma_f16_ts(tmem + 256u + 128u * t, tmem + 128u * t + 8u * k, v_desc<D>(sv + 2048u * k), id_pv, j > 0 || k > 0);
-                        if (t == tiles - 1) tc::mma_commit(VEMPTY(j & 1));
-                        if (j == nk - 1) tc::mma_commit(OFULL(t));
-                    }
-                    __syncwarp();
-                    if (j + 1 < nk) {
-                        if (t == 0 && !(ok = pf_wait(KFULL((j + 1) & 1), ((j + 1) >> 1) & 1))) break;
-                        tc::tc_fence_after();
-                        qk(t, j + 1);
-                        if (t == tiles - 1 && lane == 0) tc::mma_commit(KEMPTY((j + 1) & 1));
-                        __syncwarp();
-                    }
+                    for (int i = 0; i < 4; ++i)
+                        mma_f16_ts(256u + 128u * t, 128u * t + 64u * half + 8u * i, v + 128 * i, id_pv, u > 0 || i > 0);
+                    tc::mma_commit(ODONE(t));
+                    if (half) tc::mma_commit(VEMPTY(j & 1));
+                    if (u == 2 * nk - 1) tc::mma_commit(OFULL(t));
                 }
+                __syncwarp();
+                if (j + 1 < nk) qk(j + 1, half);
             }
             // nothing of this CTA is in flight when tensor memory is given back
-            if (lane == 0) tc::mma_commit(DRAIN);
+            if (one) tc::mma_commit(DRAIN);
             __syncwarp();
             ok = pf_wait(DRAIN, 0) && ok;
         }
