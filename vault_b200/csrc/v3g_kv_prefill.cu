@@ -21,7 +21,7 @@
 // margin of 8 from the maximum itself, some row of the 32 did so at every second step on scores of standard deviation 3.
 //
 // K scales multiply the scores; a V scale vs enters the exponent, P' = 2^(s - m + log2(vs / ref)), ref a power of two
-// that follows the largest vs, and the row sum takes P' ref / vs.  vs / ref is held at or above 2^-40, where P' rounds to
+// that follows the largest vs (the same for the whole CTA), and the row sum takes P' ref / vs.  vs / ref is held at or above 2^-40, where P' rounds to
 // zero in fp16 whatever p is: a block with scale 0 adds nothing to O and its full weight to the sum.
 #include <atomic>
 #include <cfloat>
@@ -46,26 +46,34 @@ struct PfSmem {
 };
 
 struct alignas(16) PfPlaces {   // of one key tile, per 16-key block
-    float ks[8], lv[8], iv[8];   // K scale, log2 of the V scale, its inverse
+    float ks[8], w[8], iw[8];    // K scale, log2 of vs / ref, ref / vs (both with vs / ref held at 2^-40 or above)
     int64_t at[8];               // index of the block in the layer
-    uint32_t valid, pad[7];      // bit i: block i has a page and some row sees it
+    int k0;                      // first key
+    uint32_t valid, whole;       // bit i: block i has a page and some row sees it; bit 2 tile + half: every key of the half is visible
+    float al, ref;               // what a change of ref multiplies the accumulators by, ref
+    uint32_t pad[3];
 };
 static_assert(sizeof(PfPlaces) == 192, "ring slot");
 
 #define TC_REGS8(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7])
 #define TC_IN8(r, o) "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7])
-__device__ __forceinline__ void tmem_ld32(uint32_t a, uint32_t *r) {
+// 64 consecutive columns of the warp's 32 lanes; the values are there when it returns
+__device__ __forceinline__ void tmem_ld64_wait(uint32_t a, uint32_t (&r)[64]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
-        "%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : TC_REGS8(r, 0), TC_REGS8(r, 8), TC_REGS8(r, 16), TC_REGS8(r, 24)
-        : "r"(a));
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+        "%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,"
+        "%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n"
+        "tcgen05.wait::ld.sync.aligned;"
+        : TC_REGS8(r, 0), TC_REGS8(r, 8), TC_REGS8(r, 16), TC_REGS8(r, 24), TC_REGS8(r, 32), TC_REGS8(r, 40), TC_REGS8(r, 48), TC_REGS8(r, 56)
+        : "r"(a)
+        : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t a, const uint32_t *r) {
+__device__ __forceinline__ void tmem_ld16_wait(uint32_t a, uint32_t (&r)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
-        "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::TC_IN8(r, 0),
-        TC_IN8(r, 8), TC_IN8(r, 16), TC_IN8(r, 24), "r"(a)
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+        "tcgen05.wait::ld.sync.aligned;"
+        : TC_REGS8(r, 0), TC_REGS8(r, 8)
+        : "r"(a)
         : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t a, const uint32_t *r) {
@@ -112,6 +120,11 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {   // NaN operands are passed over, as by fmaxf
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 __device__ __forceinline__ float pf_ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -136,21 +149,6 @@ __device__ __forceinline__ uint4 pf_convert8(uint32_t a, uint32_t b) {   // eigh
 
 // a whole warp's bounded wait: one answer for all its lanes
 __device__ __forceinline__ bool pf_wait(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity)); }
-// The same for warps that are ahead of their consumers: they sleep between looks and leave their issue slots to others.
-__device__ __forceinline__ bool pf_wait_idle(uint32_t bar, uint32_t parity) {
-    for (uint32_t i = 0; i < tc::WAIT_LIMIT; ++i) {
-        uint32_t done;
-        asm volatile(
-            "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
-            : "=r"(done)
-            : "r"(bar), "r"(parity)
-            : "memory");
-        if (__all_sync(0xffffffffu, done)) return true;
-        __nanosleep(40);
-    }
-    return false;
-}
-
 // visible keys of 32 consecutive ones from kb, as a bit mask, for a row at position p
 __device__ __forceinline__ uint32_t pf_mask(const KvAttnArgs &a, int p, int kb, uint32_t pages) {
     auto below = [](int n) { return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1u); };   // the first n bits
@@ -269,117 +267,95 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
                 if (lane == 0) tc::mbar_arrive(QFULL);
             }
             const int p = live ? p0 + tok : -1;
-            const int tn = min(rn - 128 * tile, 128);
-            const int pmin = p0 + (r0 + 128 * tile) / a.group, pmax = p0 + (r0 + 128 * tile + tn - 1) / a.group;
-            float m = -INFINITY, l = 0.f, eref = -126.f;   // eref: log2 of ref
-            uint32_t s[64];
-            float f[4], wv[4], ivs[4];   // of the step's four blocks: score factor, log2 of the V scale, its inverse
-            uint32_t valid = 0;
-            // What step u starts with: its scales (written before the K that its scores come from) and its scores, their
-            // loads under way.
-            auto fetch = [&](int u) {
-                const PfPlaces &at = places[(u >> 1) & (PF_RING - 1)];
-                if (!(ok = pf_wait(SFULL(tile, u & 1), (u >> 1) & 1))) return;
-                tc::tc_fence_after();
-                tmem_ld32(tS + 64 * (u & 1), s);
-                tmem_ld32(tS + 64 * (u & 1) + 32, s + 32);
-                const float4 k4 = *reinterpret_cast<const float4 *>(at.ks + 4 * (u & 1)), l4 = *reinterpret_cast<const float4 *>(at.lv + 4 * (u & 1)),
-                             i4 = *reinterpret_cast<const float4 *>(at.iv + 4 * (u & 1));
-                valid = at.valid >> (4 * (u & 1)) & 15u;
-                f[0] = k4.x, f[1] = k4.y, f[2] = k4.z, f[3] = k4.w;
-                wv[0] = l4.x, wv[1] = l4.y, wv[2] = l4.z, wv[3] = l4.w;
-                ivs[0] = i4.x, ivs[1] = i4.y, ivs[2] = i4.z, ivs[3] = i4.w;
-            };
+            float m = -INFINITY, l = 0.f;
             auto step = [&](int u) {
-                const int j = u >> 1, half = u & 1, k0 = key0(j) + 64 * half;
-                const bool whole = valid == 15u && k0 + 63 <= pmin && (a.window == 0 || k0 > pmax - a.window || k0 + 63 < a.n_sink);
+                const int j = u >> 1, half = u & 1;
+                if (!(ok = pf_wait(SFULL(tile, half), j & 1))) return;
+                tc::tc_fence_after();
+                // the tile's scales were written before the K that the scores come from
+                const PfPlaces &at = places[j & (PF_RING - 1)];
+                const float4 k4 = *reinterpret_cast<const float4 *>(at.ks + 4 * half), w4 = *reinterpret_cast<const float4 *>(at.w + 4 * half),
+                             i4 = *reinterpret_cast<const float4 *>(at.iw + 4 * half);
+                float f[4] = {k4.x * qf, k4.y * qf, k4.z * qf, k4.w * qf};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) f[i] *= qf;
-                const float vmax = fmaxf(fmaxf(wv[0], wv[1]), fmaxf(wv[2], wv[3]));
-                tc::tmem_ld_wait();
-#pragma unroll
-                for (int i = 0; i < 64; ++i) asm volatile("" : "+r"(s[i]));   // no use moves above the wait
-                auto rest = [&](auto masked) {   // twice in the code, so that whole steps carry no tests
-                    constexpr bool MASKED = decltype(masked)::value;
-                    uint32_t see[2] = {~0u, ~0u};
-                    if constexpr (MASKED) {
-                        see[0] = pf_mask(a, p, k0, valid);
-                        see[1] = pf_mask(a, p, k0 + 32, valid >> 2);
-#pragma unroll
-                        for (int i = 0; i < 64; ++i)
-                            if (!(see[i >> 5] >> (i & 31) & 1u)) s[i] = 0xFF800000u;
-                    }
-                    float mx = -INFINITY;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float g = __uint_as_float(s[16 * i]);
-#pragma unroll
-                        for (int e = 1; e < 16; ++e) g = fmaxf(g, __uint_as_float(s[16 * i + e]));
-                        mx = fmaxf(mx, g * f[i]);
-                    }
-                    float al = 1.f;
-                    bool change = false;
-                    if (mx > m + 11.f) {
-                        al = pf_ex2(m - (mx + 3.f));
-                        m = mx + 3.f;
-                        l *= al;
-                        change = true;
-                    }
-                    if (vmax > eref + 4.f) {   // the same in every thread of the CTA
-                        const float e = fminf(fmaxf(ceilf(vmax), -120.f), 120.f);
-                        al *= pf_ex2(eref - e);
-                        change = true;
-                        eref = e;
-                    }
-                    if (__any_sync(0xffffffffu, change) && u > 0) {   // O as it stands after the step before this one
-                        if (!(ok = pf_wait(ODONE(tile), (u - 1) & 1))) return;
-                        tc::tc_fence_after();
-#pragma unroll 1
-                        for (int c = 0; c < D / 16; ++c) {
-                            uint32_t o[16];
-                            tc::tmem_ld16(tO + 16 * c, o);
-                            tc::tmem_ld_wait();
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(o[i]));
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
-                            tmem_st16(tO + 16 * c, o);
-                        }
-                    }
-                    const float mu = m == -INFINITY ? 0.f : m, ref = pf_ex2(eref);
+                for (int i = 0; i < 4; ++i)
+                    if (f[i] < 0x1p-100f) f[i] = 0x1p-100f;   // hidden keys' -inf stays -inf in a block of scale 0; a NaN stays one
+                float wv[4] = {w4.x, w4.y, w4.z, w4.w}, iw[4] = {i4.x, i4.y, i4.z, i4.w};
+                const float al_ref = half ? 1.f : at.al;
+                uint32_t s[64];
+                tmem_ld64_wait(tS + 64 * half, s);
+                if (!(at.whole >> (2 * tile + half) & 1u)) {   // hide keys; a block that the row does not see at all loses its scales
+                    const int k0 = at.k0 + 64 * half;
+                    const uint32_t valid = at.valid >> (4 * half);
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        uint32_t pk[16];
+                        const uint32_t see = pf_mask(a, p, k0 + 32 * c, valid >> (2 * c));
 #pragma unroll
-                        for (int h2 = 0; h2 < 2; ++h2) {
-                            const int i = 2 * c + h2;
-                            const float w = wv[i] - eref, cw = (w < -40.f ? -40.f : w) - mu;   // a NaN scale stays one
-                            const uint64_t f2 = f2_pack(f[i], f[i]), c2 = f2_pack(cw, cw);
-                            uint64_t sum2 = 0;   // two zeros
+                        for (int i = 0; i < 32; ++i)
+                            if (!(see >> i & 1u)) s[32 * c + i] = 0xFF800000u;
 #pragma unroll
-                            for (int e = 0; e < 16; e += 2) {
-                                float x, y;
-                                f2_unpack(f2_fma(f2_pack(__uint_as_float(s[16 * i + e]), __uint_as_float(s[16 * i + e + 1])), f2, c2), x, y);
-                                x = pf_ex2(x);
-                                y = pf_ex2(y);
-                                if constexpr (MASKED) {
-                                    x = see[c] >> (16 * h2 + e) & 1u ? x : 0.f;
-                                    y = see[c] >> (16 * h2 + e + 1) & 1u ? y : 0.f;
-                                }
-                                sum2 = f2_add(sum2, f2_pack(x, y));
-                                pk[8 * h2 + e / 2] = pf_half2(x, y);
+                        for (int h2 = 0; h2 < 2; ++h2)
+                            if (!(see >> (16 * h2) & 0xFFFFu)) {
+                                f[2 * c + h2] = 1.f;
+                                wv[2 * c + h2] = 0.f;
+                                iw[2 * c + h2] = 0.f;
                             }
-                            float sum, odd;
-                            f2_unpack(sum2, sum, odd);
-                            l = fmaf(sum + odd, fminf(ivs[i] * ref, 0x1p40f), l);
-                        }
-                        tmem_st16(tS + 64 * half + 16 * c, pk);
                     }
-                };
-                if (whole) rest(std::false_type());
-                else rest(std::true_type());
-                if (!ok) return;
-                if (u + 1 < 2 * nk) fetch(u + 1);   // long there: its wait and loads pass under the stores
+                }
+                float mx = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float g = __uint_as_float(s[16 * i]);
+#pragma unroll
+                    for (int e = 1; e < 15; e += 2) g = max3(g, __uint_as_float(s[16 * i + e]), __uint_as_float(s[16 * i + e + 1]));
+                    mx = fmaxf(mx, fmaxf(g, __uint_as_float(s[16 * i + 15])) * f[i]);
+                }
+                float al = al_ref;
+                bool change = al_ref != 1.f;
+                if (mx > m + 11.f) {
+                    const float f = pf_ex2(m - (mx + 3.f));
+                    m = mx + 3.f;
+                    l *= f;
+                    al *= f;
+                    change = true;
+                }
+                if (__any_sync(0xffffffffu, change) && u > 0) {   // O as it stands after the step before this one
+                    if (!(ok = pf_wait(ODONE(tile), (u - 1) & 1))) return;
+                    tc::tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < D / 16; ++c) {
+                        uint32_t o[16];
+                        tmem_ld16_wait(tO + 16 * c, o);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
+                        tmem_st16(tO + 16 * c, o);
+                    }
+                }
+                const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int h2 = 0; h2 < 2; ++h2) {
+                        const int i = 2 * c + h2;
+                        const float cw = wv[i] - mu;
+                        const uint64_t f2 = f2_pack(f[i], f[i]), c2 = f2_pack(cw, cw);
+                        uint64_t sum2 = 0;   // two zeros
+#pragma unroll
+                        for (int e = 0; e < 16; e += 2) {
+                            float x, y;
+                            f2_unpack(f2_fma(f2_pack(__uint_as_float(s[16 * i + e]), __uint_as_float(s[16 * i + e + 1])), f2, c2), x, y);
+                            x = pf_ex2(x);
+                            y = pf_ex2(y);
+                            sum2 = f2_add(sum2, f2_pack(x, y));
+                            pk[8 * h2 + e / 2] = pf_half2(x, y);
+                        }
+                        float sum, odd;
+                        f2_unpack(sum2, sum, odd);
+                        l = fmaf(sum + odd, iw[i], l);
+                    }
+                    tmem_st16(tS + 64 * half + 16 * c, pk);
+                }
                 if (!ok) return;
                 tmem_st_wait();
                 tc::tc_fence_before();
@@ -389,14 +365,14 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
                     if (u == 0 && tile == 0) tc::mbar_arrive(GO);
                 }
             };
-            if (nk > 0) fetch(0);
             for (int u = 0; u < 2 * nk && ok; ++u) step(u);
             const int64_t out_row = (int64_t)(first + tok) * a.c.heads * a.group + qh;
             float inv = 0.f;
             if (nk > 0 && ok) {
                 ok = pf_wait(OFULL(tile), 0);
                 tc::tc_fence_after();
-                inv = a.pf_splits > 1 ? pf_ex2(eref) : (l == 0.f ? 0.f : pf_ex2(eref) / l);
+                inv = places[(nk - 1) & (PF_RING - 1)].ref;
+                if (a.pf_splits == 1) inv = l == 0.f ? 0.f : inv / l;
             }
             const int64_t part = out_row * a.part_stride + blockIdx.z;
             if (ok && (nk > 0 || a.pf_splits == 1))   // an empty share has no accumulator
@@ -406,10 +382,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[i] = 0u;
                     if (nk > 0) {
-                        tc::tmem_ld16(tO + 16 * c, o);
-                        tc::tmem_ld_wait();
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(o[i]));
+                        tmem_ld16_wait(tO + 16 * c, o);
                     }
                     if (live)
 #pragma unroll
@@ -427,53 +400,53 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
         }
     } else if (warp < 12) {   // ----------------------------------------------------------------------- converters
         asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
-        constexpr int CH = D / 16, RP = 128 / CH, NL = 128 / RP;   // 16-byte pieces of a key, keys of a pass, passes
-        const int ct = threadIdx.x - 256, ch = ct % CH, kr = ct / CH;
+        // A thread takes 16 codes of a key at a time: 32 keys and 64 dims a pass.  Eight lanes then hold two keys, whose swizzled
+        // rows fill all banks.
+        constexpr int HV = D / 64, NL = 4 * HV;   // halves of the dims, passes
+        const int ct = threadIdx.x - 256, ch = ct & 3, kr = ct >> 2, sw = kr & 7;
+        const uint8_t *kc = a.c.k + (kr & 15) * D + 16 * ch, *vc = a.c.v + (kr & 15) * D + 16 * ch;
+        const int d0 = kr * 128 + ((2 * ch ^ sw) << 4), d1 = kr * 128 + (((2 * ch + 1) ^ sw) << 4);
         uint4 xk[NL], xv[NL];   // a tile's codes, a tile ahead of their conversion
         auto load = [&](uint4 *x, const uint8_t *codes, int j) {
-            const PfPlaces &sc = places[j & (PF_RING - 1)];
-            const uint32_t valid = sc.valid;
+            const PfPlaces &at = places[j & (PF_RING - 1)];
+            const uint32_t valid = at.valid >> (kr >> 4);
+            const int64_t *where = at.at + (kr >> 4);
 #pragma unroll
             for (int u = 0; u < NL; ++u) {
-                const int key = u * RP + kr;
+                const int blk = u / HV * 2;
                 x[u] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-                if (valid >> (key >> 4) & 1u) x[u] = ldg_stream16(codes + (sc.at[key >> 4] * KV_BLOCK + (key & 15)) * D + 16 * ch);
+                if (valid >> blk & 1u) x[u] = ldg_stream16(codes + where[blk] * (KV_BLOCK * D) + u % HV * 64);
             }
         };
         auto store = [&](const uint4 *x, uint8_t *op) {
 #pragma unroll
             for (int u = 0; u < NL; ++u) {
-                const int key = u * RP + kr;
-                uint8_t *d = op + (ch >> 2) * 16384 + key * 128;
-                const uint4 lo = pf_convert8(x[u].x, x[u].y), hi = pf_convert8(x[u].z, x[u].w);
-                const int c0 = (ch & 3) * 2, sw = key & 7;
-                // lanes of the second half store their upper piece first, so that eight lanes fill all banks
-                const bool swap = ch & 4;
-                *reinterpret_cast<uint4 *>(d + (((c0 + swap) ^ sw) << 4)) = swap ? hi : lo;
-                *reinterpret_cast<uint4 *>(d + (((c0 + !swap) ^ sw) << 4)) = swap ? lo : hi;
+                uint8_t *d = op + u % HV * 16384 + u / HV * 4096;
+                *reinterpret_cast<uint4 *>(d + d0) = pf_convert8(x[u].x, x[u].y);
+                *reinterpret_cast<uint4 *>(d + d1) = pf_convert8(x[u].z, x[u].w);
             }
             tc::fence_proxy_async();
             __syncwarp();
         };
-        if (nk > 0 && (ok = pf_wait_idle(ATFULL(0), 0))) {
-            load(xk, a.c.k, 0);
-            load(xv, a.c.v, 0);
+        if (nk > 0 && (ok = pf_wait(ATFULL(0), 0))) {
+            load(xk, kc, 0);
+            load(xv, vc, 0);
             if (lane == 0) tc::mbar_arrive(ATEMPTY(0));
         }
         for (int j = 0; j < nk && ok; ++j) {
             const int s = j & 1, t = (j + 1) & (PF_RING - 1);
-            if (j >= 2 && !(ok = pf_wait_idle(KEMPTY(s), ((j >> 1) - 1) & 1))) break;
+            if (j >= 2 && !(ok = pf_wait(KEMPTY(s), ((j >> 1) - 1) & 1))) break;
             store(xk, smem + SM::K + s * SM::OP);
             if (lane == 0) tc::mbar_arrive(KFULL(s));
             if (j + 1 < nk) {
-                if (!(ok = pf_wait_idle(ATFULL(t), ((j + 1) / PF_RING) & 1))) break;
-                load(xk, a.c.k, j + 1);
+                if (!(ok = pf_wait(ATFULL(t), ((j + 1) / PF_RING) & 1))) break;
+                load(xk, kc, j + 1);
             }
-            if (j >= 2 && !(ok = pf_wait_idle(VEMPTY(s), ((j >> 1) - 1) & 1))) break;
+            if (j >= 2 && !(ok = pf_wait(VEMPTY(s), ((j >> 1) - 1) & 1))) break;
             store(xv, smem + SM::V + s * SM::OP);
             if (lane == 0) tc::mbar_arrive(VFULL(s));
             if (j + 1 < nk) {
-                load(xv, a.c.v, j + 1);
+                load(xv, vc, j + 1);
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(ATEMPTY(t));
             }
@@ -481,8 +454,11 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
         if (warp == 14) {   // ------------------------------------------------------ pages, some tiles ahead
+            // first and last position of each tile's rows
+            const int lo1 = p0 + (r0 + 128) / a.group, hi0 = tiles > 1 ? p0 + (r0 + 127) / a.group : phi;
+            float e = -126.f;   // log2 of ref
             for (int j = 0; j < nk && ok; ++j) {
-                const int s = j & (PF_RING - 1), kb = key0(j) + 16 * lane;
+                const int s = j & (PF_RING - 1), k0 = key0(j), kb = k0 + 16 * lane;
                 int pg = -1;
                 // blocks that no row of the CTA sees count as blocks without a page
                 if (lane < 8 && kb <= phi && (a.window == 0 || kb + 15 > plo - a.window || kb < a.n_sink)) pg = a.c.page_of(b, kb);
@@ -494,14 +470,34 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
                     ks = a.c.ks[at];
                     vs = a.c.vs[at];
                 }
-                if (j >= PF_AHEAD && !(ok = pf_wait_idle(ATEMPTY((j - PF_AHEAD) & (PF_RING - 1)), ((j - PF_AHEAD) / PF_RING) & 1))) break;
+                const float lv = log2f(vs), top = warp_max(lane < 8 ? lv : -INFINITY);
+                float al = 1.f;
+                if (top > e + 4.f) {
+                    const float up = fminf(fmaxf(ceilf(top), -120.f), 120.f);
+                    al = pf_ex2(e - up);
+                    e = up;
+                }
+                const float ref = pf_ex2(e), w = lv - e;
+                uint32_t whole = 0;
+                if (lane < 4) {
+                    const int t = lane >> 1, k = k0 + 64 * (lane & 1), lo = t ? lo1 : plo, hi = t ? phi : hi0;
+                    whole = (valid >> (4 * (lane & 1)) & 15u) == 15u && k + 63 <= lo && (a.window == 0 || k > hi - a.window || k + 63 < a.n_sink);
+                }
+                whole = __ballot_sync(0xffffffffu, whole);
+                if (j >= PF_AHEAD && !(ok = pf_wait(ATEMPTY((j - PF_AHEAD) & (PF_RING - 1)), ((j - PF_AHEAD) / PF_RING) & 1))) break;
                 if (lane < 8) {
                     places[s].ks[lane] = ks;
-                    places[s].lv[lane] = log2f(vs);
-                    places[s].iv[lane] = 1.f / vs;
+                    places[s].w[lane] = w < -40.f ? -40.f : w;   // a NaN stays one
+                    places[s].iw[lane] = fminf(ref / vs, 0x1p40f);
                     places[s].at[lane] = at;
                 }
-                if (lane == 8) places[s].valid = valid;
+                if (lane == 8) {
+                    places[s].k0 = k0;
+                    places[s].valid = valid;
+                    places[s].whole = whole;
+                    places[s].al = al;
+                    places[s].ref = ref;
+                }
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(ATFULL(s));
             }
