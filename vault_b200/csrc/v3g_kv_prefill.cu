@@ -194,8 +194,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
     auto OFULL = [&](int t) { return bars + 8u * (19 + t); };
     auto ATFULL = [&](int s) { return bars + 8u * (21 + s); };
     auto ATEMPTY = [&](int s) { return bars + 8u * (29 + s); };
-    const uint32_t DRAIN = bars + 8u * 37, GO = bars + 8u * 38;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + SM::BAR + 8 * 39);
+    const uint32_t DRAIN = bars + 8u * 37;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + SM::BAR + 8 * 38);
     PfPlaces *places = reinterpret_cast<PfPlaces *>(smem + SM::SC);
     if (threadIdx.x == 0) {
         tc::mbar_init(QFULL, 4 * tiles);
@@ -216,7 +216,6 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
             tc::mbar_init(ATEMPTY(s), 4);
         }
         tc::mbar_init(DRAIN, tiles);
-        tc::mbar_init(GO, 4);   // used once
         tc::mbar_fence_init();
     }
     if (warp == 12) tc::tmem_alloc(tc::smem_addr(tmem_slot), 512);
@@ -268,6 +267,22 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
             }
             const int p = live ? p0 + tok : -1;
             float m = -INFINITY, l = 0.f;
+            // Warps w of the two tiles share a quarter of the SM and its exponential unit, so they take turns at it (named
+            // barriers 1 + w and 5 + w, equal step counts): together they took 1,250 clocks for 64 keys each, in turn 750.
+            bool had_turn = false, gave_turn = false;
+            auto turn = [&](int id, bool wait) {
+                if (tiles == 1) return;
+                if (wait) asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory");
+                else asm volatile("bar.arrive %0, 64;" ::"r"(id) : "memory");
+            };
+            auto my_turn = [&]() {
+                turn(1 + 4 * tile + (warp & 3), true);
+                had_turn = true;
+            };
+            auto turn_over = [&](int u) {
+                if (tile == 0 || u + 1 < 2 * nk) turn(5 - 4 * tile + (warp & 3), false);
+                gave_turn = true;
+            };
             auto step = [&](int u) {
                 const int j = u >> 1, half = u & 1;
                 if (!(ok = pf_wait(SFULL(tile, half), j & 1))) return;
@@ -332,6 +347,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
                     }
                 }
                 const float mu = m == -INFINITY ? 0.f : m;
+                my_turn();
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     uint32_t pk[16];
@@ -356,16 +372,21 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
                     }
                     tmem_st16(tS + 64 * half + 16 * c, pk);
                 }
-                if (!ok) return;
+                turn_over(u);
                 tmem_st_wait();
                 tc::tc_fence_before();
                 __syncwarp();
-                if (lane == 0) {
-                    tc::mbar_arrive(PFULL(tile, half));
-                    if (u == 0 && tile == 0) tc::mbar_arrive(GO);
-                }
+                if (lane == 0) tc::mbar_arrive(PFULL(tile, half));
             };
-            for (int u = 0; u < 2 * nk && ok; ++u) step(u);
+            if (tile == 1) turn(1 + (warp & 3), false);
+            for (int u = 0; u < 2 * nk; ++u) {
+                if (ok) step(u);
+                if (!ok) {   // a wait ran out: the partner must not wait for this warp's turns
+                    if (!had_turn) my_turn();
+                    if (!gave_turn) turn_over(u);
+                }
+                had_turn = gave_turn = false;
+            }
             const int64_t out_row = (int64_t)(first + tok) * a.c.heads * a.group + qh;
             float inv = 0.f;
             if (nk > 0 && ok) {
@@ -520,8 +541,6 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
                 __syncwarp();
             };
             ok = pf_wait(QFULL, 0) && pf_wait(KFULL(0), 0);
-            // Tile 1 begins when tile 0 has its first P', so that the two do not start at the exponentials together
-            if (t == 1) ok = ok && pf_wait(GO, 0);
             tc::tc_fence_after();
             if (ok) {
                 qk(0, 0);
