@@ -2,6 +2,7 @@
 //
 // All three move bytes and are bound by HBM at large sizes and by launch latency at small ones.
 #include <cfloat>
+#include <type_traits>
 
 #include "v3g_internal.h"
 #include "v3g_kv.cuh"
@@ -17,7 +18,7 @@ namespace v3g {
 //
 // x' = rotation of x (pairs i, i + D/2; fp32, each product and sum rounded by itself), s = max(s_old, max |x'| / 127),
 // code = rint(x' * (1 / s)).  A larger s moves the block's earlier codes to rint(code * (s_old / s)).
-constexpr int APPEND_WARPS = 8;
+constexpr int APPEND_WARPS = 4;
 
 struct AppendArgs {
     KvView c;
@@ -30,19 +31,54 @@ struct AppendArgs {
     bool k_vec, v_vec, q_vec;
 };
 
-// the rotation of the four dims that start at 4 l (l: lane in the row) given the partner half's four values
-template <int D>
-__device__ __forceinline__ float4 rotate4(float4 x, float4 other, const float *cs, int l) {
-    constexpr int HL = D / 8;                              // lanes of a half row
-    const float4 c = *reinterpret_cast<const float4 *>(cs + 4 * (l % HL));
-    float4 s = *reinterpret_cast<const float4 *>(cs + D / 2 + 4 * (l % HL));
-    if (l < HL) s = make_float4(-s.x, -s.y, -s.z, -s.w);   // x1 c - x2 s; x2 c + x1 s
-    return make_float4(__fadd_rn(__fmul_rn(x.x, c.x), __fmul_rn(other.x, s.x)), __fadd_rn(__fmul_rn(x.y, c.y), __fmul_rn(other.y, s.y)),
-                       __fadd_rn(__fmul_rn(x.z, c.z), __fmul_rn(other.z, s.z)), __fadd_rn(__fmul_rn(x.w, c.w), __fmul_rn(other.w, s.w)));
-}
-__device__ __forceinline__ float4 shfl4(float4 x, int mask) {
-    return make_float4(__shfl_xor_sync(0xffffffffu, x.x, mask), __shfl_xor_sync(0xffffffffu, x.y, mask),
-                       __shfl_xor_sync(0xffffffffu, x.z, mask), __shfl_xor_sync(0xffffffffu, x.w, mask));
+// A lane's consecutive elements of a row: 16 bytes of them
+template <typename T>
+struct Piece {
+    static constexpr int N = 16 / sizeof(T);
+    float x[N];
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = 0.f;
+    }
+    __device__ __forceinline__ void load(const T *p, bool vec) {
+        T e[N];
+        if (vec) *reinterpret_cast<uint4 *>(e) = ldg_stream16(p);
+        else
+#pragma unroll
+            for (int i = 0; i < N; ++i) e[i] = p[i];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if constexpr (std::is_same<T, float>::value) x[i] = e[i];
+            else if constexpr (std::is_same<T, __half>::value) x[i] = __half2float(e[i]);
+            else x[i] = __bfloat162float(e[i]);
+        }
+    }
+    __device__ __forceinline__ void store(T *p) const {
+        uint4 r;
+        T *e = reinterpret_cast<T *>(&r);
+#pragma unroll
+        for (int i = 0; i < N; i += 4) kv_store4(e + i, make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]));
+        *reinterpret_cast<uint4 *>(p) = r;
+    }
+};
+
+// The rotation of lane l's piece of a row: pairs i, i + D/2 sit LR / 2 lanes apart.  x1 c - x2 s; x2 c + x1 s, every product and
+// sum rounded by itself.
+template <typename T, int D>
+__device__ __forceinline__ void rotate(Piece<T> &x, const float *cs, int l, bool turn) {
+    constexpr int N = Piece<T>::N, LR = D / N;
+    const bool low = l < LR / 2;
+    const float *c = cs + N * (l % (LR / 2));
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        const float4 c4 = *reinterpret_cast<const float4 *>(c + i), s4 = *reinterpret_cast<const float4 *>(c + D / 2 + i);
+        const float cc[4] = {c4.x, c4.y, c4.z, c4.w}, ss[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float o = __shfl_xor_sync(0xffffffffu, x.x[i + k], LR / 2);
+            if (turn) x.x[i + k] = __fadd_rn(__fmul_rn(x.x[i + k], cc[k]), __fmul_rn(o, low ? -ss[k] : ss[k]));
+        }
+    }
 }
 __device__ __forceinline__ uint32_t code_byte(float x, float inv) {
     return (uint32_t)((int)rintf(fminf(fmaxf(__fmul_rn(x, inv), -127.f), 127.f)) + 128);
@@ -55,19 +91,19 @@ __device__ __forceinline__ uint32_t moved_codes(uint32_t w, float ratio) {
     return r;
 }
 
-// one head's rows [s0, s1) of a block: the rounding described above
+// one head's rows [s0, s1) of a block: the rounding described above.  cs: the rotation's rows, from row s0's on
 template <typename T, int D>
 __device__ __forceinline__ void append_rows(const T *src, int64_t tok_ld, bool vec, const float *cs, bool turn, int s0, int s1,
                                             uint8_t *codes, float *scale, int lane) {
-    constexpr int LR = D / 4, RP = 32 / LR, NP = KV_BLOCK / RP;   // lanes of a row, rows of a pass, passes
+    constexpr int N = Piece<T>::N, LR = D / N, RP = 32 / LR, NP = KV_BLOCK / RP;   // lanes of a row, rows of a pass, passes
     const int l = lane % LR, sub = lane / LR;
     const float s_old = s0 > 0 ? *scale : 0.f;
-    float4 x[NP];
+    Piece<T> x[NP];
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
         const int r = s0 + i * RP + sub;
-        x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r < s1) x[i] = kv_load4<T>(src + (int64_t)(r - s0) * tok_ld + 4 * l, vec);
+        x[i].zero();
+        if (r < s1) x[i].load(src + (int64_t)(r - s0) * tok_ld + N * l, vec);
     }
     float top = 0.f;
     bool bad = false;
@@ -75,13 +111,12 @@ __device__ __forceinline__ void append_rows(const T *src, int64_t tok_ld, bool v
     for (int i = 0; i < NP; ++i) {
         const int r = s0 + i * RP + sub;
         if (s0 + i * RP >= s1) break;   // uniform over the warp
-        if (turn) {
-            const float4 o = shfl4(x[i], LR / 2);
-            if (r < s1) x[i] = rotate4<D>(x[i], o, cs + (r - s0) * D, l);
+        if (turn) rotate<T, D>(x[i], cs + (r < s1 ? r - s0 : 0) * D, l, r < s1);
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            top = fmaxf(top, fabsf(x[i].x[k]));
+            bad |= !(fabsf(x[i].x[k]) <= FLT_MAX);
         }
-        const float a = fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
-        bad |= !(fabsf(x[i].x) <= FLT_MAX && fabsf(x[i].y) <= FLT_MAX && fabsf(x[i].z) <= FLT_MAX && fabsf(x[i].w) <= FLT_MAX);
-        top = fmaxf(top, a);
     }
     top = warp_max(top);
     bad = __any_sync(0xffffffffu, bad) || s_old != s_old;
@@ -92,18 +127,25 @@ __device__ __forceinline__ void append_rows(const T *src, int64_t tok_ld, bool v
     if (s0 > 0 && s != s_old) {
         const float ratio = s > 0.f ? __fdiv_rn(s_old, s) : 0.f;
         for (int r = sub; r < s0; r += RP) {
-            uint32_t *p = reinterpret_cast<uint32_t *>(codes + r * D + 4 * l);
-            *p = moved_codes(*p, ratio);
+            uint32_t *p = reinterpret_cast<uint32_t *>(codes + r * D + N * l);
+#pragma unroll
+            for (int k = 0; k < N / 4; ++k) p[k] = moved_codes(p[k], ratio);
         }
     }
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
         const int r = s0 + i * RP + sub;
         if (r < s1) {
-            uint32_t w = 0x80808080u;
-            if (!bad)
-                w = code_byte(x[i].x, inv) | code_byte(x[i].y, inv) << 8 | code_byte(x[i].z, inv) << 16 | code_byte(x[i].w, inv) << 24;
-            *reinterpret_cast<uint32_t *>(codes + r * D + 4 * l) = w;
+            uint32_t w[N / 4];
+#pragma unroll
+            for (int k = 0; k < N / 4; ++k) {
+                const float *y = x[i].x + 4 * k;
+                w[k] = bad ? 0x80808080u
+                           : code_byte(y[0], inv) | code_byte(y[1], inv) << 8 | code_byte(y[2], inv) << 16 | code_byte(y[3], inv) << 24;
+            }
+            uint32_t *p = reinterpret_cast<uint32_t *>(codes + r * D + N * l);
+            if constexpr (N == 8) *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+            else *p = w[0];
         }
     }
     __syncwarp();
@@ -146,28 +188,25 @@ __global__ void __launch_bounds__(32 * APPEND_WARPS) k_kv_append(const __grid_co
                               (is_v ? a.c.v : a.c.k) + at * (KV_BLOCK * D), (is_v ? a.c.vs : a.c.ks) + at, lane);
         }
     if (a.q) {   // the queries of the same tokens: rotated, not rounded further than their own type
-        constexpr int LR = D / 4, RP = 32 / LR, U = 4;
+        constexpr int N = Piece<T>::N, LR = D / N, RP = 32 / LR, U = 4;
         const int l = lane % LR, sub = lane / LR, rows = nt * a.q_heads;
         // shares of the warps that hold no K/V row come first
         const int w1 = (w0 + step - 2 * heads % step) % step;
         for (int r0 = w1 * RP * U; r0 < rows; r0 += step * RP * U) {
-            float4 x[U];
+            Piece<T> x[U];
+            int tok[U], h[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int r = r0 + u * RP + sub, tok = r / a.q_heads, h = r - tok * a.q_heads;
-                x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (r < rows)
-                    x[u] = kv_load4<T>(static_cast<const T *>(a.q) + (int64_t)(t0 + tok) * a.q_tok + (int64_t)h * a.q_head + 4 * l, a.q_vec);
+                const int r = r0 + u * RP + sub;
+                tok[u] = r / a.q_heads, h[u] = r - tok[u] * a.q_heads;
+                x[u].zero();
+                if (r < rows && tok[u] < placed)
+                    x[u].load(static_cast<const T *>(a.q) + (int64_t)(t0 + tok[u]) * a.q_tok + (int64_t)h[u] * a.q_head + N * l, a.q_vec);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int r = r0 + u * RP + sub, tok = r / a.q_heads, h = r - tok * a.q_heads;
-                const float4 o = shfl4(x[u], LR / 2);
-                if (r < rows) {
-                    if (tok >= placed) x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    else if (turn) x[u] = rotate4<D>(x[u], o, cs + tok * D, l);
-                    kv_store4(static_cast<T *>(a.q_out) + ((int64_t)(t0 + tok) * a.q_heads + h) * D + 4 * l, x[u]);
-                }
+                if (turn) rotate<T, D>(x[u], cs + (tok[u] < placed ? tok[u] : 0) * D, l, tok[u] < placed);
+                if (tok[u] < nt) x[u].store(static_cast<T *>(a.q_out) + ((int64_t)(t0 + tok[u]) * a.q_heads + h[u]) * D + N * l);
             }
         }
     }
@@ -202,18 +241,43 @@ __global__ void __launch_bounds__(256) k_kv_read(const __grid_constant__ ReadArg
     const bool in = base <= row && row < a.c.q_start[b + 1] && pos >= 0 && pos < a.c.len(b);
     const int page = in ? a.c.page_of(b, pos) : -1;
     const int64_t at = page >= 0 ? a.c.block(page, h, pos) : 0;
-    for (int l = blockIdx.y; l < a.layers; l += gridDim.y) {
+    constexpr int U = 4;   // layers in flight
+    const int64_t src = (at * KV_BLOCK + (pos & 15)) * D + d, dst = (row * a.c.heads + h) * D + d, layer_out = (int64_t)a.c.n_tokens * a.c.heads * D;
+    for (int l0 = blockIdx.y; l0 < a.layers; l0 += U * gridDim.y) {
+        uint2 w[U][2];
+        float s[U][2];
 #pragma unroll
-        for (int kind = 0; kind < 2; ++kind) {
-            float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
-            if (page >= 0) {
-                const uint8_t *codes = (kind ? a.c.v : a.c.k) + l * a.layer_codes;
-                const float s = (kind ? a.c.vs : a.c.ks)[l * a.layer_scales + at];
-                read8(*reinterpret_cast<const uint2 *>(codes + (at * KV_BLOCK + (pos & 15)) * D + d), s, lo, hi);
+        for (int u = 0; u < U; ++u) {
+            const int l = l0 + u * gridDim.y;
+#pragma unroll
+            for (int kind = 0; kind < 2; ++kind) {
+                w[u][kind] = make_uint2(0x80808080u, 0x80808080u);
+                s[u][kind] = 0.f;
+                if (page >= 0 && l < a.layers) {
+                    w[u][kind] = ldg_stream8((kind ? a.c.v : a.c.k) + l * a.layer_codes + src);
+                    s[u][kind] = (kind ? a.c.vs : a.c.ks)[l * a.layer_scales + at];
+                }
             }
-            T *out = static_cast<T *>(kind ? a.v : a.k) + (((int64_t)l * a.c.n_tokens + row) * a.c.heads + h) * D + d;
-            kv_store4(out, lo);
-            kv_store4(out + 4, hi);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int l = l0 + u * gridDim.y;
+            if (l < a.layers)
+#pragma unroll
+                for (int kind = 0; kind < 2; ++kind) {
+                    float4 lo, hi;
+                    read8(w[u][kind], s[u][kind], lo, hi);
+                    T *out = static_cast<T *>(kind ? a.v : a.k) + l * layer_out + dst;
+                    if constexpr (sizeof(T) == 2) {
+                        uint4 r;
+                        kv_store4(reinterpret_cast<T *>(&r), lo);
+                        kv_store4(reinterpret_cast<T *>(&r) + 4, hi);
+                        __stcs(reinterpret_cast<uint4 *>(out), r);
+                    } else {
+                        kv_store4(out, lo);
+                        kv_store4(out + 4, hi);
+                    }
+                }
         }
     }
 }
@@ -347,9 +411,10 @@ static int launched(const char *who) {
 
 static size_t dtype_bytes(int t) { return t == V3G_F32 ? 4 : 2; }
 
-// four-wide loads of rows: the base and both strides keep 4-element alignment
+// 16-byte loads of rows: the base and both strides keep that alignment
 static bool rows_vec(const v3g_rows_t &r, int dtype) {
-    return aligned_to(r.data, 4 * dtype_bytes(dtype)) && r.tok_stride % 4 == 0 && r.head_stride % 4 == 0;
+    const int64_t n = 16 / (int64_t)dtype_bytes(dtype);
+    return aligned_to(r.data, 16) && r.tok_stride % n == 0 && r.head_stride % n == 0;
 }
 
 template <typename T>
@@ -409,11 +474,11 @@ extern "C" int v3g_kv_append(const v3g_kv_cache_t *cache, uint32_t layer, const 
     a.rope_rows = (int)rope_rows;
     a.status = dev_status;
     const uint32_t items = batch->n_tokens / KV_BLOCK + 2 * batch->batch;
-    // heads are shared out over more CTAs while the blocks alone leave SMs idle; past one pass of the warps over
-    // the rows there is nothing left to share
+    // A block's heads are shared out over CTAs until the warps of the whole GPU have a few rows each (6,000 tokens, 32/8
+    // heads: one CTA a block 218 us, four NNN us); past one pass of the warps over the rows there is nothing left to share.
     const uint32_t passes = (2 * cache->n_kv_heads + (q ? n_q_heads * 2 : 0) + APPEND_WARPS - 1) / APPEND_WARPS;
-    uint32_t ny = 296 / (items ? items : 1);
-    ny = ny < 1 ? 1 : (ny > passes ? passes : ny);
+    uint32_t ny = (148 * 16 + items - 1) / items;
+    ny = ny > passes ? passes : ny;
     const dim3 grid(items, ny);
     const cudaStream_t st = (cudaStream_t)stream;
     if (dtype == V3G_F32) launch_append<float>(a, (int)cache->head_dim, grid, st);

@@ -74,7 +74,6 @@ __global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 3) k_kv_decode(c
     constexpr int ROWS = 8 * NT, NCH = D / 64, VB = D / 8, MT = D / 16, OS = D + 4;
     __shared__ float sm_m[DEC_WARPS][ROWS], sm_l[DEC_WARPS][ROWS];
     __shared__ __align__(16) float sm_o[DEC_WARPS][ROWS][OS];
-    griddep_launch();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     int idx = blockIdx.x;
     const int rt0 = idx % a.row_tiles;
@@ -84,10 +83,11 @@ __global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 3) k_kv_decode(c
     const int h = idx % a.c.heads, b = idx / a.c.heads;
     int first;
     const int n = a.c.tokens(b, first);
-    if (n * a.group > a.max_rows) return;                                    // the many-row kernel's
+    const int rows = n * a.group > a.max_rows ? 0 : n * a.group;             // else they are the many-row kernel's
     const int p0 = a.c.end(b) - n;
-    for (int rt = rt0; rt * ROWS < n * a.group; rt += a.row_tiles) {
-        const int r0 = rt * ROWS, rn = min(n * a.group - r0, ROWS);
+    griddep_launch();
+    for (int rt = rt0; rt * ROWS < rows; rt += a.row_tiles) {
+        const int r0 = rt * ROWS, rn = min(rows - r0, ROWS);
         const int pmin = p0 + r0 / a.group, pmax = p0 + (r0 + rn - 1) / a.group;
         int sb, ws;                                                          // blocks [0, sb) and [ws, ws + nb - sb)
         const int nb = kv_visible(a, pmin, pmax, KV_BLOCK, sb, ws);
@@ -327,61 +327,70 @@ __global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 3) k_kv_decode(c
         }
         __syncthreads();
     }
+    // beside the many-row kernel: whoever waits for this one's end waits for both
+    if (a.after_many) griddep_wait();
 }
 
-// joins the splits of one row (a warp each, in split order)
-template <typename T, int D>
+// Joins the shares of a row: WR warps take every WR-th share each, in order, and are added in order.
+template <typename T, int D, int WR>
 __global__ void __launch_bounds__(128) k_kv_join(const __grid_constant__ KvAttnArgs a) {
+    constexpr int W = D / 32, ROWS = 4 / WR;
+    __shared__ float sm_o[4][D], sm_l[4];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, qh = a.c.heads * a.group, w0 = warp % WR;
+    const int64_t row = (int64_t)blockIdx.x * ROWS + warp / WR;
+    int shares = 0;
+    if (row < (int64_t)a.c.n_tokens * qh) {
+        const int tok = (int)(row / qh);
+        int64_t base;
+        const int b = kv_find(a.c.q_start, a.c.batch, a.c.n_tokens, 1, 1, 0, tok, base);
+        int first;
+        const int n = a.c.tokens(b, first);
+        if (tok >= first && tok < first + n) shares = n * a.group > a.max_rows ? a.pf_splits : a.splits;
+    }
+    if (WR == 4 && shares <= 1) return;            // no sequence's row, or a finished one
     griddep_wait();
-    const int lane = threadIdx.x & 31, qh = a.c.heads * a.group;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (row >= (int64_t)a.c.n_tokens * qh) return;
-    const int tok = (int)(row / qh);
-    int64_t base;
-    const int b = kv_find(a.c.q_start, a.c.batch, a.c.n_tokens, 1, 1, 0, tok, base);
-    int first;
-    const int n = a.c.tokens(b, first);
-    if (tok < first || tok >= first + n) return;   // no sequence's
-    const int splits = n * a.group > a.max_rows ? a.pf_splits : a.splits;
-    if (splits <= 1) return;                       // the row is finished
     const float2 *ml = a.part_ml + row * a.part_stride;
-    float mx = -INFINITY, ls = 0.f;
-    for (int s = lane; s < splits; s += 32) mx = fmaxf(mx, ml[s].x);
-    mx = warp_max(mx);
-    const float mu = mx == -INFINITY ? 0.f : mx;
-    constexpr int W = D / 32;
-    float o[W];
+    float mx = -INFINITY, ls = 0.f, o[W];
 #pragma unroll
     for (int i = 0; i < W; ++i) o[i] = 0.f;
-    bool poison = false;
-    for (int s0 = 0; s0 < splits; s0 += 32) {
-        float f = 0.f, lw = 0.f;
-        if (s0 + lane < splits) {
-            const float2 x = ml[s0 + lane];
-            f = exp2f(x.x - mu);
-            lw = x.y * f;
-            if (x.y != x.y) poison = true;
-        }
-        ls += warp_sum(lw);
-        const int cnt = min(32, splits - s0);
-#pragma unroll 8
-        for (int s = 0; s < cnt; ++s) {
-            const float fs = __shfl_sync(0xffffffffu, f, s);
-            if (fs == 0.f) continue;
-            const float *p = a.part_o + (row * a.part_stride + s0 + s) * D + W * lane;
+    if (shares > 1) {
+        for (int s = lane; s < shares; s += 32) mx = fmaxf(mx, ml[s].x);
+        mx = warp_max(mx);
+        const float mu = mx == -INFINITY ? 0.f : mx;
+#pragma unroll 4
+        for (int s = w0; s < shares; s += WR) {
+            const float2 x = ml[s];
+            const float f = ex2(x.x - mu);         // 0 for a share without a visible key, whose part was not written
+            const float *p = a.part_o + (row * a.part_stride + s) * D + W * lane;
+            ls += x.y * f;
 #pragma unroll
-            for (int i = 0; i < W; ++i) o[i] += fs * p[i];
+            for (int i = 0; i < W; ++i) {
+                const float v = p[i];
+                o[i] += x.x == -INFINITY ? 0.f : f * v;
+            }
         }
     }
-    poison = __any_sync(0xffffffffu, poison);
-    const float inv = poison ? __int_as_float(0x7FC00000) : (ls == 0.f ? 0.f : 1.f / ls);
+    if constexpr (WR > 1) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) sm_o[warp][W * lane + i] = o[i];
+        if (lane == 0) sm_l[warp] = ls;
+        __syncthreads();
+        if (w0 > 0) return;
+        for (int k = 1; k < WR; ++k) {             // a NaN in any share stays one
+            ls += sm_l[warp + k];
+#pragma unroll
+            for (int i = 0; i < W; ++i) o[i] += sm_o[warp + k][W * lane + i];
+        }
+    }
+    if (shares <= 1) return;
+    const float inv = ls == 0.f ? 0.f : 1.f / ls;
     T *out = static_cast<T *>(a.out) + row * D + W * lane;
 #pragma unroll
     for (int i = 0; i < W; ++i) {
         if constexpr (std::is_same<T, __half>::value) out[i] = __float2half_rn(o[i] * inv);
         else out[i] = __float2bfloat16_rn(o[i] * inv);
     }
-    if (a.lse && lane == 0) a.lse[row] = poison ? inv : (ls == 0.f ? -INFINITY : (mx + log2f(ls)) * 0.69314718f);
+    if (a.lse && lane == 0) a.lse[row] = ls == 0.f ? -INFINITY : (mx + log2f(ls)) * 0.69314718f;
 }
 
 // ----------------------------------------------------------------------------------------------------------- host
@@ -391,7 +400,7 @@ constexpr size_t PART_BYTES_MAX = (size_t)64 << 20;   // partial results stay in
 
 struct KvAttnPlan {
     bool few, many;              // kernels that run
-    int nt, row_tiles, splits, pf_splits, part_stride, max_rows;
+    int nt, row_tiles, splits, pf_items, pf_splits, part_stride, max_rows;
     size_t part_o, bytes;
 };
 
@@ -432,11 +441,16 @@ static KvAttnPlan kv_plan(const v3g_kv_cache_t *c, const v3g_kv_batch_t *b, uint
         p.splits = s < 1 ? 1 : (s > 128 ? 128 : (int)s);
     }
     if (p.many) {
-        const uint64_t ctas = (longest * group + 255) / 256 * c->n_kv_heads * (p.few ? 1 : b->batch);
-        const uint64_t most = (seen(longest) + 1023) / 1024;                    // eight key tiles a share at least
-        uint64_t s = 148 / ctas;
+        // Units that have room in the grid, and about how many of them hold rows: sequences end within one.  Fewer than
+        // half the SMs: shares of the keys fill the others, eight key tiles each at least.  (Splitting what is left after whole
+        // rounds of the SMs was no gain: 216 units on 148 SMs, 78 us whole, 70 us and 6 us for the join with the last 68 in
+        // two.)
+        const uint64_t items = (uint64_t)b->n_tokens * group / PF_ROWS + b->batch, live = (items - b->batch / 2) * c->n_kv_heads;
+        const uint64_t most = (seen(longest) + 1023) / 1024;
+        uint64_t s = 148 / live;
         s = s > most ? most : s;
         s = s > room ? room : s;
+        p.pf_items = (int)items;
         p.pf_splits = s < 1 ? 1 : (s > 128 ? 128 : (int)s);
     }
     p.part_stride = p.splits > p.pf_splits ? p.splits : p.pf_splits;
@@ -454,12 +468,14 @@ static cudaError_t launch_attention_kernels(const KvAttnArgs &a, const KvAttnPla
     if (p.many) e = launch_kv_prefill(a, dtype, D, a.max_rows + 1, st);
     if (e == cudaSuccess && p.few) {
         const dim3 grid((uint32_t)((uint64_t)a.c.batch * a.c.heads * a.splits * a.row_tiles));
-        if (p.nt == 1) e = launch_k(false, k_kv_decode<T, D, 1>, grid, 32 * DEC_WARPS, 0, st, a);
-        else e = launch_k(false, k_kv_decode<T, D, 2>, grid, 32 * DEC_WARPS, 0, st, a);
+        if (p.nt == 1) e = launch_k(p.many, k_kv_decode<T, D, 1>, grid, 32 * DEC_WARPS, 0, st, a);
+        else e = launch_k(p.many, k_kv_decode<T, D, 2>, grid, 32 * DEC_WARPS, 0, st, a);
     }
     if (e != cudaSuccess || a.part_stride == 1) return e;
+    // four warps a row while rows are few
     const int64_t rows = (int64_t)a.c.n_tokens * a.c.heads * a.group;
-    return launch_k(true, k_kv_join<T, D>, dim3((uint32_t)((rows + 3) / 4)), 128, 0, st, a);
+    if (rows <= 148 * 16) return launch_k(true, k_kv_join<T, D, 4>, dim3((uint32_t)rows), 128, 0, st, a);
+    return launch_k(true, k_kv_join<T, D, 1>, dim3((uint32_t)((rows + 3) / 4)), 128, 0, st, a);
 }
 
 }  // namespace v3g
@@ -498,7 +514,8 @@ extern "C" int v3g_kv_attention(const v3g_kv_cache_t *cache, uint32_t layer, con
     const KvAttnPlan p = kv_plan(cache, batch, n_q_heads, max_q, max_kv, window, n_sink);
     if (p.bytes && (!dev_work || work_bytes < p.bytes)) return v3g_fail(V3G_E_SIZE, "v3g_kv_attention: workspace too small");
     if (p.bytes && reinterpret_cast<uintptr_t>(dev_work) % 256) return v3g_fail(V3G_E_ALIGN, "v3g_kv_attention: the workspace needs 256-byte alignment");
-    if ((uint64_t)batch->batch * cache->n_kv_heads * p.splits * p.row_tiles > 0x7FFFFFFFu)
+    if ((uint64_t)batch->batch * cache->n_kv_heads * p.splits * p.row_tiles > 0x7FFFFFFFu ||
+        (uint64_t)p.pf_items * cache->n_kv_heads * p.pf_splits > 0x7FFFFFFFu)
         return v3g_fail(V3G_E_LIMIT, "v3g_kv_attention: too many sequences and heads");
     a.q = q->data;
     a.q_tok = q->tok_stride;
@@ -513,7 +530,9 @@ extern "C" int v3g_kv_attention(const v3g_kv_cache_t *cache, uint32_t layer, con
     a.splits = p.splits;
     a.row_tiles = p.row_tiles;
     a.max_rows = p.max_rows;
+    a.pf_items = p.pf_items;
     a.pf_splits = p.pf_splits;
+    a.after_many = p.many && p.few;
     a.part_stride = p.part_stride;
     a.status = dev_status;
     a.part_ml = static_cast<float2 *>(dev_work);

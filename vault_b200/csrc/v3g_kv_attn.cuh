@@ -19,7 +19,8 @@ struct KvAttnArgs {
     // sequences of at most max_rows rows (tokens x group) are the few-row kernel's, the others the many-row kernel's
     int max_rows;
     int splits, row_tiles;     // few rows: key shares, row tiles in the grid
-    int pf_splits;             // many rows: key shares
+    int pf_items, pf_splits;   // many rows: units of 256 rows that a head has room for, key shares
+    bool after_many;           // the few-row kernel runs beside the many-row kernel and ends after it
     int part_stride;           // shares that a row has room for
     float2 *part_ml;           // [row][share] maximum (log2 units) and sum
     float *part_o;             // [row][share][D]
@@ -62,6 +63,8 @@ __device__ __forceinline__ float kv_scale_ref(float vs) {
     const uint32_t e = ((__float_as_uint(vs) + 0x7FFFFFu) >> 23) & 255u;
     return __uint_as_float(min(max(e, 7u), 247u) << 23);
 }
+
+constexpr int PF_ROWS = 256;   // rows of a many-row CTA
 
 // the many-row kernel over every sequence of at least min_rows rows (v3g_kv_prefill.cu)
 cudaError_t launch_kv_prefill(const KvAttnArgs &a, int dtype, int head_dim, int min_rows, cudaStream_t st);

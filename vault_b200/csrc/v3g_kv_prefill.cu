@@ -33,7 +33,7 @@
 
 namespace v3g {
 
-constexpr int PF_ROWS = 256, PF_KEYS = 128, PF_THREADS = 512;
+constexpr int PF_KEYS = 128, PF_THREADS = 512;
 // Ring of the tiles' places and scales.  Its writer is at most PF_AHEAD tiles past the converters' loads; they load tile t + 1
 // after tile t - 2's PV, which needed every softmax warp to be through with that tile's scales, so a slot is written again
 // only after its last reader.
@@ -148,7 +148,18 @@ __device__ __forceinline__ uint4 pf_convert8(uint32_t a, uint32_t b) {   // eigh
 }
 
 // a whole warp's bounded wait: one answer for all its lanes
-__device__ __forceinline__ bool pf_wait(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity)); }
+__device__ __forceinline__ bool pf_wait(uint32_t bar, uint32_t parity) {
+    for (uint32_t i = 0; i < tc::WAIT_LIMIT; ++i) {
+        uint32_t done;
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+            : "=r"(done)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (__all_sync(0xffffffffu, done)) return true;
+    }
+    return false;
+}
 // visible keys of 32 consecutive ones from kb, as a bit mask, for a row at position p
 __device__ __forceinline__ uint32_t pf_mask(const KvAttnArgs &a, int p, int kb, uint32_t pages) {
     auto below = [](int n) { return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1u); };   // the first n bits
@@ -163,11 +174,13 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + ((1024u - (tc::smem_addr(smem_raw) & 1023u)) & 1023u);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // the rows of this CTA; late tiles see the most keys and go first
+    griddep_launch();
+    // the rows of this CTA, and its share of their keys; late rows see the most keys and go first
+    const int shares = a.pf_splits, share = blockIdx.x % shares, unit = blockIdx.x / shares;
+    const int64_t item = a.pf_items - 1 - unit / a.c.heads;
+    const int h = unit % a.c.heads;
     int64_t base;
-    const int64_t item = gridDim.x - 1 - blockIdx.x;
     const int b = kv_find(a.c.q_start, a.c.batch, a.c.n_tokens, PF_ROWS, a.group, 1, item, base);
-    const int h = blockIdx.y;
     int first;
     const int n = a.c.tokens(b, first);
     const int64_t off = (item - base) * PF_ROWS;
@@ -178,7 +191,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
     const int plo = p0 + r0 / a.group, phi = p0 + (r0 + rn - 1) / a.group;
     const int all = kv_visible(a, plo, phi, PF_KEYS, sb, ws);
     // this CTA's share of the key tiles
-    const int per = (all + a.pf_splits - 1) / a.pf_splits, jlo = min((int)blockIdx.z * per, all), nk = min(per, all - jlo);
+    const int per = (all + shares - 1) / shares, jlo = min(share * per, all), nk = min(per, all - jlo);
     auto key0 = [&](int j) { return (j + jlo < sb ? j + jlo : j + jlo - sb + ws) * PF_KEYS; };
 
     const uint32_t bars = tc::smem_addr(smem + SM::BAR);
@@ -393,10 +406,10 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
                 ok = pf_wait(OFULL(tile), 0);
                 tc::tc_fence_after();
                 inv = places[(nk - 1) & (PF_RING - 1)].ref;
-                if (a.pf_splits == 1) inv = l == 0.f ? 0.f : inv / l;
+                if (shares == 1) inv = l == 0.f ? 0.f : inv / l;
             }
-            const int64_t part = out_row * a.part_stride + blockIdx.z;
-            if (ok && (nk > 0 || a.pf_splits == 1))   // an empty share has no accumulator
+            const int64_t part = out_row * a.part_stride + share;
+            if (ok && (nk > 0 || shares == 1))   // an empty share has no accumulator
 #pragma unroll 1
                 for (int c = 0; c < D / 16; ++c) {
                     uint32_t o[16];
@@ -410,12 +423,12 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
                         for (int i = 0; i < 16; i += 4) {
                             const float4 v = make_float4(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv,
                                                          __uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
-                            if (a.pf_splits > 1) kv_store4(a.part_o + part * D + 16 * c + i, v);
+                            if (shares > 1) kv_store4(a.part_o + part * D + 16 * c + i, v);
                             else kv_store4(static_cast<T *>(a.out) + out_row * D + 16 * c + i, v);
                         }
                 }
             if (live && ok) {
-                if (a.pf_splits > 1) a.part_ml[part] = make_float2(m, l);
+                if (shares > 1) a.part_ml[part] = make_float2(m, l);
                 else if (a.lse) a.lse[out_row] = l == 0.f ? -INFINITY : ((m == -INFINITY ? 0.f : m) + log2f(l)) * 0.69314718f;
             }
         }
@@ -594,8 +607,7 @@ static cudaError_t launch_pf(const KvAttnArgs &a, int min_rows, cudaStream_t st)
         if (e != cudaSuccess) return e;
         if (dev >= 0 && dev < 64) ready.fetch_or(1ull << dev);
     }
-    const int64_t items = (int64_t)a.c.n_tokens * a.group / PF_ROWS + a.c.batch;
-    return launch_k(false, kern, dim3((uint32_t)items, a.c.heads, a.pf_splits), PF_THREADS, PfSmem<D>::BYTES, st, a, min_rows);
+    return launch_k(false, kern, dim3((uint32_t)((uint64_t)a.pf_items * a.c.heads * a.pf_splits)), PF_THREADS, PfSmem<D>::BYTES, st, a, min_rows);
 }
 
 cudaError_t launch_kv_prefill(const KvAttnArgs &a, int dtype, int head_dim, int min_rows, cudaStream_t st) {
