@@ -3,8 +3,8 @@
 //   score(k, t) = (logit[k][t] - lse_k) + scores[k],   lse_k = max + log(sum exp(logit - max))
 //
 // The logits are read once (4 bytes and an exponential per element: HBM bounds it).  Inside a beam the order of the
-// scores is the order of the logits, so the first kernel needs no lse: a CTA keeps 4,096 logits of one beam in
-// registers, reduces their maximum and sum of exponentials, and writes its `beams` best as 64-bit keys (value, then lower
+// scores is the order of the logits, so the first kernel needs no lse: a CTA keeps a slice of 4,096 or 8,192 logits of
+// one beam in registers, reduces their maximum and sum of exponentials, and writes its `beams` best as 64-bit keys (value, then lower
 // index).  The second kernel joins the sums of a beam, scores the beams x slices x beams keys and selects again.  Both
 // selections are exact: the smallest of at least `beams` group maxima bounds the answer from below, the few values at or
 // above it are collected and ranked by counting, and a slice that holds too many of them (long ties, sorted logits)
@@ -14,7 +14,7 @@
 
 namespace v3g {
 
-constexpr int BEAM_THREADS = 256, BEAM_EPT = 16, BEAM_SLICE = BEAM_THREADS * BEAM_EPT;
+constexpr int BEAM_THREADS = 256;
 constexpr int BEAM_BUF = 256;   // collected keys that are ranked by counting
 
 typedef unsigned long long u64;
@@ -77,6 +77,7 @@ __device__ __forceinline__ void beam_best(BeamShared &sm, int beams, uint32_t bo
         if ((int)threadIdx.x < n) {
             const u64 k = sm.buf[threadIdx.x];
             int rank = 0;
+#pragma unroll 8
             for (int i = 0; i < n; ++i) rank += sm.buf[i] > k;
             if (rank < beams) emit(rank, k);
         }
@@ -104,52 +105,57 @@ __device__ __forceinline__ float beam_value<__half>(__half x) { return __half2fl
 template <>
 __device__ __forceinline__ float beam_value<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-template <typename T>
-__global__ void __launch_bounds__(BEAM_THREADS) k_beam_slice(const T *logits, int64_t ld, int vocab, int beams, bool vec, u64 *keys,
-                                                            float2 *sums) {
+__device__ __forceinline__ float beam_ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+template <typename T, int EPT>
+__global__ void __launch_bounds__(BEAM_THREADS, EPT == 32 ? 4 : 6) k_beam_slice(const T *logits, int64_t ld, int vocab, int beams, bool vec,
+                                                                               u64 *keys, float2 *sums) {
     __shared__ BeamShared sm;
     __shared__ float red[BEAM_THREADS / 32];
     griddep_launch();
+    constexpr int SLICE = BEAM_THREADS * EPT, W = 16 / sizeof(T), NL = EPT / W;   // elements of a 16-byte load, loads of a thread
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int64_t row = blockIdx.y;
-    const int i0 = blockIdx.x * BEAM_SLICE;
+    const int i0 = blockIdx.x * SLICE + tid * W;
     const T *p = logits + row * ld;
-    constexpr int W = 16 / sizeof(T), NL = BEAM_EPT / W;          // elements of a 16-byte load, loads of a thread
-    float x[BEAM_EPT];
-    auto index = [&](int e) { return i0 + ((e / W) * BEAM_THREADS + tid) * W + e % W; };
-    if (vec && i0 + BEAM_SLICE <= vocab) {
+    float x[EPT];
+    auto index = [&](int e) { return i0 + (e / W) * (BEAM_THREADS * W) + e % W; };
+    if (vec && (int)(blockIdx.x + 1) * SLICE <= vocab) {
         uint4 u[NL];
 #pragma unroll
         for (int i = 0; i < NL; ++i) u[i] = ldg_stream16(p + index(i * W));
 #pragma unroll
-        for (int e = 0; e < BEAM_EPT; ++e) x[e] = beam_value(reinterpret_cast<const T *>(&u[e / W])[e % W]);
+        for (int e = 0; e < EPT; ++e) x[e] = beam_value(reinterpret_cast<const T *>(&u[e / W])[e % W]);
     } else {
 #pragma unroll
-        for (int e = 0; e < BEAM_EPT; ++e) x[e] = index(e) < vocab ? beam_value(p[index(e)]) : -INFINITY;
+        for (int e = 0; e < EPT; ++e) x[e] = index(e) < vocab ? beam_value(p[index(e)]) : -INFINITY;
     }
-    float top = -INFINITY;
+    float mine = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < BEAM_EPT; ++e) {
-        if (x[e] != x[e]) x[e] = -INFINITY;                       // a NaN is no continuation
-        top = fmaxf(top, x[e]);
-    }
-    const float bound = beam_bound(sm, top, beams);
-    top = sm.group[lane];
+    for (int e = 0; e < EPT; ++e) mine = fmaxf(mine, x[e]);       // NaN logits are passed over
+    const float bound = beam_bound(sm, mine, beams);
+    float top = sm.group[lane];
     if (lane >= (beams <= 8 ? 8 : (beams <= 16 ? 16 : 32))) top = -INFINITY;
-    top = warp_max(top);                                          // the block's maximum
+    top = warp_max(top);                                          // the slice's maximum
+    // Sum of 2^((x - top) log2 e).  The difference comes first: logits at the type's lowest value would leave its range as
+    // products.  Hidden and NaN logits end at 2^-200 = 0, and so does a slice whose maximum is infinite.
     float sum = 0.f;
-    if (top > -INFINITY)
 #pragma unroll
-        for (int e = 0; e < BEAM_EPT; ++e) sum += __expf(x[e] - top);
+    for (int e = 0; e < EPT; ++e) sum += beam_ex2(fmaxf((x[e] - top) * 1.44269504f, -200.f));
     sum = warp_sum(sum);
     if (lane == 0) red[warp] = sum;
     const int64_t slice = row * gridDim.x + blockIdx.x;
     beam_best(
         sm, beams, float_key(bound),
         [&](auto f) {
+            if (mine >= bound)                                    // few threads hold one of the best
 #pragma unroll
-            for (int e = 0; e < BEAM_EPT; ++e)
-                if (x[e] > -INFINITY && x[e] < INFINITY) f(((u64)float_key(x[e]) << 32) | (0xFFFFFFFFu - (uint32_t)index(e)));
+                for (int e = 0; e < EPT; ++e)
+                    if (x[e] > -INFINITY && x[e] < INFINITY) f(((u64)float_key(x[e]) << 32) | (0xFFFFFFFFu - (uint32_t)index(e)));
         },
         [&](int rank, u64 k) { keys[slice * beams + rank] = k; });
     if (tid == 0) {   // red was written before beam_best's barrier
@@ -160,7 +166,7 @@ __global__ void __launch_bounds__(BEAM_THREADS) k_beam_slice(const T *logits, in
 }
 
 struct BeamArgs {
-    const u64 *keys;
+    u64 *keys;          // the slices' best; the join scores them in place
     const float2 *sums;
     const float *scores;
     const uint8_t *finished;
@@ -172,45 +178,65 @@ struct BeamArgs {
 
 __global__ void __launch_bounds__(BEAM_THREADS) k_beam_join(const __grid_constant__ BeamArgs a) {
     __shared__ BeamShared sm;
-    __shared__ float lse[V3G_BEAM_MAX], run[V3G_BEAM_MAX];
+    __shared__ u64 only[V3G_BEAM_MAX];
     __shared__ bool done[V3G_BEAM_MAX];
     griddep_wait();
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, K = a.beams;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, K = a.beams, per = a.slices * K;
     const int64_t g0 = (int64_t)blockIdx.x * K;
+    // a warp takes a beam: its logsumexp, then the scores of its slices' best
+    uint32_t top = 0;
     for (int k = warp; k < K; k += BEAM_THREADS / 32) {
         const float2 *p = a.sums + (g0 + k) * a.slices;
+        u64 *keys = a.keys + (g0 + k) * per;
+        const float run_k = a.scores[g0 + k];
+        const bool done_k = a.finished && a.finished[g0 + k];
+        u64 ahead[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ahead[i] = lane + 32 * i < per ? keys[lane + 32 * i] : 0ull;
         float m = -INFINITY;
         for (int i = lane; i < a.slices; i += 32) m = fmaxf(m, p[i].x);
         m = warp_max(m);
         float s = 0.f;
         for (int i = lane; i < a.slices; i += 32) {
             const float2 v = p[i];
-            if (v.x > -INFINITY) s += v.y * __expf(v.x - m);
+            if (v.x > -INFINITY) s += v.y * beam_ex2((v.x - m) * 1.44269504f);
         }
-        s = warp_sum(s);
+        const float lse = m + logf(warp_sum(s));
+        auto score = [&](u64 key) -> u64 {
+            const float y = (key_float((uint32_t)(key >> 32)) - lse) + run_k;
+            if (done_k || !key || !(y > -INFINITY && y < INFINITY)) return 0ull;
+            return ((u64)float_key(y) << 32) | (0xFFFFFFFFu - ((uint32_t)k * (uint32_t)a.vocab + (0xFFFFFFFFu - (uint32_t)key)));
+        };
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (lane + 32 * i < per) {
+                const u64 y = score(ahead[i]);
+                keys[lane + 32 * i] = y;
+                top = max(top, (uint32_t)(y >> 32));
+            }
+        for (int i = lane + 128; i < per; i += 32) {
+            const u64 y = score(keys[i]);
+            keys[i] = y;
+            top = max(top, (uint32_t)(y >> 32));
+        }
+        // a finished beam's one continuation
+        const bool goes_on = done_k && a.eos >= 0 && run_k > -INFINITY && run_k < INFINITY;
         if (lane == 0) {
-            lse[k] = m + logf(s);
-            run[k] = a.scores[g0 + k];
-            done[k] = a.finished && a.finished[g0 + k];
+            done[k] = done_k;
+            only[k] = goes_on ? ((u64)float_key(run_k) << 32) | (0xFFFFFFFFu - ((uint32_t)k * (uint32_t)a.vocab + (uint32_t)a.eos)) : 0ull;
+            if (goes_on) top = max(top, float_key(run_k));
         }
     }
-    __syncthreads();
-    const int per = a.slices * K, total = per * K;
-    const u64 *keys = a.keys + g0 * per;
-    auto each = [&](auto f) {
-        for (int i = tid; i < total; i += BEAM_THREADS) {
-            const int k = i / per;
-            const u64 key = done[k] ? 0ull : keys[i];
-            if (!key) continue;
-            const float s = (key_float((uint32_t)(key >> 32)) - lse[k]) + run[k];
-            const uint32_t token = 0xFFFFFFFFu - (uint32_t)key;
-            if (s > -INFINITY && s < INFINITY) f(((u64)float_key(s) << 32) | (0xFFFFFFFFu - ((uint32_t)k * (uint32_t)a.vocab + token)));
+    auto each = [&](auto f) {   // every thread its own keys again
+        for (int k = warp; k < K; k += BEAM_THREADS / 32) {
+            const u64 *keys = a.keys + (g0 + k) * per;
+            for (int i = lane; i < per; i += 32) {
+                const u64 y = keys[i];
+                if (y) f(y);
+            }
+            if (lane == 0 && only[k]) f(only[k]);
         }
-        if (tid < K && done[tid] && a.eos >= 0 && run[tid] > -INFINITY && run[tid] < INFINITY)
-            f(((u64)float_key(run[tid]) << 32) | (0xFFFFFFFFu - ((uint32_t)tid * (uint32_t)a.vocab + (uint32_t)a.eos)));
     };
-    uint32_t top = 0;
-    each([&](u64 k) { top = max(top, (uint32_t)(k >> 32)); });
     const float bound = beam_bound(sm, top ? key_float(top) : -INFINITY, K);
     beam_best(sm, K, float_key(bound), each, [&](int rank, u64 k) {
         const int64_t at = g0 + rank;
@@ -231,23 +257,30 @@ __global__ void __launch_bounds__(BEAM_THREADS) k_beam_join(const __grid_constan
 }
 
 struct BeamPlan {
+    bool wide;          // slices of 8,192
     int slices;
     size_t keys, bytes;
 };
+// Wide slices cost less beside their data; narrow ones keep small steps spread over the SMs (one request of four beams
+// over 151,936 tokens: 76 wide slices, 152 narrow ones).
 static BeamPlan beam_plan(uint64_t rows, uint32_t beams, uint32_t vocab) {
     BeamPlan p;
-    p.slices = (int)(((uint64_t)vocab + BEAM_SLICE - 1) / BEAM_SLICE);
+    p.wide = rows * ((vocab + 8191) / 8192) >= 148 * 4;
+    const uint32_t slice = p.wide ? 8192 : 4096;
+    p.slices = (int)(((uint64_t)vocab + slice - 1) / slice);
     p.keys = (rows * p.slices * sizeof(float2) + 255) & ~(size_t)255;
     p.bytes = p.keys + rows * p.slices * beams * sizeof(u64);
     return p;
 }
 
 template <typename T>
-static cudaError_t launch_slices(const void *logits, int64_t ld, int vocab, int beams, int slices, uint32_t rows, u64 *keys, float2 *sums,
-                                 cudaStream_t st) {
+static cudaError_t launch_slices(const void *logits, int64_t ld, int vocab, int beams, const BeamPlan &p, uint32_t rows, u64 *keys,
+                                 float2 *sums, cudaStream_t st) {
     const bool vec = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && ld * sizeof(T) % 16 == 0;
-    return launch_k(false, k_beam_slice<T>, dim3(slices, rows), BEAM_THREADS, 0, st, static_cast<const T *>(logits), ld, vocab, beams, vec,
-                    keys, sums);
+    const dim3 grid(p.slices, rows);
+    const T *x = static_cast<const T *>(logits);
+    if (p.wide) return launch_k(false, k_beam_slice<T, 32>, grid, BEAM_THREADS, 0, st, x, ld, vocab, beams, vec, keys, sums);
+    return launch_k(false, k_beam_slice<T, 16>, grid, BEAM_THREADS, 0, st, x, ld, vocab, beams, vec, keys, sums);
 }
 
 }  // namespace v3g
@@ -294,9 +327,9 @@ extern "C" int v3g_beam_select(const void *dev_logits, int dtype, uint32_t group
     a.finished_out = finished_out;
     const cudaStream_t st = (cudaStream_t)stream;
     cudaError_t e;
-    if (dtype == V3G_F32) e = launch_slices<float>(dev_logits, (int64_t)ld, (int)vocab, (int)beams, p.slices, rows, keys, sums, st);
-    else if (dtype == V3G_F16) e = launch_slices<__half>(dev_logits, (int64_t)ld, (int)vocab, (int)beams, p.slices, rows, keys, sums, st);
-    else e = launch_slices<__nv_bfloat16>(dev_logits, (int64_t)ld, (int)vocab, (int)beams, p.slices, rows, keys, sums, st);
+    if (dtype == V3G_F32) e = launch_slices<float>(dev_logits, (int64_t)ld, (int)vocab, (int)beams, p, rows, keys, sums, st);
+    else if (dtype == V3G_F16) e = launch_slices<__half>(dev_logits, (int64_t)ld, (int)vocab, (int)beams, p, rows, keys, sums, st);
+    else e = launch_slices<__nv_bfloat16>(dev_logits, (int64_t)ld, (int)vocab, (int)beams, p, rows, keys, sums, st);
     if (e == cudaSuccess) e = launch_k(true, k_beam_join, dim3(groups), BEAM_THREADS, 0, st, a);
     return e == cudaSuccess ? V3G_OK : v3g_fail(V3G_E_CUDA, std::string("v3g_beam_select: ") + cudaGetErrorString(e));
 }

@@ -28,132 +28,166 @@ struct AppendArgs {
     int q_heads, rope_rows;
     const float *rope;                                     // [rope_rows][D / 2 cos | D / 2 sin], null: no rotation
     int32_t *status;
-    bool k_vec, v_vec, q_vec;
+    bool vec;                                              // every row starts on 8 bytes
 };
 
-// A lane's consecutive elements of a row: 16 bytes of them
-template <typename T>
+// A lane's elements of a row: H consecutive ones of the first half and their rotation partners, D / 2 further on, so that a
+// pair is in one lane
+template <typename T, int D>
 struct Piece {
-    static constexpr int N = 16 / sizeof(T);
-    float x[N];
+    static constexpr int H = 8 / sizeof(T), LR = D / 2 / H;   // 8 bytes of each half; lanes of a row
+    float x[2][H];
     __device__ __forceinline__ void zero() {
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = 0.f;
+        for (int i = 0; i < H; ++i) x[0][i] = x[1][i] = 0.f;
     }
-    __device__ __forceinline__ void load(const T *p, bool vec) {
-        T e[N];
-        if (vec) *reinterpret_cast<uint4 *>(e) = ldg_stream16(p);
-        else
+    template <bool VEC>
+    __device__ __forceinline__ void load(const T *p) {   // p: the lane's first element
+        T e[2][H];
 #pragma unroll
-            for (int i = 0; i < N; ++i) e[i] = p[i];
+        for (int k = 0; k < 2; ++k) {
+            if constexpr (VEC) *reinterpret_cast<uint2 *>(e[k]) = ldg_stream8(p + k * (D / 2));
+            else
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            if constexpr (std::is_same<T, float>::value) x[i] = e[i];
-            else if constexpr (std::is_same<T, __half>::value) x[i] = __half2float(e[i]);
-            else x[i] = __bfloat162float(e[i]);
+                for (int i = 0; i < H; ++i) e[k][i] = p[k * (D / 2) + i];
+#pragma unroll
+            for (int i = 0; i < H; ++i) {
+                if constexpr (std::is_same<T, float>::value) x[k][i] = e[k][i];
+                else if constexpr (std::is_same<T, __half>::value) x[k][i] = __half2float(e[k][i]);
+                else x[k][i] = __bfloat162float(e[k][i]);
+            }
         }
     }
     __device__ __forceinline__ void store(T *p) const {
-        uint4 r;
-        T *e = reinterpret_cast<T *>(&r);
 #pragma unroll
-        for (int i = 0; i < N; i += 4) kv_store4(e + i, make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]));
-        *reinterpret_cast<uint4 *>(p) = r;
+        for (int k = 0; k < 2; ++k) {
+            uint2 r;
+            T *e = reinterpret_cast<T *>(&r);
+            if constexpr (std::is_same<T, float>::value)
+#pragma unroll
+                for (int i = 0; i < H; ++i) e[i] = x[k][i];
+            else kv_store4(e, make_float4(x[k][0], x[k][1], x[k][2], x[k][3]));
+            *reinterpret_cast<uint2 *>(p + k * (D / 2)) = r;
+        }
+    }
+    // x1 c - x2 s; x2 c + x1 s, every product and sum rounded by itself
+    __device__ __forceinline__ void rotate(const float *cs, int l) {
+        float c[H], s[H];
+        if constexpr (H == 4) {
+            *reinterpret_cast<float4 *>(c) = *reinterpret_cast<const float4 *>(cs + 4 * l);
+            *reinterpret_cast<float4 *>(s) = *reinterpret_cast<const float4 *>(cs + D / 2 + 4 * l);
+        } else {
+            *reinterpret_cast<float2 *>(c) = *reinterpret_cast<const float2 *>(cs + 2 * l);
+            *reinterpret_cast<float2 *>(s) = *reinterpret_cast<const float2 *>(cs + D / 2 + 2 * l);
+        }
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+            const float a = x[0][i], b = x[1][i];
+            x[0][i] = __fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, s[i]));
+            x[1][i] = __fadd_rn(__fmul_rn(b, c[i]), __fmul_rn(a, s[i]));
+        }
     }
 };
 
-// The rotation of lane l's piece of a row: pairs i, i + D/2 sit LR / 2 lanes apart.  x1 c - x2 s; x2 c + x1 s, every product and
-// sum rounded by itself.
-template <typename T, int D>
-__device__ __forceinline__ void rotate(Piece<T> &x, const float *cs, int l, bool turn) {
-    constexpr int N = Piece<T>::N, LR = D / N;
-    const bool low = l < LR / 2;
-    const float *c = cs + N * (l % (LR / 2));
-#pragma unroll
-    for (int i = 0; i < N; i += 4) {
-        const float4 c4 = *reinterpret_cast<const float4 *>(c + i), s4 = *reinterpret_cast<const float4 *>(c + D / 2 + i);
-        const float cc[4] = {c4.x, c4.y, c4.z, c4.w}, ss[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float o = __shfl_xor_sync(0xffffffffu, x.x[i + k], LR / 2);
-            if (turn) x.x[i + k] = __fadd_rn(__fmul_rn(x.x[i + k], cc[k]), __fmul_rn(o, low ? -ss[k] : ss[k]));
-        }
-    }
-}
-__device__ __forceinline__ uint32_t code_byte(float x, float inv) {
-    return (uint32_t)((int)rintf(fminf(fmaxf(__fmul_rn(x, inv), -127.f), 127.f)) + 128);
-}
-__device__ __forceinline__ uint32_t moved_codes(uint32_t w, float ratio) {
-    uint32_t r = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        r |= (uint32_t)((int)rintf(__fmul_rn((float)((int)((w >> (8 * i)) & 255u) - 128), ratio)) + 128) << (8 * i);
+__device__ __forceinline__ float max_nan(float a, float b) {   // a NaN wins
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
+}
+// rint(x inv) + 128 in the low byte: adding 1.5 x 2^23 rounds to the nearest even integer.  |x inv| is at most 127 and a few
+// 2^-24 of it, so no clamp is needed.
+__device__ __forceinline__ uint32_t code_bits(float x, float inv) { return __float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.f + 128.f)); }
+__device__ __forceinline__ uint32_t pack_bytes(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x0040u); }
+
+__device__ __forceinline__ uint32_t moved_code(uint32_t c, float ratio) {
+    return (uint32_t)((int)rintf(__fmul_rn((float)((int)c - 128), ratio)) + 128);
 }
 
 // one head's rows [s0, s1) of a block: the rounding described above.  cs: the rotation's rows, from row s0's on
-template <typename T, int D>
-__device__ __forceinline__ void append_rows(const T *src, int64_t tok_ld, bool vec, const float *cs, bool turn, int s0, int s1,
+template <typename T, int D, bool VEC>
+__device__ __forceinline__ void append_rows(const T *src, int64_t tok_ld, const float *cs, bool turn, int s0, int s1,
                                             uint8_t *codes, float *scale, int lane) {
-    constexpr int N = Piece<T>::N, LR = D / N, RP = 32 / LR, NP = KV_BLOCK / RP;   // lanes of a row, rows of a pass, passes
-    const int l = lane % LR, sub = lane / LR;
+    typedef Piece<T, D> P;
+    constexpr int H = P::H, RP = 32 / P::LR, NP = KV_BLOCK / RP;   // rows of a pass, passes
+    const int l = lane % P::LR, sub = lane / P::LR;
     const float s_old = s0 > 0 ? *scale : 0.f;
-    Piece<T> x[NP];
+    P x[NP];
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
         const int r = s0 + i * RP + sub;
         x[i].zero();
-        if (r < s1) x[i].load(src + (int64_t)(r - s0) * tok_ld + N * l, vec);
+        if (r < s1) x[i].template load<VEC>(src + (int64_t)(r - s0) * tok_ld + H * l);
     }
     float top = 0.f;
-    bool bad = false;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
         const int r = s0 + i * RP + sub;
         if (s0 + i * RP >= s1) break;   // uniform over the warp
-        if (turn) rotate<T, D>(x[i], cs + (r < s1 ? r - s0 : 0) * D, l, r < s1);
+        if (turn && r < s1) x[i].rotate(cs + (r - s0) * D, l);
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
-            top = fmaxf(top, fabsf(x[i].x[k]));
-            bad |= !(fabsf(x[i].x[k]) <= FLT_MAX);
-        }
+        for (int k = 0; k < H; ++k) top = max_nan(max_nan(top, fabsf(x[i].x[0][k])), fabsf(x[i].x[1][k]));
     }
-    top = warp_max(top);
-    bad = __any_sync(0xffffffffu, bad) || s_old != s_old;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const bool bad = !(top <= FLT_MAX) || s_old != s_old;
     float s = fmaxf(s_old, __fmul_rn(top, 1.f / 127.f));
     if (s < KV_SCALE_MIN) s = 0.f;
     if (bad) s = __int_as_float(0x7FC00000);   // the block holds a NaN or an infinity: it reads as NaN
     const float inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
     if (s0 > 0 && s != s_old) {
         const float ratio = s > 0.f ? __fdiv_rn(s_old, s) : 0.f;
-        for (int r = sub; r < s0; r += RP) {
-            uint32_t *p = reinterpret_cast<uint32_t *>(codes + r * D + N * l);
-#pragma unroll
-            for (int k = 0; k < N / 4; ++k) p[k] = moved_codes(p[k], ratio);
+        for (int i = lane; i < s0 * D / 4; i += 32) {
+            uint32_t *p = reinterpret_cast<uint32_t *>(codes) + i;
+            const uint32_t w = *p;
+            *p = moved_code(w & 255u, ratio) | moved_code(w >> 8 & 255u, ratio) << 8 | moved_code(w >> 16 & 255u, ratio) << 16 |
+                 moved_code(w >> 24, ratio) << 24;
         }
     }
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
         const int r = s0 + i * RP + sub;
         if (r < s1) {
-            uint32_t w[N / 4];
 #pragma unroll
-            for (int k = 0; k < N / 4; ++k) {
-                const float *y = x[i].x + 4 * k;
-                w[k] = bad ? 0x80808080u
-                           : code_byte(y[0], inv) | code_byte(y[1], inv) << 8 | code_byte(y[2], inv) << 16 | code_byte(y[3], inv) << 24;
+            for (int k = 0; k < 2; ++k) {
+                const float *y = x[i].x[k];
+                uint8_t *p = codes + r * D + k * (D / 2) + H * l;
+                const uint32_t lo = pack_bytes(code_bits(y[0], inv), code_bits(y[1], inv));
+                if constexpr (H == 4) {
+                    const uint32_t hi = pack_bytes(code_bits(y[2], inv), code_bits(y[3], inv));
+                    *reinterpret_cast<uint32_t *>(p) = bad ? 0x80808080u : __byte_perm(lo, hi, 0x5410u);
+                } else {
+                    *reinterpret_cast<uint16_t *>(p) = bad ? 0x8080u : (uint16_t)lo;
+                }
             }
-            uint32_t *p = reinterpret_cast<uint32_t *>(codes + r * D + N * l);
-            if constexpr (N == 8) *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
-            else *p = w[0];
         }
     }
     __syncwarp();
     if (lane == 0) *scale = s;
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(32 * APPEND_WARPS) k_kv_append(const __grid_constant__ AppendArgs a) {
+// one query head's rows of a block, rotated and not rounded further than their own type; rows past `placed` become zero
+template <typename T, int D, bool VEC>
+__device__ __forceinline__ void turn_rows(const T *src, int64_t tok_ld, const float *cs, bool turn, int rows, int placed, T *out,
+                                          int64_t out_ld, int lane) {
+    typedef Piece<T, D> P;
+    constexpr int RP = 32 / P::LR, NP = KV_BLOCK / RP;
+    const int l = lane % P::LR, sub = lane / P::LR;
+    P x[NP];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        x[i].zero();
+        if (i * RP + sub < placed) x[i].template load<VEC>(src + (int64_t)(i * RP + sub) * tok_ld + P::H * l);
+    }
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        const int r = i * RP + sub;
+        if (turn && r < placed) x[i].rotate(cs + r * D, l);
+        if (r < rows) x[i].store(out + r * out_ld + P::H * l);
+    }
+}
+
+template <typename T, int D, bool VEC>
+__global__ void __launch_bounds__(32 * APPEND_WARPS, 5) k_kv_append(const __grid_constant__ AppendArgs a) {
     __shared__ __align__(16) float cs[KV_BLOCK * D];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int64_t base;
@@ -176,39 +210,21 @@ __global__ void __launch_bounds__(32 * APPEND_WARPS) k_kv_append(const __grid_co
         for (int i = threadIdx.x; i < placed * D / 4; i += 32 * APPEND_WARPS) reinterpret_cast<float4 *>(cs)[i] = __ldg(src + i);
         __syncthreads();
     }
-    const int heads = a.c.heads, step = APPEND_WARPS * gridDim.y, w0 = blockIdx.y * APPEND_WARPS + warp;
-    if (page >= 0 && placed > 0)
-        for (int t = w0; t < 2 * heads; t += step) {
-            const bool is_v = t >= heads;
-            const int h = is_v ? t - heads : t;
-            const int64_t at = a.c.block(page, h, lo);
-            const T *src = is_v ? static_cast<const T *>(a.v) + (int64_t)t0 * a.v_tok + (int64_t)h * a.v_head
-                                : static_cast<const T *>(a.k) + (int64_t)t0 * a.k_tok + (int64_t)h * a.k_head;
-            append_rows<T, D>(src, is_v ? a.v_tok : a.k_tok, is_v ? a.v_vec : a.k_vec, cs, turn && !is_v, s0, s0 + placed,
-                              (is_v ? a.c.v : a.c.k) + at * (KV_BLOCK * D), (is_v ? a.c.vs : a.c.ks) + at, lane);
+    // a warp takes the block's rows of one head at a time: the query heads, then K, then V
+    const int heads = a.c.heads, step = APPEND_WARPS * gridDim.y;
+    for (int t = blockIdx.y * APPEND_WARPS + warp; t < a.q_heads + 2 * heads; t += step) {
+        if (t < a.q_heads) {
+            turn_rows<T, D, VEC>(static_cast<const T *>(a.q) + (int64_t)t0 * a.q_tok + (int64_t)t * a.q_head, a.q_tok, cs, turn, nt, placed,
+                            static_cast<T *>(a.q_out) + ((int64_t)t0 * a.q_heads + t) * D, (int64_t)a.q_heads * D, lane);
+            continue;
         }
-    if (a.q) {   // the queries of the same tokens: rotated, not rounded further than their own type
-        constexpr int N = Piece<T>::N, LR = D / N, RP = 32 / LR, U = 4;
-        const int l = lane % LR, sub = lane / LR, rows = nt * a.q_heads;
-        // shares of the warps that hold no K/V row come first
-        const int w1 = (w0 + step - 2 * heads % step) % step;
-        for (int r0 = w1 * RP * U; r0 < rows; r0 += step * RP * U) {
-            Piece<T> x[U];
-            int tok[U], h[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int r = r0 + u * RP + sub;
-                tok[u] = r / a.q_heads, h[u] = r - tok[u] * a.q_heads;
-                x[u].zero();
-                if (r < rows && tok[u] < placed)
-                    x[u].load(static_cast<const T *>(a.q) + (int64_t)(t0 + tok[u]) * a.q_tok + (int64_t)h[u] * a.q_head + N * l, a.q_vec);
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (turn) rotate<T, D>(x[u], cs + (tok[u] < placed ? tok[u] : 0) * D, l, tok[u] < placed);
-                if (tok[u] < nt) x[u].store(static_cast<T *>(a.q_out) + ((int64_t)(t0 + tok[u]) * a.q_heads + h[u]) * D + N * l);
-            }
-        }
+        if (page < 0 || placed == 0) continue;
+        const int kind = t - a.q_heads >= heads, h = t - a.q_heads - kind * heads;
+        const int64_t at = a.c.block(page, h, lo);
+        const T *src = kind ? static_cast<const T *>(a.v) + (int64_t)t0 * a.v_tok + (int64_t)h * a.v_head
+                            : static_cast<const T *>(a.k) + (int64_t)t0 * a.k_tok + (int64_t)h * a.k_head;
+        append_rows<T, D, VEC>(src, kind ? a.v_tok : a.k_tok, cs, turn && !kind, s0, s0 + placed,
+                          (kind ? a.c.v : a.c.k) + at * (KV_BLOCK * D), (kind ? a.c.vs : a.c.ks) + at, lane);
     }
 }
 
@@ -411,16 +427,21 @@ static int launched(const char *who) {
 
 static size_t dtype_bytes(int t) { return t == V3G_F32 ? 4 : 2; }
 
-// 16-byte loads of rows: the base and both strides keep that alignment
+// 8-byte loads of rows: the base and both strides keep that alignment
 static bool rows_vec(const v3g_rows_t &r, int dtype) {
-    const int64_t n = 16 / (int64_t)dtype_bytes(dtype);
-    return aligned_to(r.data, 16) && r.tok_stride % n == 0 && r.head_stride % n == 0;
+    const int64_t n = 8 / (int64_t)dtype_bytes(dtype);
+    return aligned_to(r.data, 8) && r.tok_stride % n == 0 && r.head_stride % n == 0;
 }
 
 template <typename T>
 static void launch_append(const AppendArgs &a, int D, dim3 grid, cudaStream_t st) {
-    if (D == 64) k_kv_append<T, 64><<<grid, 32 * APPEND_WARPS, 0, st>>>(a);
-    else k_kv_append<T, 128><<<grid, 32 * APPEND_WARPS, 0, st>>>(a);
+    if (a.vec) {
+        if (D == 64) k_kv_append<T, 64, true><<<grid, 32 * APPEND_WARPS, 0, st>>>(a);
+        else k_kv_append<T, 128, true><<<grid, 32 * APPEND_WARPS, 0, st>>>(a);
+    } else {
+        if (D == 64) k_kv_append<T, 64, false><<<grid, 32 * APPEND_WARPS, 0, st>>>(a);
+        else k_kv_append<T, 128, false><<<grid, 32 * APPEND_WARPS, 0, st>>>(a);
+    }
 }
 
 template <typename T>
@@ -460,13 +481,11 @@ extern "C" int v3g_kv_append(const v3g_kv_cache_t *cache, uint32_t layer, const 
     a.k_head = k->head_stride;
     a.v_tok = v->tok_stride;
     a.v_head = v->head_stride;
-    a.k_vec = rows_vec(*k, dtype);
-    a.v_vec = rows_vec(*v, dtype);
+    a.vec = rows_vec(*k, dtype) && rows_vec(*v, dtype) && (!q || rows_vec(*q, dtype));
     if (q) {
         a.q = q->data;
         a.q_tok = q->tok_stride;
         a.q_head = q->head_stride;
-        a.q_vec = rows_vec(*q, dtype);
         a.q_heads = (int)n_q_heads;
         a.q_out = q_out;
     }
@@ -476,7 +495,7 @@ extern "C" int v3g_kv_append(const v3g_kv_cache_t *cache, uint32_t layer, const 
     const uint32_t items = batch->n_tokens / KV_BLOCK + 2 * batch->batch;
     // A block's heads are shared out over CTAs until the warps of the whole GPU have a few rows each (6,000 tokens, 32/8
     // heads: one CTA a block 218 us, four NNN us); past one pass of the warps over the rows there is nothing left to share.
-    const uint32_t passes = (2 * cache->n_kv_heads + (q ? n_q_heads * 2 : 0) + APPEND_WARPS - 1) / APPEND_WARPS;
+    const uint32_t passes = (2 * cache->n_kv_heads + (q ? n_q_heads : 0) + APPEND_WARPS - 1) / APPEND_WARPS;
     uint32_t ny = (148 * 16 + items - 1) / items;
     ny = ny > passes ? passes : ny;
     const dim3 grid(items, ny);

@@ -13,8 +13,9 @@
 //   fp16 integers exactly (byte permute to 1024 + c, minus 1152).  fp16 queries enter as they are, bf16 queries as fp16
 //   after an exact power of two per row that puts the largest magnitude in [2^13, 2^14).
 // * The K scale of the block multiplies the scores, the V scale the probabilities: P' = p vs / ref with ref a power of
-//   two that follows the largest V scale seen, so P' keeps fp16's 11 bits whatever the scales are.  Sums, maxima and
-//   the accumulators are fp32.  The maximum is raised only when a score exceeds it by 8 (P' then stays below 2^12).
+//   two that follows the largest V scale seen, so P' keeps fp16's 11 bits whatever the scales are; for fp16 outputs it
+//   enters as two fp16 parts, since the rounding of one would be as large as that of the output itself.  Sums, maxima
+//   and the accumulators are fp32.  The maximum is raised only when a score exceeds it by 8 (P' then stays below 2^12).
 // * O^T[d, row] = V^T P'^T: V's bytes of four keys are interleaved into fragments, P' is transposed with movmatrix.
 //   Splits of one row are joined by a second kernel in split order, so results do not depend on timing.
 #include <cfloat>
@@ -72,6 +73,7 @@ struct Bytes<8> {
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 3) k_kv_decode(const __grid_constant__ KvAttnArgs a) {
     constexpr int ROWS = 8 * NT, NCH = D / 64, VB = D / 8, MT = D / 16, OS = D + 4;
+    constexpr bool TWO = std::is_same<T, __half>::value;
     __shared__ float sm_m[DEC_WARPS][ROWS], sm_l[DEC_WARPS][ROWS];
     __shared__ __align__(16) float sm_o[DEC_WARPS][ROWS][OS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -247,7 +249,7 @@ __global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 3) k_kv_decode(c
                             for (int i = 0; i < 4; ++i) acc[j][nt][i] *= al;
                 }
                 const float w = vs * inv_ref;
-                uint32_t pb[NT][2];
+                uint32_t pb[NT][2], pl[NT][2];   // P' as fp16, and for fp16 outputs what that rounding left
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     float pw[4];
@@ -258,8 +260,15 @@ __global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 3) k_kv_decode(c
                         l[nt][i & 1] += p;
                         pw[i] = s[nt][i] == -INFINITY ? 0.f : p * w;   // a hidden key counts for nothing, whatever its block's scale
                     }
-                    pb[nt][0] = movmatrix(pack_half2(pw[0], pw[1]));
-                    pb[nt][1] = movmatrix(pack_half2(pw[2], pw[3]));
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t hi = pack_half2(pw[2 * i], pw[2 * i + 1]);
+                        if constexpr (TWO) {
+                            const float2 r = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+                            pl[nt][i] = movmatrix(pack_half2(pw[2 * i] - r.x, pw[2 * i + 1] - r.y));
+                        }
+                        pb[nt][i] = movmatrix(hi);
+                    }
                 }
 #pragma unroll
                 for (int j = 0; j < MT; ++j) {
@@ -268,7 +277,10 @@ __global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 3) k_kv_decode(c
                     const uint32_t a0 = magic_half2(x, 0x4140u), a1 = magic_half2(x, 0x4342u);
                     const uint32_t a2 = magic_half2(y, 0x4140u), a3 = magic_half2(y, 0x4342u);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma16816(acc[j][nt], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma16816(acc[j][nt], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+                        if constexpr (TWO) mma16816(acc[j][nt], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
+                    }
                 }
                 load_v(next);
                 at = next;
