@@ -71,7 +71,7 @@ struct Bytes<8> {
 };
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 3) k_kv_decode(const __grid_constant__ KvAttnArgs a) {
+__global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 2) k_kv_decode(const __grid_constant__ KvAttnArgs a) {
     constexpr int ROWS = 8 * NT, NCH = D / 64, VB = D / 8, MT = D / 16, OS = D + 4;
     constexpr bool TWO = std::is_same<T, __half>::value;
     __shared__ float sm_m[DEC_WARPS][ROWS], sm_l[DEC_WARPS][ROWS];
@@ -96,6 +96,14 @@ __global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 3) k_kv_decode(c
         const int per = max((nb + a.splits - 1) / a.splits, DEC_MIN_BLOCKS);
         const int lo = split * per, hi = min(nb, lo + per);
 
+        if (lo >= hi && a.splits > 1) {                                      // no share for this CTA
+            if (threadIdx.x < rn) {
+                const int rr = r0 + threadIdx.x, tok = rr / a.group;
+                const int64_t row = (int64_t)(first + tok) * a.c.heads * a.group + h * a.group + rr - tok * a.group;
+                a.part_ml[row * a.part_stride + split] = make_float2(-INFINITY, 0.f);
+            }
+            continue;
+        }
         // queries: row g of each n tile, dims 64 c + 16 t .. + 15
         uint32_t qf[NT][NCH][8];
         float qs[NT][2], m[NT][2], l[NT][2];
@@ -432,7 +440,6 @@ static KvAttnPlan kv_plan(const v3g_kv_cache_t *c, const v3g_kv_batch_t *b, uint
     }
     uint64_t keys = (uint64_t)b->max_pages * c->page;
     if (max_kv && max_kv < keys) keys = max_kv;
-    // splits that fill the SMs once: 4 CTA slots per SM and DEC_MIN_BLOCKS blocks a share for few rows
     auto seen = [&](uint64_t tokens) {
         const uint64_t w = (uint64_t)window + n_sink + tokens + 2 * KV_BLOCK;
         return window && w < keys ? w : keys;
@@ -447,7 +454,10 @@ static KvAttnPlan kv_plan(const v3g_kv_cache_t *c, const v3g_kv_batch_t *b, uint
         while (tiles > 1 && tiles * seq > 0x1000000u) tiles = (tiles + 1) / 2;   // a tile loop serves the rest
         p.row_tiles = (int)tiles;
         const uint64_t blocks = (seen(tokens) + KV_BLOCK - 1) / KV_BLOCK, most = (blocks + DEC_MIN_BLOCKS - 1) / DEC_MIN_BLOCKS;
-        uint64_t s = 148 * 4 / (seq * tiles);
+        // Every CTA slot (4 per SM) gets a share, none less than DEC_MIN_BLOCKS blocks.  More shares than slots cost more than the
+        // balance they bring (64 sequences of 1,411-4,608 keys: 29.5 us, with twice the shares 31.5 us); beside the many-row
+        // kernel, whose sequences take no shares here, twice as many.
+        uint64_t s = (p.many ? 148 * 8 : 148 * 4) / (seq * tiles);
         s = s > most ? most : s;
         s = s > room ? room : s;
         p.splits = s < 1 ? 1 : (s > 128 ? 128 : (int)s);

@@ -39,9 +39,35 @@ def rope_table(n_positions: int, head_dim: int, theta: float = 1_000_000.0, devi
 
 
 def _index(t: torch.Tensor, name: str, device, n: int) -> int:
-    if t.dtype != torch.int32 or t.device != device or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.numel() != n or t.dim() != 1 or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor of {n} entries on {device}")
     return t.data_ptr()
+
+
+def _stream(device) -> int:
+    """torch's current stream on `device` as the C ABI takes it (the call behind torch.cuda.current_stream, without the
+    Python object around it: 0.1 us instead of 2.3)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+class _Workspaces:
+    """Device workspaces, one for each stream that has used them: a stream runs its calls in order, so they can share one.
+    They grow and are kept until their owner goes.  A captured call has one of its own, in the graph's memory."""
+
+    def __init__(self):
+        self.by_stream = {}
+
+    def get(self, device, stream: int, size: int) -> int:
+        if torch.cuda.is_current_stream_capturing():
+            return torch.empty(size, dtype=torch.uint8, device=device).data_ptr()
+        held = self.by_stream.get((device.index, stream))
+        if held is None or held[0] < size:
+            t = torch.empty(size, dtype=torch.uint8, device=device)
+            held = self.by_stream[(device.index, stream)] = (size, t.data_ptr(), t)
+        return held[1]
+
+
+_beam_work = _Workspaces()
 
 
 class PagedKVCache:
@@ -80,6 +106,8 @@ class PagedKVCache:
         self.n_layers, self.n_pages, self.n_kv_heads, self.page, self.head_dim = k.shape
         self.device = k.device
         self.status_word = torch.zeros(1, dtype=torch.int32, device=k.device)
+        self._status = self.status_word.data_ptr()
+        self._work = _Workspaces()
         self._c = _lib.KVCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), *k.shape)
         self._ref = C.byref(self._c)
 
@@ -96,28 +124,25 @@ class PagedKVCache:
                                 if bits & _lib.V3G_STATUS_BOUNDS else "a kernel gave up waiting, its output is invalid"))
 
     # ---- arguments
-    def _stream(self) -> int:
-        return torch.cuda.current_stream(self.device).cuda_stream
-
-    def _table(self, page_table: torch.Tensor) -> int:
-        if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.device != self.device or \
-                page_table.shape[1] < 1 or page_table.stride(1) != 1 or \
-                (page_table.shape[0] > 1 and page_table.stride(0) < page_table.shape[1]):
-            raise ValueError("page_table must be int32 [batch, pages] on the cache's device with contiguous rows")
-        return page_table.data_ptr()
-
     def _batch(self, page_table, kv_len, q_start, n_tokens: int) -> _lib.KVBatch:
-        table = self._table(page_table)
+        dev = self.device
+        if page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.device != dev:
+            raise ValueError("page_table must be int32 [batch, pages] on the cache's device")
         n, cols = page_table.shape
-        return _lib.KVBatch(table, max(page_table.stride(0), cols), _index(kv_len, "kv_len", self.device, n),
-                            _index(q_start, "q_start", self.device, n + 1), n, cols, n_tokens)
+        ld, one = page_table.stride()
+        if cols < 1 or (one != 1 and cols > 1) or (n > 1 and ld < cols):
+            raise ValueError("page_table needs at least one column and contiguous rows")
+        lens = _index(kv_len, "kv_len", dev, n)
+        starts = lens if q_start is None else _index(q_start, "q_start", dev, n + 1)
+        return _lib.KVBatch(page_table.data_ptr(), ld if ld > cols else cols, lens, starts, n, cols, n_tokens)
 
     def _rows(self, x: torch.Tensor, name: str, heads: int, n: int, dtype) -> _lib.Rows:
-        if x.dim() != 3 or x.shape[0] != n or x.shape[1] != heads or x.shape[2] != self.head_dim or x.dtype != dtype or \
-                x.device != self.device or x.stride(2) != 1:
-            raise ValueError(f"{name} must be {dtype} [{n}, {heads}, {self.head_dim}] on the cache's device, its last "
-                             "dimension contiguous")
-        return _lib.Rows(x.data_ptr(), x.stride(0), x.stride(1))
+        if x.dim() == 3 and x.dtype is dtype and x.device == self.device:
+            shape = x.shape
+            tok, head, one = x.stride()
+            if one == 1 and shape[0] == n and shape[1] == heads and shape[2] == self.head_dim:
+                return _lib.Rows(x.data_ptr(), tok, head)
+        raise ValueError(f"{name} must be {dtype} [{n}, {heads}, {self.head_dim}] on the cache's device, its last dimension contiguous")
 
     def _layer(self, layer: int) -> int:
         if not 0 <= layer < self.n_layers:
@@ -125,11 +150,15 @@ class PagedKVCache:
         return layer
 
     def _call(self, fn, what: str, *args) -> None:
-        if torch.cuda.current_device() == self.device.index:
-            _lib.check(fn(*args, self._stream()), what)
+        """fn on torch's current stream of the cache's device, which becomes the current device for the call."""
+        dev = self.device
+        if torch._C._cuda_getDevice() == dev.index:
+            rc = fn(*args, _stream(dev))
         else:
-            with torch.cuda.device(self.device):
-                _lib.check(fn(*args, self._stream()), what)
+            with torch.cuda.device(dev):
+                rc = fn(*args, _stream(dev))
+        if rc:
+            _lib.check(rc, what)
 
     # ---- operators
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, kv_len: torch.Tensor,
@@ -139,33 +168,35 @@ class PagedKVCache:
         strides), k rotated at its position when `rope` (rope_table) is given.  With q [tokens, heads, head_dim] of the
         same type, the rotated queries are returned (in q_out, if given).  A block of 16 tokens keeps one scale per
         head: when a later token is larger, the block's earlier codes are rounded again under the larger scale."""
-        n = k.shape[0]
-        dt = _DTYPES.get(k.dtype)
+        n, dtype = k.shape[0], k.dtype
+        dt = _DTYPES.get(dtype)
         if dt is None:
             raise ValueError("k must be fp32, fp16 or bf16")
-        kr = self._rows(k, "k", self.n_kv_heads, n, k.dtype)
-        vr = self._rows(v, "v", self.n_kv_heads, n, k.dtype)
+        kr = self._rows(k, "k", self.n_kv_heads, n, dtype)
+        vr = self._rows(v, "v", self.n_kv_heads, n, dtype)
         batch = self._batch(page_table, kv_len, q_start, n)
-        if rope is not None and (rope.dim() != 2 or rope.shape[1] != self.head_dim or rope.dtype != torch.float32 or
-                                 rope.device != self.device or not rope.is_contiguous() or rope.shape[0] < 1):
-            raise ValueError("rope must be a contiguous fp32 [positions, head_dim] table on the cache's device")
-        qr = None
-        heads = 0
+        positions = 0
+        if rope is not None:
+            if rope.dim() != 2 or rope.dtype is not torch.float32 or rope.device != self.device or not rope.is_contiguous() or \
+                    rope.shape[1] != self.head_dim or rope.shape[0] < 1:
+                raise ValueError("rope must be a contiguous fp32 [positions, head_dim] table on the cache's device")
+            positions = rope.shape[0]
+        qr, heads = None, 0
         if q is not None:
             heads = q.shape[1] if q.dim() == 3 else 0
-            qr = self._rows(q, "q", heads, n, k.dtype)
+            qr = self._rows(q, "q", heads, n, dtype)
+            if heads == 0:
+                raise ValueError("q has no heads")
             if q_out is None:
-                q_out = torch.empty(n, heads, self.head_dim, dtype=q.dtype, device=self.device)
-            elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.device != self.device or not q_out.is_contiguous():
+                q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            elif q_out.shape != q.shape or q_out.dtype is not dtype or q_out.device != self.device or not q_out.is_contiguous():
                 raise ValueError("q_out must be a contiguous tensor of q's shape and type")
-        if n and heads == 0 and q is not None:
-            raise ValueError("q has no heads")
-        if n == 0:
-            return q_out if q is not None else None
-        self._call(_lib.lib().v3g_kv_append, "v3g_kv_append", self._ref, self._layer(layer), batch, dt, kr, vr, qr, heads,
-                   q_out.data_ptr() if q is not None else None, None if rope is None else rope.data_ptr(),
-                   0 if rope is None else rope.shape[0], self.status_word.data_ptr())
-        return q_out if q is not None else None
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        if n:
+            self._call(_lib.lib().v3g_kv_append, "v3g_kv_append", self._ref, self._layer(layer), batch, dt, kr, vr, qr, heads,
+                       None if q is None else q_out.data_ptr(), None if rope is None else rope.data_ptr(), positions, self._status)
+        return q_out
 
     def attention(self, layer: int, q: torch.Tensor, page_table: torch.Tensor, kv_len: torch.Tensor, q_start: torch.Tensor,
                   scale: Optional[float] = None, window: int = 0, n_sink: int = 0, max_q: int = 0, max_kv: int = 0,
@@ -175,20 +206,18 @@ class PagedKVCache:
         return_lse also the logarithm of the softmax sum [tokens, heads]; a row that sees no key gives zeros and -inf.
         max_q and max_kv (largest token count and length in the batch, where the host knows them) steer how work is
         split and never what is computed.  scale defaults to head_dim ** -0.5."""
-        heads = q.shape[1] if q.dim() == 3 else 0
-        n = q.shape[0]
-        dt = _DTYPES.get(q.dtype)
-        if dt not in (_lib.V3G_F16, _lib.V3G_BF16):
+        n, heads, dtype = q.shape[0], q.shape[1] if q.dim() == 3 else 0, q.dtype
+        if dtype is not torch.float16 and dtype is not torch.bfloat16:
             raise ValueError("q must be fp16 or bf16")
         if heads == 0 or heads % self.n_kv_heads:
             raise ValueError("the query heads must be a multiple of the KV heads")
         if window < 0 or n_sink < 0 or max_q < 0 or max_kv < 0:
             raise ValueError("window, n_sink, max_q and max_kv must not be negative")
-        qr = self._rows(q, "q", heads, n, q.dtype)
+        qr = self._rows(q, "q", heads, n, dtype)
         batch = self._batch(page_table, kv_len, q_start, n)
         if out is None:
-            out = torch.empty(n, heads, self.head_dim, dtype=q.dtype, device=self.device)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.device != self.device or not out.is_contiguous():
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        elif out.shape != q.shape or out.dtype is not dtype or out.device != self.device or not out.is_contiguous():
             raise ValueError("out must be a contiguous tensor of q's shape and type")
         lse = torch.empty(n, heads, dtype=torch.float32, device=self.device) if return_lse else None
         if n:
@@ -196,10 +225,10 @@ class PagedKVCache:
             window, n_sink = min(window, 1 << 30), min(n_sink, 1 << 30)
             max_q, max_kv = min(max_q, 0x7FFFFFFF), min(max_kv, 0x7FFFFFFF)
             size = L.v3g_kv_attention_work_size(self._ref, batch, heads, max_q, max_kv, window, n_sink)
-            work = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
-            self._call(L.v3g_kv_attention, "v3g_kv_attention", self._ref, self._layer(layer), batch, dt, qr, heads,
+            self._call(L.v3g_kv_attention, "v3g_kv_attention", self._ref, self._layer(layer), batch, _DTYPES[dtype], qr, heads,
                        self.head_dim ** -0.5 if scale is None else float(scale), window, n_sink, max_q, max_kv, out.data_ptr(),
-                       None if lse is None else lse.data_ptr(), self.status_word.data_ptr(), None if work is None else work.data_ptr(), size)
+                       None if lse is None else lse.data_ptr(), self._status,
+                       self._work.get(self.device, _stream(self.device), size) if size else None, size)
         return (out, lse) if return_lse else out
 
     def read(self, page_table: torch.Tensor, first: torch.Tensor, kv_len: torch.Tensor, row_start: torch.Tensor, n_rows: int,
@@ -213,10 +242,11 @@ class PagedKVCache:
         if n_rows < 0:
             raise ValueError("n_rows must not be negative")
         batch = self._batch(page_table, kv_len, row_start, n_rows)
-        f = _index(first, "first", self.device, page_table.shape[0])
+        f = _index(first, "first", self.device, batch.batch)
         l0, layers = (0, self.n_layers) if layer is None else (self._layer(layer), 1)
-        k, v = (torch.empty(layers, n_rows, self.n_kv_heads, self.head_dim, dtype=dtype, device=self.device) for _ in range(2))
-        if page_table.shape[0] == 0:
+        k = torch.empty(layers, n_rows, self.n_kv_heads, self.head_dim, dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
+        if batch.batch == 0:
             return k.zero_(), v.zero_()
         if n_rows:
             self._call(_lib.lib().v3g_kv_read, "v3g_kv_read", self._ref, l0, layers, batch, f, dt, k.data_ptr(), v.data_ptr())
@@ -228,18 +258,16 @@ class PagedKVCache:
         returns the new page table, in which row g * beams + j shares the full pages of its parent; the page still being
         filled is copied, in every layer, into dst_page ([rows] int32; default: the row's own entry).  The rows of a
         group have equal kv_len."""
-        if parents.dtype != torch.int32 or parents.dim() != 2 or parents.device != self.device or not parents.is_contiguous() or \
-                parents.numel() != page_table.shape[0] or parents.shape[1] < 1:
+        rows, dev = page_table.shape[0], self.device
+        if parents.dtype is not torch.int32 or parents.dim() != 2 or parents.device != dev or not parents.is_contiguous() or \
+                parents.numel() != rows or parents.shape[1] < 1:
             raise ValueError("parents must be a contiguous int32 [groups, beams] tensor with one entry for each row")
-        rows = parents.numel()
-        lens = _index(kv_len, "kv_len", self.device, rows)
-        table = self._table(page_table)
-        batch = _lib.KVBatch(table, max(page_table.stride(0), page_table.shape[1]), lens, lens, rows, page_table.shape[1], 0)
-        dst = None if dst_page is None else _index(dst_page, "dst_page", self.device, rows)
-        out = torch.empty(page_table.shape, dtype=torch.int32, device=self.device)
+        batch = self._batch(page_table, kv_len, None, 0)
+        dst = None if dst_page is None else _index(dst_page, "dst_page", dev, rows)
+        out = torch.empty_like(page_table, memory_format=torch.contiguous_format)
         if rows:
             self._call(_lib.lib().v3g_kv_reorder, "v3g_kv_reorder", self._ref, batch, parents.shape[1], parents.data_ptr(), dst,
-                       out.data_ptr(), out.shape[1], self.status_word.data_ptr())
+                       out.data_ptr(), batch.max_pages, self._status)
         return out
 
 
@@ -250,29 +278,40 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: Optional[t
     `beams` best in descending order: (tokens, parents, scores, finished), each [groups, beams].  A finished beam goes on
     with eos_id alone, at its own score; equal scores go to the lower (beam, token); continuations at -inf or NaN are
     never chosen, and slots left over come back finished, with score -inf."""
-    if logits.dim() != 3 or logits.dtype not in _DTYPES or not logits.is_cuda or logits.numel() == 0:
+    dt = _DTYPES.get(logits.dtype)
+    if dt is None or logits.dim() != 3 or not logits.is_cuda or logits.numel() == 0:
         raise ValueError("logits must be a CUDA tensor [groups, beams, vocab] of fp32, fp16 or bf16")
-    b, k, v = logits.shape
-    ld = logits.stride(1) if k > 1 else (logits.stride(0) if b > 1 else v)
-    if (logits.stride(2) != 1 and v > 1) or ld < v or (b > 1 and k > 1 and logits.stride(0) != k * ld):
+    shape = b, k, v = logits.shape
+    s0, s1, s2 = logits.stride()
+    ld = s1 if k > 1 else (s0 if b > 1 else v)
+    if (s2 != 1 and v > 1) or ld < v or (b > 1 and k > 1 and s0 != k * ld):
         raise ValueError("logits must have contiguous rows, evenly spaced")
     dev = logits.device
-    if scores.shape != (b, k) or scores.dtype != torch.float32 or scores.device != dev or not scores.is_contiguous():
+    if scores.dtype is not torch.float32 or scores.shape != shape[:2] or scores.device != dev or not scores.is_contiguous():
         raise ValueError("scores must be a contiguous fp32 [groups, beams] tensor on the logits' device")
-    if finished is not None and (finished.shape != (b, k) or finished.dtype not in (torch.uint8, torch.bool) or
+    if finished is not None and (finished.dtype not in (torch.uint8, torch.bool) or finished.shape != shape[:2] or
                                  finished.device != dev or not finished.is_contiguous()):
         raise ValueError("finished must be a contiguous uint8 [groups, beams] tensor on the logits' device")
     L = _lib.lib()
     size = L.v3g_beam_select_work_size(b, k, v)
-    work = torch.empty(max(size, 1), dtype=torch.uint8, device=dev)
-    tokens, parents = (torch.empty(b, k, dtype=torch.int32, device=dev) for _ in range(2))
-    best = torch.empty(b, k, dtype=torch.float32, device=dev)
-    done = torch.empty(b, k, dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        _lib.check(L.v3g_beam_select(logits.data_ptr(), _DTYPES[logits.dtype], b, k, v, ld, scores.data_ptr(),
-                                     None if finished is None else finished.data_ptr(), int(eos_id), tokens.data_ptr(),
-                                     parents.data_ptr(), best.data_ptr(), done.data_ptr(), work.data_ptr(), size,
-                                     torch.cuda.current_stream(dev).cuda_stream), "v3g_beam_select")
+    best = torch.empty_like(scores)
+    tokens = torch.empty_like(scores, dtype=torch.int32)
+    parents = torch.empty_like(tokens)
+    done = torch.empty_like(scores, dtype=torch.uint8)
+
+    def call():
+        stream = _stream(dev)
+        return L.v3g_beam_select(logits.data_ptr(), dt, b, k, v, ld, scores.data_ptr(), None if finished is None else finished.data_ptr(),
+                                 eos_id, tokens.data_ptr(), parents.data_ptr(), best.data_ptr(), done.data_ptr(),
+                                 _beam_work.get(dev, stream, size) if size else None, size, stream)
+
+    if torch._C._cuda_getDevice() == dev.index:
+        rc = call()
+    else:
+        with torch.cuda.device(dev):
+            rc = call()
+    if rc:
+        _lib.check(rc, "v3g_beam_select")
     return tokens, parents, best, done
 
 
