@@ -9,6 +9,8 @@
 // selections are exact: the smallest of at least `beams` group maxima bounds the answer from below, the few values at or
 // above it are collected and ranked by counting, and a slice that holds too many of them (long ties, sorted logits)
 // takes `beams` rounds of a block maximum instead.
+#include <cfloat>
+
 #include "v3g_internal.h"
 #include "v3g_kv.cuh"
 
@@ -141,21 +143,31 @@ __global__ void __launch_bounds__(BEAM_THREADS, EPT == 32 ? 4 : 6) k_beam_slice(
     float top = sm.group[lane];
     if (lane >= (beams <= 8 ? 8 : (beams <= 16 ? 16 : 32))) top = -INFINITY;
     top = warp_max(top);                                          // the slice's maximum
-    // Sum of 2^((x - top) log2 e).  The difference comes first: logits at the type's lowest value would leave its range as
-    // products.  Hidden and NaN logits end at 2^-200 = 0, and so does a slice whose maximum is infinite.
+    // Sum of 2^((x - top) log2 e), in one product where that stays in range.  Otherwise (logits at the type's lowest value,
+    // an infinite maximum) or where a NaN came in, the difference comes first, and what is no number ends at 2^-200 = 0.
     float sum = 0.f;
+    const bool plain = fabsf(top) < 1e38f;
+    if (plain) {
+        const float shift = -top * 1.44269504f;
 #pragma unroll
-    for (int e = 0; e < EPT; ++e) sum += beam_ex2(fmaxf((x[e] - top) * 1.44269504f, -200.f));
+        for (int e = 0; e < EPT; ++e) sum += beam_ex2(fmaf(x[e], 1.44269504f, shift));
+    }
+    if (!plain || sum != sum) {
+        sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < EPT; ++e) sum += beam_ex2(fmaxf((x[e] - top) * 1.44269504f, -200.f));
+    }
     sum = warp_sum(sum);
     if (lane == 0) red[warp] = sum;
     const int64_t slice = row * gridDim.x + blockIdx.x;
     beam_best(
         sm, beams, float_key(bound),
         [&](auto f) {
-            if (mine >= bound)                                    // few threads hold one of the best
+            const float lo = fmaxf(bound, -FLT_MAX);              // finite ones only; few threads hold one of the best
+            if (mine >= lo)
 #pragma unroll
                 for (int e = 0; e < EPT; ++e)
-                    if (x[e] > -INFINITY && x[e] < INFINITY) f(((u64)float_key(x[e]) << 32) | (0xFFFFFFFFu - (uint32_t)index(e)));
+                    if (x[e] >= lo && x[e] <= FLT_MAX) f(((u64)float_key(x[e]) << 32) | (0xFFFFFFFFu - (uint32_t)index(e)));
         },
         [&](int rank, u64 k) { keys[slice * beams + rank] = k; });
     if (tid == 0) {   // red was written before beam_best's barrier
