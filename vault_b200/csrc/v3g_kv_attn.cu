@@ -543,6 +543,7 @@ extern "C" int v3g_kv_attention(const v3g_kv_cache_t *cache, uint32_t layer, con
     a.q_tok = q->tok_stride;
     a.q_head = q->head_stride;
     a.q_vec = reinterpret_cast<uintptr_t>(q->data) % 8 == 0 && q->tok_stride % 4 == 0 && q->head_stride % 4 == 0;
+    a.q_vec8 = reinterpret_cast<uintptr_t>(q->data) % 16 == 0 && q->tok_stride % 8 == 0 && q->head_stride % 8 == 0;
     a.group = (int)(n_q_heads / cache->n_kv_heads);
     a.scale_log2 = scale * 1.44269504f;
     a.window = (int)window;

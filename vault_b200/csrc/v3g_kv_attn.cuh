@@ -10,7 +10,7 @@ struct KvAttnArgs {
     KvView c;
     const void *q;
     int64_t q_tok, q_head;     // strides in elements
-    bool q_vec;                // four-element loads of q are aligned
+    bool q_vec, q_vec8;        // four- and eight-element loads of q are aligned
     int group;                 // query heads per KV head
     float scale_log2;          // scale x log2(e)
     int window, n_sink;        // window 0: every earlier key

@@ -42,7 +42,7 @@ constexpr int PF_RING = 8, PF_AHEAD = 5;
 template <int D>
 struct PfSmem {
     static constexpr int OP = 128 * D * 2;                      // one 128 x D fp16 operand
-    static constexpr int Q = 0, K = 2 * OP, V = 4 * OP, SC = 6 * OP, BAR = SC + PF_RING * 192, END = BAR + 384, BYTES = END + 1024;
+    static constexpr int Q = 0, K = 2 * OP, V = 4 * OP, SC = 6 * OP, BAR = SC + PF_RING * 192, QF = BAR + 384, BYTES = QF + 1024 + 1024;
 };
 
 struct alignas(16) PfPlaces {   // of one key tile, per 16-key block
@@ -246,38 +246,49 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
         const int qh = h * a.group + r - tok * a.group;
         const uint32_t lane_tm = tmem + ((uint32_t)(32 * (warp & 3)) << 16), tS = lane_tm + 128u * tile, tO = lane_tm + 256u + 128u * tile;
         if (tile < tiles) {
-            // the row's query: a power of two brings it into fp16 (sign of the scale with it), 128-byte swizzled halves
-            float qf;
+            // The warp's 32 query rows, LPR lanes to a row so that reads are whole lines: a power of two brings a row into fp16 (the
+            // sign of the scale with it), in 128-byte swizzled halves
+            constexpr int LPR = D / 8, RPI = 32 / LPR;
+            const int row_w = 128 * tile + 32 * (warp & 3);   // the warp's first row in the CTA
+            const int pc = lane % LPR, pr = lane / LPR;       // this lane's piece, and its row in a pass
+            float *qfac = reinterpret_cast<float *>(smem + SM::QF);
+            uint8_t *piece = smem + SM::Q + tile * SM::OP + (pc >> 3) * 16384;   // rows of 128 bytes, piece pc & 7
             {
-                const T *src = static_cast<const T *>(a.q) + (int64_t)(first + tok) * a.q_tok + (int64_t)qh * a.q_head;
-                float4 x[D / 4];   // all loads in flight at once
-                float top = 0.f;
+                uint4 x[LPR];
 #pragma unroll
-                for (int i = 0; i < D / 4; ++i) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (live && a.q_vec) {
+                for (int i = 0; i < LPR; ++i) {
+                    const int rr = row_w + i * RPI + pr, tk = (r0 + rr) / a.group, hd = h * a.group + r0 + rr - tk * a.group;
+                    x[i] = make_uint4(0u, 0u, 0u, 0u);
+                    if (rr < rn) {
+                        const T *src = static_cast<const T *>(a.q) + (int64_t)(first + tk) * a.q_tok + (int64_t)hd * a.q_head + 8 * pc;
+                        if (a.q_vec8) x[i] = ldg_stream16(src);
+                        else
 #pragma unroll
-                    for (int i = 0; i < D / 4; ++i) x[i] = kv_load4<T>(src + 4 * i, true);
-                } else if (live) {
-#pragma unroll
-                    for (int i = 0; i < D / 4; ++i) x[i] = kv_load4<T>(src + 4 * i, false);
+                            for (int e = 0; e < 8; ++e) reinterpret_cast<T *>(&x[i])[e] = src[e];
+                    }
                 }
 #pragma unroll
-                for (int i = 0; i < D / 4; ++i)
-                    top = fmaxf(fmaxf(top, fmaxf(fabsf(x[i].x), fabsf(x[i].y))), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
-                const int up = kv_row_exponent<T>(top);
-                const float f = __int_as_float((up + 127) << 23) * (a.scale_log2 < 0.f ? -1.f : 1.f);
-                qf = __int_as_float((127 - up) << 23) * fabsf(a.scale_log2);
-                uint8_t *dst = smem + SM::Q + tile * SM::OP + row * 128;
+                for (int i = 0; i < LPR; ++i) {
+                    float y[8], top = 0.f;
 #pragma unroll
-                for (int c = 0; c < D / 8; ++c) {
-                    const float4 u = x[2 * c], v = x[2 * c + 1];
-                    *reinterpret_cast<uint4 *>(dst + (c >> 3) * 16384 + (((c & 7) ^ (row & 7)) << 4)) =
-                        make_uint4(pf_half2(u.x * f, u.y * f), pf_half2(u.z * f, u.w * f), pf_half2(v.x * f, v.y * f), pf_half2(v.z * f, v.w * f));
+                    for (int e = 0; e < 8; e += 4) {
+                        const float4 v = kv_load4<T>(reinterpret_cast<const T *>(&x[i]) + e, true);
+                        y[e] = v.x, y[e + 1] = v.y, y[e + 2] = v.z, y[e + 3] = v.w;
+                        top = fmaxf(fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+                    }
+#pragma unroll
+                    for (int o = 1; o < LPR; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    const int up = kv_row_exponent<T>(top), rl = 32 * (warp & 3) + i * RPI + pr;
+                    const float f = __int_as_float((up + 127) << 23) * (a.scale_log2 < 0.f ? -1.f : 1.f);
+                    *reinterpret_cast<uint4 *>(piece + rl * 128 + (((pc & 7) ^ (rl & 7)) << 4)) =
+                        make_uint4(pf_half2(y[0] * f, y[1] * f), pf_half2(y[2] * f, y[3] * f), pf_half2(y[4] * f, y[5] * f), pf_half2(y[6] * f, y[7] * f));
+                    if (pc == 0) qfac[128 * tile + rl] = __int_as_float((127 - up) << 23) * fabsf(a.scale_log2);
                 }
                 tc::fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(QFULL);
             }
+            const float qf = qfac[128 * tile + row];
             const int p = live ? p0 + tok : -1;
             float m = -INFINITY, l = 0.f;
             // Warps w of the two tiles share a quarter of the SM and its exponential unit, so they take turns at it (named
@@ -409,24 +420,47 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
                 if (shares == 1) inv = l == 0.f ? 0.f : inv / l;
             }
             const int64_t part = out_row * a.part_stride + share;
-            if (ok && (nk > 0 || shares == 1))   // an empty share has no accumulator
+            if (ok && shares > 1 && nk > 0) {   // (an empty share has no accumulator)
 #pragma unroll 1
+                for (int c = 0; c < D / 16; ++c) {
+                    uint32_t o[16];
+                    tmem_ld16_wait(tO + 16 * c, o);
+                    if (live)
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4)
+                            kv_store4(a.part_o + part * D + 16 * c + i, make_float4(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv,
+                                                                                    __uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv));
+                }
+            } else if (ok && shares == 1) {   // rows through the query's place in shared memory (no MMA reads it any more), out in whole lines
+                uint8_t *mine = smem + SM::Q + tile * SM::OP + row * 128;
+#pragma unroll 2
                 for (int c = 0; c < D / 16; ++c) {
                     uint32_t o[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[i] = 0u;
-                    if (nk > 0) {
-                        tmem_ld16_wait(tO + 16 * c, o);
-                    }
-                    if (live)
+                    if (nk > 0) tmem_ld16_wait(tO + 16 * c, o);
 #pragma unroll
-                        for (int i = 0; i < 16; i += 4) {
-                            const float4 v = make_float4(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv,
-                                                         __uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
-                            if (shares > 1) kv_store4(a.part_o + part * D + 16 * c + i, v);
-                            else kv_store4(static_cast<T *>(a.out) + out_row * D + 16 * c + i, v);
-                        }
+                    for (int k = 0; k < 2; ++k) {
+                        uint4 w;
+#pragma unroll
+                        for (int i = 0; i < 8; i += 4)
+                            kv_store4(reinterpret_cast<T *>(&w) + i,
+                                      make_float4(__uint_as_float(o[8 * k + i]) * inv, __uint_as_float(o[8 * k + i + 1]) * inv,
+                                                  __uint_as_float(o[8 * k + i + 2]) * inv, __uint_as_float(o[8 * k + i + 3]) * inv));
+                        const int pcs = 2 * c + k;
+                        *reinterpret_cast<uint4 *>(mine + (pcs >> 3) * 16384 + (((pcs & 7) ^ (row & 7)) << 4)) = w;
+                    }
                 }
+                __syncwarp();
+#pragma unroll 4
+                for (int i = 0; i < LPR; ++i) {
+                    const int rl = 32 * (warp & 3) + i * RPI + pr, rr = 128 * tile + rl, tk = (r0 + rr) / a.group;
+                    if (rr < rn)
+                        *reinterpret_cast<uint4 *>(static_cast<T *>(a.out) +
+                                                   ((int64_t)(first + tk) * a.c.heads * a.group + h * a.group + r0 + rr - tk * a.group) * D + 8 * pc) =
+                            *reinterpret_cast<const uint4 *>(piece + rl * 128 + (((pc & 7) ^ (rl & 7)) << 4));
+                }
+            }
             if (live && ok) {
                 if (shares > 1) a.part_ml[part] = make_float2(m, l);
                 else if (a.lse) a.lse[out_row] = l == 0.f ? -INFINITY : ((m == -INFINITY ? 0.f : m) + log2f(l)) * 0.69314718f;
