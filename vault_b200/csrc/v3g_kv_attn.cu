@@ -347,8 +347,6 @@ __global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 2) k_kv_decode(c
         }
         __syncthreads();
     }
-    // beside the many-row kernel: whoever waits for this one's end waits for both
-    if (a.after_many) griddep_wait();
 }
 
 // Joins the shares of a row: WR warps take every WR-th share each, in order, and are added in order.
@@ -487,12 +485,12 @@ static KvAttnPlan kv_plan(const v3g_kv_cache_t *c, const v3g_kv_batch_t *b, uint
 template <typename T, int D>
 static cudaError_t launch_attention_kernels(const KvAttnArgs &a, const KvAttnPlan &p, int dtype, cudaStream_t st) {
     cudaError_t e = cudaSuccess;
-    if (p.many) e = launch_kv_prefill(a, dtype, D, a.max_rows + 1, st);
-    if (e == cudaSuccess && p.few) {
+    if (p.few) {
         const dim3 grid((uint32_t)((uint64_t)a.c.batch * a.c.heads * a.splits * a.row_tiles));
-        if (p.nt == 1) e = launch_k(p.many, k_kv_decode<T, D, 1>, grid, 32 * DEC_WARPS, 0, st, a);
-        else e = launch_k(p.many, k_kv_decode<T, D, 2>, grid, 32 * DEC_WARPS, 0, st, a);
+        if (p.nt == 1) e = launch_k(false, k_kv_decode<T, D, 1>, grid, 32 * DEC_WARPS, 0, st, a);
+        else e = launch_k(false, k_kv_decode<T, D, 2>, grid, 32 * DEC_WARPS, 0, st, a);
     }
+    if (e == cudaSuccess && p.many) e = launch_kv_prefill(a, dtype, D, a.max_rows + 1, st);
     if (e != cudaSuccess || a.part_stride == 1) return e;
     // four warps a row while rows are few
     const int64_t rows = (int64_t)a.c.n_tokens * a.c.heads * a.group;
@@ -555,7 +553,7 @@ extern "C" int v3g_kv_attention(const v3g_kv_cache_t *cache, uint32_t layer, con
     a.max_rows = p.max_rows;
     a.pf_items = p.pf_items;
     a.pf_splits = p.pf_splits;
-    a.after_many = p.many && p.few;
+    a.after_few = p.many && p.few;
     a.part_stride = p.part_stride;
     a.status = dev_status;
     a.part_ml = static_cast<float2 *>(dev_work);

@@ -20,7 +20,7 @@ struct KvAttnArgs {
     int max_rows;
     int splits, row_tiles;     // few rows: key shares, row tiles in the grid
     int pf_items, pf_splits;   // many rows: units of 256 rows that a head has room for, key shares
-    bool after_many;           // the few-row kernel runs beside the many-row kernel and ends after it
+    bool after_few;            // the many-row kernel starts while the few-row kernel runs, and ends after it
     int part_stride;           // shares that a row has room for
     float2 *part_ml;           // [row][share] maximum (log2 units) and sum
     float *part_o;             // [row][share][D]

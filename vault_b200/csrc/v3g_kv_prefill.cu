@@ -57,16 +57,20 @@ static_assert(sizeof(PfPlaces) == 192, "ring slot");
 
 #define TC_REGS8(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7])
 #define TC_IN8(r, o) "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7])
-// 64 consecutive columns of the warp's 32 lanes; the values are there when it returns
-__device__ __forceinline__ void tmem_ld64_wait(uint32_t a, uint32_t (&r)[64]) {
+// 64 consecutive columns of the warp's 32 lanes; the values are there after tmem_ld64_done
+__device__ __forceinline__ void tmem_ld64(uint32_t a, uint32_t (&r)[64]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
         "%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,"
-        "%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n"
-        "tcgen05.wait::ld.sync.aligned;"
+        "%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];"
         : TC_REGS8(r, 0), TC_REGS8(r, 8), TC_REGS8(r, 16), TC_REGS8(r, 24), TC_REGS8(r, 32), TC_REGS8(r, 40), TC_REGS8(r, 48), TC_REGS8(r, 56)
         : "r"(a)
         : "memory");
+}
+__device__ __forceinline__ void tmem_ld64_done(uint32_t (&r)[64]) {
+    tc::tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 64; ++i) asm volatile("" : "+r"(r[i]));   // no use moves above the wait
 }
 __device__ __forceinline__ void tmem_ld16_wait(uint32_t a, uint32_t (&r)[16]) {
     asm volatile(
@@ -184,7 +188,10 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
     int first;
     const int n = a.c.tokens(b, first);
     const int64_t off = (item - base) * PF_ROWS;
-    if (off < 0 || off >= (int64_t)n * a.group || n * a.group < min_rows) return;
+    if (off < 0 || off >= (int64_t)n * a.group || n * a.group < min_rows) {
+        if (a.after_few) griddep_wait();
+        return;
+    }
     const int r0 = (int)off, rn = min(n * a.group - r0, PF_ROWS), tiles = rn > 128 ? 2 : 1;
     const int p0 = a.c.end(b) - n;
     int sb, ws;
@@ -311,6 +318,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
                 const int j = u >> 1, half = u & 1;
                 if (!(ok = pf_wait(SFULL(tile, half), j & 1))) return;
                 tc::tc_fence_after();
+                uint32_t s[64];
+                tmem_ld64(tS + 64 * half, s);
                 // the tile's scales were written before the K that the scores come from
                 const PfPlaces &at = places[j & (PF_RING - 1)];
                 const float4 k4 = *reinterpret_cast<const float4 *>(at.ks + 4 * half), w4 = *reinterpret_cast<const float4 *>(at.w + 4 * half),
@@ -321,9 +330,9 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
                     if (f[i] < 0x1p-100f) f[i] = 0x1p-100f;   // hidden keys' -inf stays -inf in a block of scale 0; a NaN stays one
                 float wv[4] = {w4.x, w4.y, w4.z, w4.w}, iw[4] = {i4.x, i4.y, i4.z, i4.w};
                 const float al_ref = half ? 1.f : at.al;
-                uint32_t s[64];
-                tmem_ld64_wait(tS + 64 * half, s);
-                if (!(at.whole >> (2 * tile + half) & 1u)) {   // hide keys; a block that the row does not see at all loses its scales
+                const bool whole = at.whole >> (2 * tile + half) & 1u;
+                tmem_ld64_done(s);
+                if (!whole) {   // hide keys; a block that the row does not see at all loses its scales
                     const int k0 = at.k0 + 64 * half;
                     const uint32_t valid = at.valid >> (4 * half);
 #pragma unroll
@@ -622,6 +631,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
     __syncthreads();
     tc::tc_fence_after();
     if (warp == 12) tc::tmem_dealloc(tmem, 512);
+    if (a.after_few) griddep_wait();   // whoever waits for this kernel's end waits for both
 }
 
 template <typename T, int D>
@@ -641,7 +651,7 @@ static cudaError_t launch_pf(const KvAttnArgs &a, int min_rows, cudaStream_t st)
         if (e != cudaSuccess) return e;
         if (dev >= 0 && dev < 64) ready.fetch_or(1ull << dev);
     }
-    return launch_k(false, kern, dim3((uint32_t)((uint64_t)a.pf_items * a.c.heads * a.pf_splits)), PF_THREADS, PfSmem<D>::BYTES, st, a, min_rows);
+    return launch_k(a.after_few, kern, dim3((uint32_t)((uint64_t)a.pf_items * a.c.heads * a.pf_splits)), PF_THREADS, PfSmem<D>::BYTES, st, a, min_rows);
 }
 
 cudaError_t launch_kv_prefill(const KvAttnArgs &a, int dtype, int head_dim, int min_rows, cudaStream_t st) {
