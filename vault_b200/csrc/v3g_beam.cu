@@ -6,7 +6,7 @@
 // scores is the order of the logits, so the first kernel needs no lse: a CTA keeps a slice of 4,096 or 8,192 logits of
 // one beam in registers, reduces their maximum and sum of exponentials, and writes its `beams` best as 64-bit keys (value, then lower
 // index).  The second kernel joins the sums of a beam, scores the beams x slices x beams keys and selects again.  Both
-// selections are exact: the smallest of at least `beams` group maxima bounds the answer from below, the few values at or
+// selections are exact: the `beams`-th largest of some group maxima bounds the answer from below, the few values at or
 // above it are collected and ranked by counting, and a slice that holds too many of them (long ties, sorted logits)
 // takes `beams` rounds of a block maximum instead.
 #include <cfloat>
@@ -34,19 +34,25 @@ struct BeamShared {
     int count;
 };
 
-// Smallest of G group maxima of the threads' values, G = 8, 16 or 32 >= beams equal groups of threads: at least
-// `beams` values of the block are at or above it.
+// The `beams`-th largest of the maxima of G groups of threads, G = 8, 16 or 32 >= beams: at least `beams` values of the
+// block are at or above it.
+__device__ __forceinline__ int beam_groups(int beams) { return beams <= 8 ? 8 : (beams <= 16 ? 16 : 32); }
 __device__ __forceinline__ float beam_bound(BeamShared &sm, float v, int beams) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int per = beams <= 8 ? 1 : (beams <= 16 ? 2 : 4);       // groups of a warp
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, groups = beam_groups(beams), per = groups / 8;   // groups of a warp
     for (int o = 1; o < 32 / per; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     if (threadIdx.x == 0) sm.count = 0;
     if (lane % (32 / per) == 0) sm.group[warp * per + lane / (32 / per)] = v;
     __syncthreads();
-    float lo = sm.group[lane % (8 * per)];
+    v = lane < groups ? sm.group[lane] : -INFINITY;
+    int rank = 0;
+    for (int k = 0; k < groups; k += 8)
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    return lo;
+        for (int u = 0; u < 8; ++u) {
+            const float o = __shfl_sync(0xffffffffu, v, k + u);
+            rank += o > v || (o == v && k + u < lane);
+        }
+    const uint32_t at = __ballot_sync(0xffffffffu, lane < groups && rank == beams - 1);
+    return __shfl_sync(0xffffffffu, v, __ffs(at) - 1);
 }
 
 // the block's largest key, to every thread
@@ -141,7 +147,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, EPT == 32 ? 4 : 6) k_beam_slice(
     for (int e = 0; e < EPT; ++e) mine = fmaxf(mine, x[e]);       // NaN logits are passed over
     const float bound = beam_bound(sm, mine, beams);
     float top = sm.group[lane];
-    if (lane >= (beams <= 8 ? 8 : (beams <= 16 ? 16 : 32))) top = -INFINITY;
+    if (lane >= beam_groups(beams)) top = -INFINITY;
     top = warp_max(top);                                          // the slice's maximum
     // Sum of 2^((x - top) log2 e), in one product where that stays in range.  Otherwise (logits at the type's lowest value,
     // an infinite maximum) or where a NaN came in, the difference comes first, and what is no number ends at 2^-200 = 0.
