@@ -3,12 +3,12 @@
 //   score(k, t) = (logit[k][t] - lse_k) + scores[k],   lse_k = max + log(sum exp(logit - max))
 //
 // The logits are read once (4 bytes and an exponential per element: HBM bounds it).  Inside a beam the order of the
-// scores is the order of the logits, so the first kernel needs no lse: a CTA keeps a slice of 4,096 or 8,192 logits of
-// one beam in registers, reduces their maximum and sum of exponentials, and writes its `beams` best as 64-bit keys (value, then lower
-// index).  The second kernel joins the sums of a beam, scores the beams x slices x beams keys and selects again.  Both
-// selections are exact: the `beams`-th largest of some group maxima bounds the answer from below, the few values at or
-// above it are collected and ranked by counting, and a slice that holds too many of them (long ties, sorted logits)
-// takes `beams` rounds of a block maximum instead.
+// scores is the order of the logits, so the first kernel needs no lse: a CTA streams a slice of one beam's logits, each
+// thread keeping the maximum and the sum of exponentials of its own, and writes the slice's `beams` best as 64-bit keys
+// (value, then lower index).  The second kernel joins the sums of a beam, scores the beams x slices x beams keys and
+// selects again.  Both selections are exact: the `beams`-th largest of some group maxima bounds the answer from below; the few
+// threads whose maximum reaches it read their logits again, and what is at or above it is collected and ranked by
+// counting; where too much is (long ties, sorted logits), `beams` rounds of a block maximum take its place.
 #include <cfloat>
 
 #include "v3g_internal.h"
@@ -119,67 +119,89 @@ __device__ __forceinline__ float beam_ex2(float x) {
     return r;
 }
 
-template <typename T, int EPT>
-__global__ void __launch_bounds__(BEAM_THREADS, EPT == 32 ? 4 : 6) k_beam_slice(const T *logits, int64_t ld, int vocab, int beams, bool vec,
-                                                                               u64 *keys, float2 *sums) {
+// `slice` consecutive logits of a beam (a multiple of BEAM_STEP): the threads' running maxima and sums, then the best
+constexpr int BEAM_EPT = 16, BEAM_STEP = BEAM_THREADS * BEAM_EPT;
+template <typename T>
+__global__ void __launch_bounds__(BEAM_THREADS, 6) k_beam_slice(const T *logits, int64_t ld, int vocab, int slice, int beams, bool vec, u64 *keys,
+                                                               float2 *sums) {
     __shared__ BeamShared sm;
     __shared__ float red[BEAM_THREADS / 32];
     griddep_launch();
-    constexpr int SLICE = BEAM_THREADS * EPT, W = 16 / sizeof(T), NL = EPT / W;   // elements of a 16-byte load, loads of a thread
+    constexpr int W = 16 / sizeof(T), NL = BEAM_EPT / W;          // elements of a 16-byte load, loads of a step
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int64_t row = blockIdx.y;
-    const int i0 = blockIdx.x * SLICE + tid * W;
+    const int i0 = blockIdx.x * slice, steps = (min(slice, vocab - i0) + BEAM_STEP - 1) / BEAM_STEP;
     const T *p = logits + row * ld;
-    float x[EPT];
-    auto index = [&](int e) { return i0 + (e / W) * (BEAM_THREADS * W) + e % W; };
-    if (vec && (int)(blockIdx.x + 1) * SLICE <= vocab) {
-        uint4 u[NL];
+    // element e of the thread's share of a step: 16-byte pieces where the step is whole and aligned, else every 256th
+    auto whole = [&](int step) { return vec && i0 + (step + 1) * BEAM_STEP <= vocab; };
+    auto index = [&](int step, int e) {
+        return i0 + step * BEAM_STEP + (whole(step) ? (e / W) * (BEAM_THREADS * W) + tid * W + e % W : e * BEAM_THREADS + tid);
+    };
+    auto load = [&](int step, float(&x)[BEAM_EPT]) {
+        if (whole(step)) {
+            uint4 u[NL];
 #pragma unroll
-        for (int i = 0; i < NL; ++i) u[i] = ldg_stream16(p + index(i * W));
+            for (int i = 0; i < NL; ++i) u[i] = ldg_stream16(p + (i0 + step * BEAM_STEP + i * (BEAM_THREADS * W) + tid * W));
 #pragma unroll
-        for (int e = 0; e < EPT; ++e) x[e] = beam_value(reinterpret_cast<const T *>(&u[e / W])[e % W]);
-    } else {
+            for (int e = 0; e < BEAM_EPT; ++e) x[e] = beam_value(reinterpret_cast<const T *>(&u[e / W])[e % W]);
+        } else {
 #pragma unroll
-        for (int e = 0; e < EPT; ++e) x[e] = index(e) < vocab ? beam_value(p[index(e)]) : -INFINITY;
+            for (int e = 0; e < BEAM_EPT; ++e) {
+                const int i = i0 + step * BEAM_STEP + e * BEAM_THREADS + tid;
+                x[e] = i < vocab ? beam_value(p[i]) : -INFINITY;
+            }
+        }
+    };
+    // a power that ends at 2^-200 = 0 where the difference is no number: hidden logits, NaN, an infinite maximum
+    auto power = [](float a, float b) { return beam_ex2(fmaxf((a - b) * 1.44269504f, -200.f)); };
+    float mine = -INFINITY, sum = 0.f;                            // of the thread's logits: maximum, sum of e^(x - maximum)
+    for (int step = 0; step < steps; ++step) {
+        float x[BEAM_EPT];
+        load(step, x);
+        float m = mine;
+#pragma unroll
+        for (int e = 0; e < BEAM_EPT; ++e) m = fmaxf(m, x[e]);    // NaN logits are passed over
+        // in one product where that stays in range (logits at the type's lowest value would leave it) and no NaN came in
+        float add = 0.f;
+        const bool plain = fabsf(m) < 1e38f;
+        if (plain) {
+            const float shift = -m * 1.44269504f;
+#pragma unroll
+            for (int e = 0; e < BEAM_EPT; ++e) add += beam_ex2(fmaf(x[e], 1.44269504f, shift));
+        }
+        if (!plain || add != add) {
+            add = 0.f;
+#pragma unroll
+            for (int e = 0; e < BEAM_EPT; ++e) add += power(x[e], m);
+        }
+        sum = sum * power(mine, m) + add;
+        mine = m;
     }
-    float mine = -INFINITY;
-#pragma unroll
-    for (int e = 0; e < EPT; ++e) mine = fmaxf(mine, x[e]);       // NaN logits are passed over
     const float bound = beam_bound(sm, mine, beams);
     float top = sm.group[lane];
     if (lane >= beam_groups(beams)) top = -INFINITY;
     top = warp_max(top);                                          // the slice's maximum
-    // Sum of 2^((x - top) log2 e), in one product where that stays in range.  Otherwise (logits at the type's lowest value,
-    // an infinite maximum) or where a NaN came in, the difference comes first, and what is no number ends at 2^-200 = 0.
-    float sum = 0.f;
-    const bool plain = fabsf(top) < 1e38f;
-    if (plain) {
-        const float shift = -top * 1.44269504f;
-#pragma unroll
-        for (int e = 0; e < EPT; ++e) sum += beam_ex2(fmaf(x[e], 1.44269504f, shift));
-    }
-    if (!plain || sum != sum) {
-        sum = 0.f;
-#pragma unroll
-        for (int e = 0; e < EPT; ++e) sum += beam_ex2(fmaxf((x[e] - top) * 1.44269504f, -200.f));
-    }
-    sum = warp_sum(sum);
+    sum = warp_sum(sum * power(mine, top));
     if (lane == 0) red[warp] = sum;
-    const int64_t slice = row * gridDim.x + blockIdx.x;
+    const int64_t at = row * gridDim.x + blockIdx.x;
+    const float lo = fmaxf(bound, -FLT_MAX);                      // finite ones only
     beam_best(
         sm, beams, float_key(bound),
-        [&](auto f) {
-            const float lo = fmaxf(bound, -FLT_MAX);              // finite ones only; few threads hold one of the best
+        [&](auto f) {   // few threads hold one of the best: they read theirs again
             if (mine >= lo)
+                for (int step = 0; step < steps; ++step) {
+                    float x[BEAM_EPT];
+                    load(step, x);
 #pragma unroll
-                for (int e = 0; e < EPT; ++e)
-                    if (x[e] >= lo && x[e] <= FLT_MAX) f(((u64)float_key(x[e]) << 32) | (0xFFFFFFFFu - (uint32_t)index(e)));
+                    for (int e = 0; e < BEAM_EPT; ++e)
+                        if (x[e] >= lo && x[e] <= FLT_MAX) f(((u64)float_key(x[e]) << 32) | (0xFFFFFFFFu - (uint32_t)index(step, e)));
+                }
         },
-        [&](int rank, u64 k) { keys[slice * beams + rank] = k; });
+        [&](int rank, u64 k) { keys[at * beams + rank] = k; });
     if (tid == 0) {   // red was written before beam_best's barrier
         sum = red[0];
         for (int w = 1; w < BEAM_THREADS / 32; ++w) sum += red[w];
-        sums[slice] = make_float2(top, sum);
+        sums[at] = make_float2(top, sum);
     }
 }
 
@@ -275,17 +297,16 @@ __global__ void __launch_bounds__(BEAM_THREADS) k_beam_join(const __grid_constan
 }
 
 struct BeamPlan {
-    bool wide;          // slices of 8,192
-    int slices;
+    int slice, slices;
     size_t keys, bytes;
 };
-// Wide slices cost less beside their data; narrow ones keep small steps spread over the SMs (one request of four beams
-// over 151,936 tokens: 76 wide slices, 152 narrow ones).
+// Long slices cost less beside their data, short ones spread small steps over the SMs: the shortest that leaves at most 32
+// CTAs an SM.
 static BeamPlan beam_plan(uint64_t rows, uint32_t beams, uint32_t vocab) {
     BeamPlan p;
-    p.wide = rows * ((vocab + 8191) / 8192) >= 148 * 4;
-    const uint32_t slice = p.wide ? 8192 : 4096;
-    p.slices = (int)(((uint64_t)vocab + slice - 1) / slice);
+    p.slice = BEAM_STEP;
+    while (p.slice < 8 * BEAM_STEP && rows * ((vocab + p.slice - 1) / p.slice) > 148 * 32) p.slice *= 2;
+    p.slices = (int)(((uint64_t)vocab + p.slice - 1) / p.slice);
     p.keys = (rows * p.slices * sizeof(float2) + 255) & ~(size_t)255;
     p.bytes = p.keys + rows * p.slices * beams * sizeof(u64);
     return p;
@@ -295,10 +316,8 @@ template <typename T>
 static cudaError_t launch_slices(const void *logits, int64_t ld, int vocab, int beams, const BeamPlan &p, uint32_t rows, u64 *keys,
                                  float2 *sums, cudaStream_t st) {
     const bool vec = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && ld * sizeof(T) % 16 == 0;
-    const dim3 grid(p.slices, rows);
-    const T *x = static_cast<const T *>(logits);
-    if (p.wide) return launch_k(false, k_beam_slice<T, 32>, grid, BEAM_THREADS, 0, st, x, ld, vocab, beams, vec, keys, sums);
-    return launch_k(false, k_beam_slice<T, 16>, grid, BEAM_THREADS, 0, st, x, ld, vocab, beams, vec, keys, sums);
+    return launch_k(false, k_beam_slice<T>, dim3(p.slices, rows), BEAM_THREADS, 0, st, static_cast<const T *>(logits), ld, vocab, p.slice,
+                    beams, vec, keys, sums);
 }
 
 }  // namespace v3g
