@@ -125,3 +125,32 @@ def test_row_strides_and_streams():
         side.synchronize()
         for a, b in zip(want, got):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_beams_over_long_slices(dtype):
+    """Enough beams that a slice has several steps, the last of them ragged; the best ones of a slice together in one
+    thread's share, in rising and falling order; every slice of a wide group at the bound."""
+    g = torch.Generator().manual_seed(5)
+    groups, beams, vocab = 40, 32, 20001
+    logits = (3 * torch.randn(groups, beams, vocab, generator=g)).to(dtype)
+    logits[1] = torch.arange(vocab) / 1024
+    logits[2] = torch.arange(vocab).flip(0) / 1024
+    logits[3, :, 8192:8232] += 20
+    logits[4, :, 256 * torch.arange(78)] += 20
+    scores = -5 * torch.rand(groups, beams, generator=g)
+    scores[5, 1:] = -math.inf
+    finished = (torch.rand(groups, beams, generator=g) < 0.2).to(torch.uint8)
+    _check(logits, scores, finished, eos=2)
+
+
+def test_ties_of_many_slices():
+    from vault_b200 import beam_select
+    flat = torch.zeros(2, 32, 151936, device="cuda")
+    tokens, parents, best, _ = beam_select(flat, torch.zeros(2, 32, device="cuda"))
+    assert tokens.cpu().tolist() == [list(range(32))] * 2 and int(parents.abs().max()) == 0
+    assert float((best + math.log(151936)).abs().max()) <= 2e-5
+    live = torch.full((2, 32), -math.inf, device="cuda")
+    live[:, 7] = -1.0
+    tokens, parents, _, _ = beam_select(flat, live)
+    assert tokens.cpu().tolist() == [list(range(32))] * 2 and parents.cpu().tolist() == [[7] * 32] * 2

@@ -5,10 +5,14 @@
 // The logits are read once (4 bytes and an exponential per element: HBM bounds it).  Inside a beam the order of the
 // scores is the order of the logits, so the first kernel needs no lse: a CTA streams a slice of one beam's logits, each
 // thread keeping the maximum and the sum of exponentials of its own, and writes the slice's `beams` best as 64-bit keys
-// (value, then lower index).  The second kernel joins the sums of a beam, scores the beams x slices x beams keys and
-// selects again.  Both selections are exact: the `beams`-th largest of some group maxima bounds the answer from below; the few
-// threads whose maximum reaches it read their logits again, and what is at or above it is collected and ranked by
-// counting; where too much is (long ties, sorted logits), `beams` rounds of a block maximum take its place.
+// (value, then lower index).  The second kernel joins the sums of a beam and selects among the slices' best, reading only
+// those of the slices whose maximum can be among the answers.  Both selections are exact: the `beams`-th largest of 64 group
+// maxima bounds the answer from below; the few threads whose maximum reaches it have their logits read again, and what is
+// at or above it is collected and ranked by counting; where too much is (long ties), `beams` rounds of a block maximum take
+// its place.
+//
+// 48 x 8 beams over 151,936 logits (233 MB) take 43 us in fp32 (slices 41, 5.7 TB/s; the join, 6 alone, starts under them) and
+// 35 us in bf16, where loads and powers of a CTA alternate; one request of 4 beams 6.6 us.
 #include <cfloat>
 
 #include "v3g_internal.h"
@@ -17,7 +21,9 @@
 namespace v3g {
 
 constexpr int BEAM_THREADS = 256;
-constexpr int BEAM_BUF = 256;   // collected keys that are ranked by counting
+constexpr int BEAM_BUF = 256;    // collected keys that are ranked by counting
+constexpr int BEAM_GROUPS = 64;  // groups of threads whose maxima give the bound: more than V3G_BEAM_MAX
+constexpr int BEAM_LIST = 512;   // slices the join picks its keys from
 
 typedef unsigned long long u64;
 
@@ -29,30 +35,37 @@ __device__ __forceinline__ u64 shfl_xor64(u64 x, int o) { return __shfl_xor_sync
 struct BeamShared {
     u64 buf[BEAM_BUF];
     u64 red[BEAM_THREADS / 32];
-    float group[32];
-    u64 best;
-    int count;
+    float4 group[BEAM_GROUPS / 4];
+    float bound;
+    int count, listed;
 };
 
-// The `beams`-th largest of the maxima of G groups of threads, G = 8, 16 or 32 >= beams: at least `beams` values of the
-// block are at or above it.
-__device__ __forceinline__ int beam_groups(int beams) { return beams <= 8 ? 8 : (beams <= 16 ? 16 : 32); }
+// The `beams`-th largest of the maxima of the block's groups of threads: at least `beams` values of the block are at or
+// above it.  With 64 groups few others are: 8 beams find 9 values in a slice on average, where 8 groups (one needed of
+// each) let 22 through.
 __device__ __forceinline__ float beam_bound(BeamShared &sm, float v, int beams) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, groups = beam_groups(beams), per = groups / 8;   // groups of a warp
-    for (int o = 1; o < 32 / per; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    if (threadIdx.x == 0) sm.count = 0;
-    if (lane % (32 / per) == 0) sm.group[warp * per + lane / (32 / per)] = v;
-    __syncthreads();
-    v = lane < groups ? sm.group[lane] : -INFINITY;
-    int rank = 0;
-    for (int k = 0; k < groups; k += 8)
+    constexpr int PER = BEAM_THREADS / BEAM_GROUPS, SHARE = BEAM_GROUPS / PER;
+    const int tid = threadIdx.x, mine = tid / PER, first = tid % PER * SHARE;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const float o = __shfl_sync(0xffffffffu, v, k + u);
-            rank += o > v || (o == v && k + u < lane);
-        }
-    const uint32_t at = __ballot_sync(0xffffffffu, lane < groups && rank == beams - 1);
-    return __shfl_sync(0xffffffffu, v, __ffs(at) - 1);
+    for (int o = 1; o < PER; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if (tid == 0) sm.count = sm.listed = 0;
+    if (first == 0) reinterpret_cast<float *>(sm.group)[mine] = v;
+    __syncthreads();
+    // the rank of the group's maximum, its comparisons shared out over the group; equal ones rank by place
+    int rank = 0;
+#pragma unroll
+    for (int k = 0; k < SHARE; k += 4) {
+        const float4 o = sm.group[(first + k) / 4];
+        rank += o.x > v || (o.x == v && first + k < mine);
+        rank += o.y > v || (o.y == v && first + k + 1 < mine);
+        rank += o.z > v || (o.z == v && first + k + 2 < mine);
+        rank += o.w > v || (o.w == v && first + k + 3 < mine);
+    }
+#pragma unroll
+    for (int o = 1; o < PER; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+    if (rank == beams - 1) sm.bound = v;
+    __syncthreads();
+    return sm.bound;
 }
 
 // the block's largest key, to every thread
@@ -120,22 +133,23 @@ __device__ __forceinline__ float beam_ex2(float x) {
 }
 
 // `slice` consecutive logits of a beam (a multiple of BEAM_STEP): the threads' running maxima and sums, then the best
-constexpr int BEAM_EPT = 16, BEAM_STEP = BEAM_THREADS * BEAM_EPT;
+constexpr int BEAM_EPT = 32, BEAM_STEP = BEAM_THREADS * BEAM_EPT;
 template <typename T>
-__global__ void __launch_bounds__(BEAM_THREADS, 6) k_beam_slice(const T *logits, int64_t ld, int vocab, int slice, int beams, bool vec, u64 *keys,
+__global__ void __launch_bounds__(BEAM_THREADS, 4) k_beam_slice(const T *logits, int64_t ld, int vocab, int slice, int beams, bool vec, u64 *keys,
                                                                float2 *sums) {
     __shared__ BeamShared sm;
     __shared__ float red[BEAM_THREADS / 32];
+    __shared__ uint32_t list[BEAM_THREADS];
     griddep_launch();
     constexpr int W = 16 / sizeof(T), NL = BEAM_EPT / W;          // elements of a 16-byte load, loads of a step
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int64_t row = blockIdx.y;
     const int i0 = blockIdx.x * slice, steps = (min(slice, vocab - i0) + BEAM_STEP - 1) / BEAM_STEP;
     const T *p = logits + row * ld;
-    // element e of the thread's share of a step: 16-byte pieces where the step is whole and aligned, else every 256th
+    // element e of thread t's share of a step: 16-byte pieces where the step is whole and aligned, else every 256th
     auto whole = [&](int step) { return vec && i0 + (step + 1) * BEAM_STEP <= vocab; };
-    auto index = [&](int step, int e) {
-        return i0 + step * BEAM_STEP + (whole(step) ? (e / W) * (BEAM_THREADS * W) + tid * W + e % W : e * BEAM_THREADS + tid);
+    auto index = [&](int step, int t, int e) {
+        return i0 + step * BEAM_STEP + (whole(step) ? (e / W) * (BEAM_THREADS * W) + t * W + e % W : e * BEAM_THREADS + t);
     };
     auto load = [&](int step, float(&x)[BEAM_EPT]) {
         if (whole(step)) {
@@ -154,13 +168,18 @@ __global__ void __launch_bounds__(BEAM_THREADS, 6) k_beam_slice(const T *logits,
     };
     // a power that ends at 2^-200 = 0 where the difference is no number: hidden logits, NaN, an infinite maximum
     auto power = [](float a, float b) { return beam_ex2(fmaxf((a - b) * 1.44269504f, -200.f)); };
-    float mine = -INFINITY, sum = 0.f;                            // of the thread's logits: maximum, sum of e^(x - maximum)
+    // of the thread's logits: their maximum, the step that has it, the other steps' maximum, the sum of e^(x - maximum)
+    float mine = -INFINITY, others = -INFINITY, sum = 0.f;
+    int best = 0;
     for (int step = 0; step < steps; ++step) {
         float x[BEAM_EPT];
         load(step, x);
-        float m = mine;
+        float m = -INFINITY;
 #pragma unroll
         for (int e = 0; e < BEAM_EPT; ++e) m = fmaxf(m, x[e]);    // NaN logits are passed over
+        others = fmaxf(others, fminf(mine, m));
+        if (m > mine) best = step;
+        m = fmaxf(mine, m);
         // in one product where that stays in range (logits at the type's lowest value would leave it) and no NaN came in
         float add = 0.f;
         const bool plain = fabsf(m) < 1e38f;
@@ -178,24 +197,30 @@ __global__ void __launch_bounds__(BEAM_THREADS, 6) k_beam_slice(const T *logits,
         mine = m;
     }
     const float bound = beam_bound(sm, mine, beams);
-    float top = sm.group[lane];
-    if (lane >= beam_groups(beams)) top = -INFINITY;
+    const float *group = reinterpret_cast<const float *>(sm.group);
+    float top = fmaxf(group[lane], group[lane + 32]);
     top = warp_max(top);                                          // the slice's maximum
     sum = warp_sum(sum * power(mine, top));
     if (lane == 0) red[warp] = sum;
     const int64_t at = row * gridDim.x + blockIdx.x;
     const float lo = fmaxf(bound, -FLT_MAX);                      // finite ones only
+    // The threads that hold one of the best, with the step to look at, or all of them (the sign bit).  A warp reads such a
+    // share again: were each thread to read its own, most warps would go through 32 elements a step for one thread's sake.
+    if (mine >= lo) list[atomicAdd(&sm.listed, 1)] = (others >= lo ? 0x80000000u : (uint32_t)best << 8) | tid;
+    __syncthreads();
+    const int listed = sm.listed;
     beam_best(
         sm, beams, float_key(bound),
-        [&](auto f) {   // few threads hold one of the best: they read theirs again
-            if (mine >= lo)
-                for (int step = 0; step < steps; ++step) {
-                    float x[BEAM_EPT];
-                    load(step, x);
-#pragma unroll
-                    for (int e = 0; e < BEAM_EPT; ++e)
-                        if (x[e] >= lo && x[e] <= FLT_MAX) f(((u64)float_key(x[e]) << 32) | (0xFFFFFFFFu - (uint32_t)index(step, e)));
+        [&](auto f) {
+            for (int k = tid / BEAM_EPT; k < listed; k += BEAM_THREADS / BEAM_EPT) {
+                const uint32_t l = list[k];
+                const int first = (int)(l >> 31 ? 0 : l >> 8), last = l >> 31 ? steps : first + 1;
+                for (int step = first; step < last; ++step) {
+                    const int i = index(step, l & 255, tid % BEAM_EPT);
+                    const float x = i < vocab ? beam_value(p[i]) : -INFINITY;
+                    if (x >= lo && x <= FLT_MAX) f(((u64)float_key(x) << 32) | (0xFFFFFFFFu - (uint32_t)i));
                 }
+            }
         },
         [&](int rank, u64 k) { keys[at * beams + rank] = k; });
     if (tid == 0) {   // red was written before beam_best's barrier
@@ -206,7 +231,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 6) k_beam_slice(const T *logits,
 }
 
 struct BeamArgs {
-    u64 *keys;          // the slices' best; the join scores them in place
+    const u64 *keys;    // the slices' best, largest first
     const float2 *sums;
     const float *scores;
     const uint8_t *finished;
@@ -219,20 +244,24 @@ struct BeamArgs {
 __global__ void __launch_bounds__(BEAM_THREADS) k_beam_join(const __grid_constant__ BeamArgs a) {
     __shared__ BeamShared sm;
     __shared__ u64 only[V3G_BEAM_MAX];
+    __shared__ float lse[V3G_BEAM_MAX], run[V3G_BEAM_MAX];
     __shared__ bool done[V3G_BEAM_MAX];
+    __shared__ int list[BEAM_LIST];
     griddep_wait();
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, K = a.beams, per = a.slices * K;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, K = a.beams, n = a.slices * K;
     const int64_t g0 = (int64_t)blockIdx.x * K;
-    // a warp takes a beam: its logsumexp, then the scores of its slices' best
-    uint32_t top = 0;
+    const float2 *sums = a.sums + g0 * a.slices;
+    const u64 *keys = a.keys + g0 * a.slices * K;
+    const bool few = n * K <= 4 * BEAM_THREADS;   // every key fits the threads' registers
+    u64 ahead[4];
+    if (few)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ahead[i] = tid + BEAM_THREADS * i < n * K ? keys[tid + BEAM_THREADS * i] : 0ull;
+    // a warp takes a beam: its logsumexp
     for (int k = warp; k < K; k += BEAM_THREADS / 32) {
-        const float2 *p = a.sums + (g0 + k) * a.slices;
-        u64 *keys = a.keys + (g0 + k) * per;
+        const float2 *p = sums + (int64_t)k * a.slices;
         const float run_k = a.scores[g0 + k];
         const bool done_k = a.finished && a.finished[g0 + k];
-        u64 ahead[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) ahead[i] = lane + 32 * i < per ? keys[lane + 32 * i] : 0ull;
         float m = -INFINITY;
         for (int i = lane; i < a.slices; i += 32) m = fmaxf(m, p[i].x);
         m = warp_max(m);
@@ -241,43 +270,52 @@ __global__ void __launch_bounds__(BEAM_THREADS) k_beam_join(const __grid_constan
             const float2 v = p[i];
             if (v.x > -INFINITY) s += v.y * beam_ex2((v.x - m) * 1.44269504f);
         }
-        const float lse = m + logf(warp_sum(s));
-        auto score = [&](u64 key) -> u64 {
-            const float y = (key_float((uint32_t)(key >> 32)) - lse) + run_k;
-            if (done_k || !key || !(y > -INFINITY && y < INFINITY)) return 0ull;
-            return ((u64)float_key(y) << 32) | (0xFFFFFFFFu - ((uint32_t)k * (uint32_t)a.vocab + (0xFFFFFFFFu - (uint32_t)key)));
-        };
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (lane + 32 * i < per) {
-                const u64 y = score(ahead[i]);
-                keys[lane + 32 * i] = y;
-                top = max(top, (uint32_t)(y >> 32));
-            }
-        for (int i = lane + 128; i < per; i += 32) {
-            const u64 y = score(keys[i]);
-            keys[i] = y;
-            top = max(top, (uint32_t)(y >> 32));
-        }
-        // a finished beam's one continuation
-        const bool goes_on = done_k && a.eos >= 0 && run_k > -INFINITY && run_k < INFINITY;
+        s = m + logf(warp_sum(s));
         if (lane == 0) {
+            // a finished beam has one continuation
+            const bool goes_on = done_k && a.eos >= 0 && run_k > -INFINITY && run_k < INFINITY;
             done[k] = done_k;
+            run[k] = run_k;
+            lse[k] = done_k ? NAN : s;   // and no others
             only[k] = goes_on ? ((u64)float_key(run_k) << 32) | (0xFFFFFFFFu - ((uint32_t)k * (uint32_t)a.vocab + (uint32_t)a.eos)) : 0ull;
-            if (goes_on) top = max(top, float_key(run_k));
         }
     }
-    auto each = [&](auto f) {   // every thread its own keys again
-        for (int k = warp; k < K; k += BEAM_THREADS / 32) {
-            const u64 *keys = a.keys + (g0 + k) * per;
-            for (int i = lane; i < per; i += 32) {
-                const u64 y = keys[i];
-                if (y) f(y);
-            }
-            if (lane == 0 && only[k]) f(only[k]);
-        }
+    __syncthreads();
+    // Scores that are no number or infinite stand for nothing.  A slice's best key comes first, and its value is the
+    // slice's maximum (if that is finite): the bound needs no keys.
+    auto score = [&](int k, float x) -> float {
+        const float y = (x - lse[k]) + run[k];
+        return y > -INFINITY && y < INFINITY ? y : -INFINITY;
     };
-    const float bound = beam_bound(sm, top ? key_float(top) : -INFINITY, K);
+    // consecutive slices go to different groups of the bound: often one beam alone has candidates
+    const int mine = tid % (BEAM_THREADS / BEAM_GROUPS) * BEAM_GROUPS + tid / (BEAM_THREADS / BEAM_GROUPS);
+    float top = tid < K && only[tid] ? run[tid] : -INFINITY;
+    for (int i = mine; i < n; i += BEAM_THREADS) top = fmaxf(top, score(i / a.slices, sums[i].x));
+    const float bound = beam_bound(sm, top, K), lo = fmaxf(bound, -FLT_MAX);
+    if (!few && top >= lo)
+        for (int i = mine; i < n; i += BEAM_THREADS)
+            if (score(i / a.slices, sums[i].x) >= lo) {
+                const int at = atomicAdd(&sm.listed, 1);
+                if (at < BEAM_LIST) list[at] = i;
+            }
+    if (!few) __syncthreads();
+    const bool all = sm.listed > BEAM_LIST;   // long ties: every slice
+    const int picked = few ? 0 : (all ? n : sm.listed);
+    auto each = [&](auto f) {
+        auto pick = [&](int k, u64 key) {
+            const float y = key ? score(k, key_float((uint32_t)(key >> 32))) : -INFINITY;
+            if (y >= lo) f(((u64)float_key(y) << 32) | (0xFFFFFFFFu - ((uint32_t)k * (uint32_t)a.vocab + (0xFFFFFFFFu - (uint32_t)key))));
+        };
+        if (few)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (ahead[i]) pick((tid + BEAM_THREADS * i) / (a.slices * K), ahead[i]);
+        for (int64_t i = tid; i < (int64_t)picked * K; i += BEAM_THREADS) {
+            const int at = all ? (int)(i / K) : list[(int)i / K];
+            pick(at / a.slices, keys[(int64_t)at * K + i % K]);
+        }
+        if (tid < K && only[tid]) f(only[tid]);
+    };
     beam_best(sm, K, float_key(bound), each, [&](int rank, u64 k) {
         const int64_t at = g0 + rank;
         if (k) {
@@ -300,13 +338,16 @@ struct BeamPlan {
     int slice, slices;
     size_t keys, bytes;
 };
-// Long slices cost less beside their data, short ones spread small steps over the SMs: the shortest that leaves at most 32
-// CTAs an SM.
+// Long slices cost less beside their data, short ones spread small steps over the SMs: as many slices as make two rounds
+// of the 4 CTAs that fit an SM (48 x 8 beams over 151,936 fp32 logits: one round 47 us, two 43, four 45; 8 x 16 beams 24.5,
+// 24.6, 26.5).
+constexpr uint64_t BEAM_SLICES = 2 * 148 * 4;
 static BeamPlan beam_plan(uint64_t rows, uint32_t beams, uint32_t vocab) {
     BeamPlan p;
-    p.slice = BEAM_STEP;
-    while (p.slice < 8 * BEAM_STEP && rows * ((vocab + p.slice - 1) / p.slice) > 148 * 32) p.slice *= 2;
-    p.slices = (int)(((uint64_t)vocab + p.slice - 1) / p.slice);
+    const uint64_t steps = ((uint64_t)vocab + BEAM_STEP - 1) / BEAM_STEP, want = std::max<uint64_t>(BEAM_SLICES / rows, 1);
+    const uint64_t each = (steps + want - 1) / want;
+    p.slice = (int)(each * BEAM_STEP);
+    p.slices = (int)((steps + each - 1) / each);
     p.keys = (rows * p.slices * sizeof(float2) + 255) & ~(size_t)255;
     p.bytes = p.keys + rows * p.slices * beams * sizeof(u64);
     return p;
