@@ -11,14 +11,15 @@ from .vlt3 import VLT3Error, read_vlt3, vlt3_config, write_vlt3
 
 
 def __getattr__(name):
-    # torch-dependent classes load lazily so the format tools work without CUDA
+    # torch-dependent classes load lazily so the format tools work without CUDA; once loaded they are plain names
     if name in ("Governor", "VAULTv3ForCausalLM", "VAULTv3State", "sample_topk"):
-        from . import model
-        return getattr(model, name)
-    if name in ("PagedKVCache", "beam_select", "rope_table"):
-        from . import paged
-        return getattr(paged, name)
-    raise AttributeError(name)
+        from . import model as home
+    elif name in ("PagedKVCache", "beam_select", "rope_table"):
+        from . import paged as home
+    else:
+        raise AttributeError(name)
+    globals()[name] = value = getattr(home, name)
+    return value
 
 
 __all__ = ["Governor", "PagedKVCache", "VAULTv3Config", "VAULTv3ForCausalLM", "VAULTv3State", "VLT3Error", "beam_select", "read_vlt3",

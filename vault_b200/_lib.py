@@ -12,6 +12,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libvault_b200.so")
 
 V3G_OK = 0
+V3G_E_SIZE = -1
 V3G_STATE_PER_SEQ_MEMORY, V3G_STATE_NO_AUTOPIN, V3G_STATE_NO_GRAPHS, V3G_STATE_NO_PERSISTENT = 1, 2, 4, 8
 V3G_STATE_TOKEN_PREFILL = 16
 V3G_STATE_FP16_ACTIVATIONS = 32

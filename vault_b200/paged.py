@@ -24,7 +24,8 @@ import torch
 
 from . import _lib
 
-BLOCK = 16   # tokens that share a scale
+BLOCK = 16      # tokens that share a scale
+_FAR = 1 << 30  # past every position
 _DTYPES = {torch.float32: _lib.V3G_F32, torch.float16: _lib.V3G_F16, torch.bfloat16: _lib.V3G_BF16}
 
 
@@ -44,10 +45,11 @@ def _index(t: torch.Tensor, name: str, device, n: int) -> int:
     return t.data_ptr()
 
 
-def _stream(device) -> int:
-    """torch's current stream on `device` as the C ABI takes it (the call behind torch.cuda.current_stream, without the
-    Python object around it: 0.1 us instead of 2.3)."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
+# The current device, torch's current stream of a device as the C ABI takes it, and whether it is being captured: the calls
+# behind torch.cuda's, without the Python objects around them (the stream 0.1 us instead of 2.3).
+_current_device = torch._C._cuda_getDevice
+_stream = torch._C._cuda_getCurrentRawStream
+_capturing = torch._C._cuda_isCurrentStreamCapturing
 
 
 class _Workspaces:
@@ -57,14 +59,26 @@ class _Workspaces:
     def __init__(self):
         self.by_stream = {}
 
-    def get(self, device, stream: int, size: int) -> int:
-        if torch.cuda.is_current_stream_capturing():
-            return torch.empty(size, dtype=torch.uint8, device=device).data_ptr()
-        held = self.by_stream.get((device.index, stream))
-        if held is None or held[0] < size:
-            t = torch.empty(size, dtype=torch.uint8, device=device)
-            held = self.by_stream[(device.index, stream)] = (size, t.data_ptr(), t)
-        return held[1]
+    def run(self, device, size, call) -> int:
+        """call(workspace, its bytes, stream) on torch's current stream of `device`, which becomes the current device for
+        the call.  The workspace that is there is offered as it is: the engine refuses one that is too small before it
+        does anything else, and only then is size() asked."""
+        index = device.index
+        if _current_device() != index:
+            with torch.cuda.device(device):
+                return self.run(device, size, call)
+        stream = _stream(index)
+        if _capturing():
+            t = torch.empty(size(), dtype=torch.uint8, device=device)
+            return call(t.data_ptr(), t.numel(), stream)
+        held = self.by_stream.get((index, stream))
+        if held is not None:
+            rc = call(held[0], held[1], stream)
+            if rc != _lib.V3G_E_SIZE:
+                return rc
+        t = torch.empty(max(size(), 1 << 16), dtype=torch.uint8, device=device)
+        self.by_stream[(index, stream)] = (t.data_ptr(), t.numel(), t)
+        return call(t.data_ptr(), t.numel(), stream)
 
 
 _beam_work = _Workspaces()
@@ -105,6 +119,8 @@ class PagedKVCache:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.n_layers, self.n_pages, self.n_kv_heads, self.page, self.head_dim = k.shape
         self.device = k.device
+        self._index = k.device.index
+        self._scale = self.head_dim ** -0.5
         self.status_word = torch.zeros(1, dtype=torch.int32, device=k.device)
         self._status = self.status_word.data_ptr()
         self._work = _Workspaces()
@@ -151,12 +167,12 @@ class PagedKVCache:
 
     def _call(self, fn, what: str, *args) -> None:
         """fn on torch's current stream of the cache's device, which becomes the current device for the call."""
-        dev = self.device
-        if torch._C._cuda_getDevice() == dev.index:
-            rc = fn(*args, _stream(dev))
+        index = self._index
+        if _current_device() == index:
+            rc = fn(*args, _stream(index))
         else:
-            with torch.cuda.device(dev):
-                rc = fn(*args, _stream(dev))
+            with torch.cuda.device(self.device):
+                rc = fn(*args, _stream(index))
         if rc:
             _lib.check(rc, what)
 
@@ -221,14 +237,17 @@ class PagedKVCache:
             raise ValueError("out must be a contiguous tensor of q's shape and type")
         lse = torch.empty(n, heads, dtype=torch.float32, device=self.device) if return_lse else None
         if n:
-            L = _lib.lib()
-            window, n_sink = min(window, 1 << 30), min(n_sink, 1 << 30)
-            max_q, max_kv = min(max_q, 0x7FFFFFFF), min(max_kv, 0x7FFFFFFF)
-            size = L.v3g_kv_attention_work_size(self._ref, batch, heads, max_q, max_kv, window, n_sink)
-            self._call(L.v3g_kv_attention, "v3g_kv_attention", self._ref, self._layer(layer), batch, _DTYPES[dtype], qr, heads,
-                       self.head_dim ** -0.5 if scale is None else float(scale), window, n_sink, max_q, max_kv, out.data_ptr(),
-                       None if lse is None else lse.data_ptr(), self._status,
-                       self._work.get(self.device, _stream(self.device), size) if size else None, size)
+            if window > _FAR or n_sink > _FAR or max_q > _FAR or max_kv > _FAR:
+                window, n_sink, max_q, max_kv = (min(x, _FAR) for x in (window, n_sink, max_q, max_kv))
+            L, ref, layer, dt = _lib.lib(), self._ref, self._layer(layer), _DTYPES[dtype]
+            scale = self._scale if scale is None else float(scale)
+            lse_ptr = None if lse is None else lse.data_ptr()
+            rc = self._work.run(
+                self.device, lambda: L.v3g_kv_attention_work_size(ref, batch, heads, max_q, max_kv, window, n_sink),
+                lambda work, size, stream: L.v3g_kv_attention(ref, layer, batch, dt, qr, heads, scale, window, n_sink, max_q, max_kv,
+                                                              out.data_ptr(), lse_ptr, self._status, work, size, stream))
+            if rc:
+                _lib.check(rc, "v3g_kv_attention")
         return (out, lse) if return_lse else out
 
     def read(self, page_table: torch.Tensor, first: torch.Tensor, kv_len: torch.Tensor, row_start: torch.Tensor, n_rows: int,
@@ -281,35 +300,29 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: Optional[t
     dt = _DTYPES.get(logits.dtype)
     if dt is None or logits.dim() != 3 or not logits.is_cuda or logits.numel() == 0:
         raise ValueError("logits must be a CUDA tensor [groups, beams, vocab] of fp32, fp16 or bf16")
-    shape = b, k, v = logits.shape
+    b, k, v = logits.shape
+    rows = (b, k)
     s0, s1, s2 = logits.stride()
     ld = s1 if k > 1 else (s0 if b > 1 else v)
     if (s2 != 1 and v > 1) or ld < v or (b > 1 and k > 1 and s0 != k * ld):
         raise ValueError("logits must have contiguous rows, evenly spaced")
     dev = logits.device
-    if scores.dtype is not torch.float32 or scores.shape != shape[:2] or scores.device != dev or not scores.is_contiguous():
+    if scores.dtype is not torch.float32 or scores.shape != rows or scores.device != dev or not scores.is_contiguous():
         raise ValueError("scores must be a contiguous fp32 [groups, beams] tensor on the logits' device")
-    if finished is not None and (finished.dtype not in (torch.uint8, torch.bool) or finished.shape != shape[:2] or
+    if finished is not None and (finished.dtype not in (torch.uint8, torch.bool) or finished.shape != rows or
                                  finished.device != dev or not finished.is_contiguous()):
         raise ValueError("finished must be a contiguous uint8 [groups, beams] tensor on the logits' device")
     L = _lib.lib()
-    size = L.v3g_beam_select_work_size(b, k, v)
     best = torch.empty_like(scores)
     tokens = torch.empty_like(scores, dtype=torch.int32)
     parents = torch.empty_like(tokens)
     done = torch.empty_like(scores, dtype=torch.uint8)
-
-    def call():
-        stream = _stream(dev)
-        return L.v3g_beam_select(logits.data_ptr(), dt, b, k, v, ld, scores.data_ptr(), None if finished is None else finished.data_ptr(),
-                                 eos_id, tokens.data_ptr(), parents.data_ptr(), best.data_ptr(), done.data_ptr(),
-                                 _beam_work.get(dev, stream, size) if size else None, size, stream)
-
-    if torch._C._cuda_getDevice() == dev.index:
-        rc = call()
-    else:
-        with torch.cuda.device(dev):
-            rc = call()
+    done_ptr = None if finished is None else finished.data_ptr()
+    rc = _beam_work.run(
+        dev, lambda: L.v3g_beam_select_work_size(b, k, v),
+        lambda work, size, stream: L.v3g_beam_select(logits.data_ptr(), dt, b, k, v, ld, scores.data_ptr(), done_ptr, eos_id,
+                                                     tokens.data_ptr(), parents.data_ptr(), best.data_ptr(), done.data_ptr(), work, size,
+                                                     stream))
     if rc:
         _lib.check(rc, "v3g_beam_select")
     return tokens, parents, best, done
