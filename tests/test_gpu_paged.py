@@ -447,3 +447,30 @@ def test_reorder_leaves_impossible_rows():
         assert torch.equal(out, t)
         for a, b in zip(_parts(cache), parts):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("batch,hkv,hq,d,page,longest,window,sinks", [(20, 16, 16, 128, 64, 2500, 0, 0), (70, 4, 16, 64, 32, 1500, 0, 0),
+                                                                     (100, 4, 4, 128, 16, 900, 300, 5), (45, 8, 16, 128, 128, 700, 0, 0)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_attention_of_uneven_batches(batch, hkv, hq, d, page, longest, window, sinks, dtype):
+    """Batches whose key shares follow the sequences' lengths: a few long ones among short ones, some of no token, some that
+    see nothing; the same bits at every call, and a hint that is too small changes nothing but the split."""
+    g = torch.Generator().manual_seed(batch)
+    new = [[1, 1, 0, 3, 2, 1, 1][b % 7] for b in range(batch)]
+    ctx = [int(longest * float(torch.rand(1, generator=g)) ** 6) for b in range(batch)]
+    ctx[0], ctx[-1], ctx[5] = longest, longest, 0
+    bt = ref.Batch(new, ctx, page, seed=batch)
+    bt.table[4] = -1
+    parts = ref.random_cache(1, bt.n_pages, hkv, page, d, seed=hkv)
+    q = torch.randn(bt.n, hq, d, generator=g).to(dtype)
+    out, lse = _attend(parts, bt, q, window, sinks, max_q=3, max_kv=longest + 3)
+    want, want_lse, tol, tol_lse = ref.attention(q, parts, 0, bt, window, sinks, d ** -0.5)
+    for _ in range(2):
+        err = (out.cpu().double() - want).abs()
+        assert bool((err <= tol + HALF_ULP[dtype] * want.abs() + SMALLEST[dtype]).all()), float((err - tol).max())
+        seen = ~torch.isinf(want_lse)
+        assert torch.equal(torch.isinf(lse.cpu()), ~seen)
+        assert bool(((lse.cpu().double() - want_lse).abs()[seen] <= tol_lse[seen]).all())
+        again = _attend(parts, bt, q, window, sinks, max_q=3, max_kv=longest + 3)
+        assert torch.equal(_attend(parts, bt, q, window, sinks, max_q=3, max_kv=longest + 3)[0], again[0])
+        out, lse = _attend(parts, bt, q, window, sinks, max_q=3, max_kv=64)

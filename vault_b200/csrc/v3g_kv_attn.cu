@@ -18,6 +18,9 @@
 //   and the accumulators are fp32.  The maximum is raised only when a score exceeds it by 8 (P' then stays below 2^12).
 // * O^T[d, row] = V^T P'^T: V's bytes of four keys are interleaved into fragments, P' is transposed with movmatrix.
 //   Splits of one row are joined by a second kernel in split order, so results do not depend on timing.
+//
+// 4 sequences of 100,000 keys, 32/8 heads (819 MB): 136 us, 6.0 TB/s; 64 of 1,411-4,608 keys, 12/2 heads (93 MB): 26 us, of
+// which about 8 are the launch, the chain length -> page -> codes and the join; one of 1,545 keys: 8 us, all latency.
 #include <cfloat>
 #include <cmath>
 #include <type_traits>
@@ -70,40 +73,146 @@ struct Bytes<8> {
     }
 };
 
+// Unit u of the a.units in which the key blocks of the whole batch are shared out: its sequence (-1: none), which of the
+// sequence's `shares` it is.  One warp works it out from the lengths (nb: place for them, a lane touches its own entries): the
+// smallest share size, to a sixteenth, whose shares fit the units.
+constexpr int BALANCE_MAX = 256;   // sequences
+__device__ __forceinline__ int kv_share(const KvAttnArgs &a, int u, int *nb, int &split, int &shares) {
+    const int lane = threadIdx.x & 31, to = (a.c.batch + 31) / 32 * 32 + lane;
+    int total = 0, top = 0;
+#pragma unroll 2
+    for (int b = lane; b < to; b += 32) {
+        const int at = min(b, a.c.batch - 1);   // the loads wait for one another nowhere
+        int first, x, y, n = a.c.tokens(at, first);
+        const int p0 = a.c.end(at) - n, seen = min(max(kv_visible(a, p0, p0 + n - 1, KV_BLOCK, x, y), 1), 1 << 22);
+        n = b < a.c.batch && n > 0 && n * a.group <= a.max_rows ? seen : 0;
+        nb[b] = n;
+        total += n;
+        top = max(top, n);
+    }
+    total = __reduce_add_sync(0xffffffffu, total);
+    top = __reduce_max_sync(0xffffffffu, top);
+    auto parts = [](int n, float inv) { return __float2int_ru(n * inv); };   // one at least; a whole multiple is not rounded up
+    int lo = max((total + a.units - 1) / a.units, DEC_MIN_BLOCKS), per = max(lo, top);   // per: one share each, which fits
+    while (per - lo > lo / 16) {
+        const int mid = (lo + per) / 2;
+        const float inv = 0.999999f / mid;
+        int need = 0;
+#pragma unroll 2
+        for (int b = lane; b < to; b += 32) need += parts(nb[b], inv);
+        if ((int)__reduce_add_sync(0xffffffffu, need) <= a.units) per = mid;
+        else lo = mid + 1;
+    }
+    const float inv = 0.999999f / per;
+    int before = 0;
+#pragma unroll 1
+    for (int b = lane; b < to; b += 32) {
+        const int mine = min(parts(nb[b], inv), a.splits);
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, u < before + upto);
+        if (past) {
+            const int l = __ffs(past) - 1;
+            shares = __shfl_sync(0xffffffffu, mine, l);
+            split = u - before - __shfl_sync(0xffffffffu, upto - mine, l);
+            return b - lane + l;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return -1;
+}
+
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 2) k_kv_decode(const __grid_constant__ KvAttnArgs a) {
     constexpr int ROWS = 8 * NT, NCH = D / 64, VB = D / 8, MT = D / 16, OS = D + 4;
     constexpr bool TWO = std::is_same<T, __half>::value;
+    __shared__ int sm_share[3];
     __shared__ float sm_m[DEC_WARPS][ROWS], sm_l[DEC_WARPS][ROWS];
     __shared__ __align__(16) float sm_o[DEC_WARPS][ROWS][OS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     int idx = blockIdx.x;
     const int rt0 = idx % a.row_tiles;
     idx /= a.row_tiles;
-    const int split = idx % a.splits;
-    idx /= a.splits;
-    const int h = idx % a.c.heads, b = idx / a.c.heads;
+    int h, b, split, shares = a.splits;
+    griddep_launch();
+    if (a.units) {
+        h = idx % a.c.heads;
+        if (warp == 0) {
+            b = kv_share(a, idx / a.c.heads, reinterpret_cast<int *>(sm_o), split, shares);
+            if (lane == 0) sm_share[0] = b, sm_share[1] = split, sm_share[2] = shares;
+        }
+        __syncthreads();
+        b = sm_share[0], split = sm_share[1], shares = sm_share[2];
+        if (b < 0) return;
+    } else {
+        split = idx % a.splits;
+        idx /= a.splits;
+        h = idx % a.c.heads;
+        b = idx / a.c.heads;
+    }
     int first;
     const int n = a.c.tokens(b, first);
     const int rows = n * a.group > a.max_rows ? 0 : n * a.group;             // else they are the many-row kernel's
     const int p0 = a.c.end(b) - n;
-    griddep_launch();
     for (int rt = rt0; rt * ROWS < rows; rt += a.row_tiles) {
         const int r0 = rt * ROWS, rn = min(rows - r0, ROWS);
         const int pmin = p0 + r0 / a.group, pmax = p0 + (r0 + rn - 1) / a.group;
         int sb, ws;                                                          // blocks [0, sb) and [ws, ws + nb - sb)
         const int nb = kv_visible(a, pmin, pmax, KV_BLOCK, sb, ws);
-        const int per = max((nb + a.splits - 1) / a.splits, DEC_MIN_BLOCKS);
+        const int per = max((nb + shares - 1) / shares, DEC_MIN_BLOCKS);
         const int lo = split * per, hi = min(nb, lo + per);
 
+        auto row_of = [&](int r) {
+            const int rr = r0 + r, tok = rr / a.group;
+            return (int64_t)(first + tok) * a.c.heads * a.group + h * a.group + rr - tok * a.group;
+        };
+        if (split == shares - 1)                                             // shares that the sequence does not have
+            for (int i = threadIdx.x; i < rn * (a.splits - shares); i += 32 * DEC_WARPS)
+                a.part_ml[row_of(i % rn) * a.part_stride + shares + i / rn] = make_float2(-INFINITY, 0.f);
         if (lo >= hi && a.splits > 1) {                                      // no share for this CTA
-            if (threadIdx.x < rn) {
-                const int rr = r0 + threadIdx.x, tok = rr / a.group;
-                const int64_t row = (int64_t)(first + tok) * a.c.heads * a.group + h * a.group + rr - tok * a.group;
-                a.part_ml[row * a.part_stride + split] = make_float2(-INFINITY, 0.f);
-            }
+            if (threadIdx.x < rn) a.part_ml[row_of(threadIdx.x) * a.part_stride + split] = make_float2(-INFINITY, 0.f);
             continue;
         }
+        // lane i looks up the i-th of the warp's next 32 blocks: its page, then its place and scales
+        int64_t my_at, at;
+        float my_ks, my_vs;
+        auto position = [&](int base) {
+            const int vi = base + DEC_WARPS * lane;
+            return vi < hi ? (vi < sb ? vi : vi - sb + ws) * KV_BLOCK : -1;
+        };
+        auto place = [&](int pos, int pg) {
+            my_at = -1;
+            my_ks = my_vs = 0.f;
+            if (pg >= 0) {
+                my_at = a.c.block(pg, h, pos);
+                my_ks = a.c.ks[my_at];
+                my_vs = a.c.vs[my_at];
+            }
+        };
+        Bytes<16> kr[NCH][2];
+        Bytes<VB> vr[4];
+        auto load_k = [&](int64_t at) {
+            if (at < 0) return;
+            const uint8_t *p = a.c.k + at * (KV_BLOCK * D) + g * D + 16 * t;
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) {
+                kr[c][0].load(p + 64 * c);
+                kr[c][1].load(p + 8 * D + 64 * c);
+            }
+        };
+        auto load_v = [&](int64_t at) {
+            if (at < 0) return;
+            const uint8_t *p = a.c.v + at * (KV_BLOCK * D) + 2 * t * D + g * VB;
+            vr[0].load(p);
+            vr[1].load(p + D);
+            vr[2].load(p + 8 * D);
+            vr[3].load(p + 9 * D);
+        };
+        const int pos0 = position(lo + warp), pg0 = a.c.page_of(b, pos0);   // on its way while the queries are laid out
         // queries: row g of each n tile, dims 64 c + 16 t .. + 15
         uint32_t qf[NT][NCH][8];
         float qs[NT][2], m[NT][2], l[NT][2];
@@ -140,6 +249,10 @@ __global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 2) k_kv_decode(c
                 l[nt][i] = 0.f;
             }
         }
+        place(pos0, pg0);
+        at = __shfl_sync(0xffffffffu, my_at, 0);
+        load_k(at);
+        load_v(at);
         float acc[MT][NT][4], ref = 0.f, inv_ref = 0.f;
 #pragma unroll
         for (int j = 0; j < MT; ++j)
@@ -149,43 +262,14 @@ __global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 2) k_kv_decode(c
                 for (int i = 0; i < 4; ++i) acc[j][nt][i] = 0.f;
 
         for (int base = lo + warp; base < hi; base += 32 * DEC_WARPS) {
-            // lane i looks up the warp's i-th block from here: page, scales
-            int64_t my_at = -1;
-            float my_ks = 0.f, my_vs = 0.f;
-            {
-                const int vi = base + DEC_WARPS * lane;
-                if (vi < hi) {
-                    const int pos = (vi < sb ? vi : vi - sb + ws) * KV_BLOCK, pg = a.c.page_of(b, pos);
-                    if (pg >= 0) {
-                        my_at = a.c.block(pg, h, pos);
-                        my_ks = a.c.ks[my_at];
-                        my_vs = a.c.vs[my_at];
-                    }
-                }
-            }
             const int cnt = min(32, (hi - base + DEC_WARPS - 1) / DEC_WARPS);
-            Bytes<16> kr[NCH][2];
-            Bytes<VB> vr[4];
-            auto load_k = [&](int64_t at) {
-                if (at < 0) return;
-                const uint8_t *p = a.c.k + at * (KV_BLOCK * D) + g * D + 16 * t;
-#pragma unroll
-                for (int c = 0; c < NCH; ++c) {
-                    kr[c][0].load(p + 64 * c);
-                    kr[c][1].load(p + 8 * D + 64 * c);
-                }
-            };
-            auto load_v = [&](int64_t at) {
-                if (at < 0) return;
-                const uint8_t *p = a.c.v + at * (KV_BLOCK * D) + 2 * t * D + g * VB;
-                vr[0].load(p);
-                vr[1].load(p + D);
-                vr[2].load(p + 8 * D);
-                vr[3].load(p + 9 * D);
-            };
-            int64_t at = __shfl_sync(0xffffffffu, my_at, 0);
-            load_k(at);
-            load_v(at);
+            if (base != lo + warp) {
+                const int pos = position(base);
+                place(pos, a.c.page_of(b, pos));
+                at = __shfl_sync(0xffffffffu, my_at, 0);
+                load_k(at);
+                load_v(at);
+            }
             for (int it = 0; it < cnt; ++it) {
                 const int64_t next = it + 1 < cnt ? __shfl_sync(0xffffffffu, my_at, it + 1) : -1;
                 const float ks = __shfl_sync(0xffffffffu, my_ks, it), vs = __shfl_sync(0xffffffffu, my_vs, it);
@@ -334,8 +418,7 @@ __global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 2) k_kv_decode(c
                 const float4 x = *reinterpret_cast<const float4 *>(&sm_o[w][r][d]);
                 o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
             }
-            const int rr = r0 + r, tok = rr / a.group;
-            const int64_t row = (int64_t)(first + tok) * a.c.heads * a.group + h * a.group + rr - tok * a.group;
+            const int64_t row = row_of(r);
             if (a.splits > 1) {
                 if (d == 0) a.part_ml[row * a.part_stride + split] = make_float2(mx, ls);
                 if (lo < hi) *reinterpret_cast<float4 *>(a.part_o + (row * a.part_stride + split) * D + d) = o;
@@ -349,7 +432,8 @@ __global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 2) k_kv_decode(c
     }
 }
 
-// Joins the shares of a row: WR warps take every WR-th share each, in order, and are added in order.
+// Joins the shares of a row: WR warps take every WR-th share each, in order, and are added in order.  Latency bounds it (5 us
+// alone for 768 rows of 4 shares); it starts under the kernel before it and finds its row's sequence meanwhile.
 template <typename T, int D, int WR>
 __global__ void __launch_bounds__(128) k_kv_join(const __grid_constant__ KvAttnArgs a) {
     constexpr int W = D / 32, ROWS = 4 / WR;
@@ -372,11 +456,17 @@ __global__ void __launch_bounds__(128) k_kv_join(const __grid_constant__ KvAttnA
 #pragma unroll
     for (int i = 0; i < W; ++i) o[i] = 0.f;
     if (shares > 1) {
-        for (int s = lane; s < shares; s += 32) mx = fmaxf(mx, ml[s].x);
+        int used = 0;                              // places past the sequence's shares hold (-inf, 0), nothing was written for them
+        for (int s = lane; s < shares; s += 32) {
+            const float2 x = ml[s];
+            mx = fmaxf(mx, x.x);
+            if (!(x.x == -INFINITY && x.y == 0.f)) used = s + 1;
+        }
         mx = warp_max(mx);
+        used = __reduce_max_sync(0xffffffffu, used);
         const float mu = mx == -INFINITY ? 0.f : mx;
 #pragma unroll 4
-        for (int s = w0; s < shares; s += WR) {
+        for (int s = w0; s < used; s += WR) {
             const float2 x = ml[s];
             const float f = ex2(x.x - mu);         // 0 for a share without a visible key, whose part was not written
             const float *p = a.part_o + (row * a.part_stride + s) * D + W * lane;
@@ -418,7 +508,7 @@ constexpr size_t PART_BYTES_MAX = (size_t)64 << 20;   // partial results stay in
 
 struct KvAttnPlan {
     bool few, many;              // kernels that run
-    int nt, row_tiles, splits, pf_items, pf_splits, part_stride, max_rows;
+    int nt, row_tiles, splits, units, pf_items, pf_splits, part_stride, max_rows;
     size_t part_o, bytes;
 };
 
@@ -452,13 +542,21 @@ static KvAttnPlan kv_plan(const v3g_kv_cache_t *c, const v3g_kv_batch_t *b, uint
         while (tiles > 1 && tiles * seq > 0x1000000u) tiles = (tiles + 1) / 2;   // a tile loop serves the rest
         p.row_tiles = (int)tiles;
         const uint64_t blocks = (seen(tokens) + KV_BLOCK - 1) / KV_BLOCK, most = (blocks + DEC_MIN_BLOCKS - 1) / DEC_MIN_BLOCKS;
-        // Every CTA slot (4 per SM) gets a share, none less than DEC_MIN_BLOCKS blocks.  More shares than slots cost more than the
-        // balance they bring (64 sequences of 1,411-4,608 keys: 29.5 us, with twice the shares 31.5 us); beside the many-row
-        // kernel, whose sequences take no shares here, twice as many.
-        uint64_t s = (p.many ? 148 * 8 : 148 * 4) / (seq * tiles);
+        // Every CTA slot (4 per SM) gets a share, none less than DEC_MIN_BLOCKS blocks; beside the many-row kernel, whose
+        // sequences take no shares here, twice as many.  Where a sequence's shares would be few (1 to 7), they are given out by
+        // the lengths instead: 64 sequences of 1,411-4,608 keys take 26.3 us instead of 29.1, 128 of them 45.6 instead of
+        // 51.9, for 2 us of one warp's work per CTA that equal lengths pay for nothing (64 of 3,000: 27.2 instead of 25.3).
+        // With more shares each, or more units than slots, nothing is won.
+        const uint64_t slots = (p.many ? 148 * 8 : 148 * 4) / (c->n_kv_heads * tiles);
+        uint64_t s = slots / b->batch;
+        if (!p.many && b->batch > 1 && b->batch <= BALANCE_MAX && slots > b->batch && slots < 8 * (uint64_t)b->batch) {
+            p.units = (int)slots;
+            s = slots - b->batch + 1 < 4 * s + 4 ? slots - b->batch + 1 : 4 * s + 4;
+        }
         s = s > most ? most : s;
         s = s > room ? room : s;
         p.splits = s < 1 ? 1 : (s > 128 ? 128 : (int)s);
+        if (p.splits == 1) p.units = 0;
     }
     if (p.many) {
         // Units that have room in the grid, and about how many of them hold rows: sequences end within one.  Fewer than
@@ -486,7 +584,7 @@ template <typename T, int D>
 static cudaError_t launch_attention_kernels(const KvAttnArgs &a, const KvAttnPlan &p, int dtype, cudaStream_t st) {
     cudaError_t e = cudaSuccess;
     if (p.few) {
-        const dim3 grid((uint32_t)((uint64_t)a.c.batch * a.c.heads * a.splits * a.row_tiles));
+        const dim3 grid((uint32_t)((a.units ? (uint64_t)a.units : (uint64_t)a.c.batch * a.splits) * a.c.heads * a.row_tiles));
         if (p.nt == 1) e = launch_k(false, k_kv_decode<T, D, 1>, grid, 32 * DEC_WARPS, 0, st, a);
         else e = launch_k(false, k_kv_decode<T, D, 2>, grid, 32 * DEC_WARPS, 0, st, a);
     }
@@ -549,6 +647,7 @@ extern "C" int v3g_kv_attention(const v3g_kv_cache_t *cache, uint32_t layer, con
     a.out = out;
     a.lse = lse;
     a.splits = p.splits;
+    a.units = p.units;
     a.row_tiles = p.row_tiles;
     a.max_rows = p.max_rows;
     a.pf_items = p.pf_items;

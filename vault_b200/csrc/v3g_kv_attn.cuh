@@ -18,7 +18,8 @@ struct KvAttnArgs {
     float *lse;                // [tokens][query heads], or null
     // sequences of at most max_rows rows (tokens x group) are the few-row kernel's, the others the many-row kernel's
     int max_rows;
-    int splits, row_tiles;     // few rows: key shares, row tiles in the grid
+    int splits, row_tiles;     // few rows: key shares of a sequence at most, row tiles in the grid
+    int units;                 // few rows: shares of the whole batch, given out by the sequences' lengths; 0: `splits` each
     int pf_items, pf_splits;   // many rows: units of 256 rows that a head has room for, key shares
     bool after_few;            // the many-row kernel starts while the few-row kernel runs, and ends after it
     int part_stride;           // shares that a row has room for
