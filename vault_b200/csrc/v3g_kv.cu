@@ -19,7 +19,8 @@ namespace v3g {
 //
 // x' = rotation of x (pairs i, i + D/2; fp32, each product and sum rounded by itself), s = max(s_old, max |x'| / 127),
 // code = rint(x' * (1 / s)).  A larger s moves the block's earlier codes to rint(code * (s_old / s)).
-// 11,247 bf16 tokens with 32/8 heads of 128 (254 MB) take 60 us, 4.2 TB/s; 16 single fp32 tokens with 12/2 heads 3.5 us.
+// 11,247 tokens with 32/8 heads of 128 take 46 us in bf16 (254 MB, 5.5 TB/s; 59 while the rows were held as fp32 and fewer
+// CTAs had room) and 122 us in fp32 (483 MB); 16 single fp32 tokens with 12/2 heads 3.6 us.
 constexpr int APPEND_WARPS = 4;
 
 struct AppendArgs {
@@ -30,64 +31,65 @@ struct AppendArgs {
     int q_heads, rope_rows;
     const float *rope;                                     // [rope_rows][D / 2 cos | D / 2 sin], null: no rotation
     int32_t *status;
-    bool vec;                                              // every row starts on 8 bytes
+    bool vec;                                              // every row starts on a multiple of four elements
 };
 
 // A lane's elements of a row: H consecutive ones of the first half and their rotation partners, D / 2 further on, so that a
 // pair is in one lane
-template <typename T, int D>
+template <int D>
 struct Piece {
-    static constexpr int H = 8 / sizeof(T), LR = D / 2 / H;   // 8 bytes of each half; lanes of a row
+    static constexpr int H = 4, LR = D / 2 / H;   // elements of each half; lanes of a row
     float x[2][H];
-    __device__ __forceinline__ void zero() {
-#pragma unroll
-        for (int i = 0; i < H; ++i) x[0][i] = x[1][i] = 0.f;
-    }
-    template <bool VEC>
-    __device__ __forceinline__ void load(const T *p) {   // p: the lane's first element
-        T e[2][H];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            if constexpr (VEC) *reinterpret_cast<uint2 *>(e[k]) = ldg_stream8(p + k * (D / 2));
-            else
-#pragma unroll
-                for (int i = 0; i < H; ++i) e[k][i] = p[k * (D / 2) + i];
-#pragma unroll
-            for (int i = 0; i < H; ++i) {
-                if constexpr (std::is_same<T, float>::value) x[k][i] = e[k][i];
-                else if constexpr (std::is_same<T, __half>::value) x[k][i] = __half2float(e[k][i]);
-                else x[k][i] = __bfloat162float(e[k][i]);
-            }
-        }
-    }
-    __device__ __forceinline__ void store(T *p) const {
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            uint2 r;
-            T *e = reinterpret_cast<T *>(&r);
-            if constexpr (std::is_same<T, float>::value)
-#pragma unroll
-                for (int i = 0; i < H; ++i) e[i] = x[k][i];
-            else kv_store4(e, make_float4(x[k][0], x[k][1], x[k][2], x[k][3]));
-            *reinterpret_cast<uint2 *>(p + k * (D / 2)) = r;
-        }
-    }
     // x1 c - x2 s; x2 c + x1 s, every product and sum rounded by itself
     __device__ __forceinline__ void rotate(const float *cs, int l) {
         float c[H], s[H];
-        if constexpr (H == 4) {
-            *reinterpret_cast<float4 *>(c) = *reinterpret_cast<const float4 *>(cs + 4 * l);
-            *reinterpret_cast<float4 *>(s) = *reinterpret_cast<const float4 *>(cs + D / 2 + 4 * l);
-        } else {
-            *reinterpret_cast<float2 *>(c) = *reinterpret_cast<const float2 *>(cs + 2 * l);
-            *reinterpret_cast<float2 *>(s) = *reinterpret_cast<const float2 *>(cs + D / 2 + 2 * l);
-        }
+        *reinterpret_cast<float4 *>(c) = *reinterpret_cast<const float4 *>(cs + H * l);
+        *reinterpret_cast<float4 *>(s) = *reinterpret_cast<const float4 *>(cs + D / 2 + H * l);
 #pragma unroll
         for (int i = 0; i < H; ++i) {
             const float a = x[0][i], b = x[1][i];
             x[0][i] = __fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, s[i]));
             x[1][i] = __fadd_rn(__fmul_rn(b, c[i]), __fmul_rn(a, s[i]));
         }
+    }
+};
+
+// The same elements as they came: for 16-bit types half the registers, so that more warps have their loads in flight
+template <typename T, int D>
+struct alignas(16) Raw {
+    typedef Piece<D> P;
+    T e[2][P::H];
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < 2 * P::H; ++i) e[i / P::H][i % P::H] = (T)0.f;
+    }
+    template <bool VEC>
+    __device__ __forceinline__ void load(const T *p) {   // p: the lane's first element
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            if constexpr (!VEC)
+#pragma unroll
+                for (int i = 0; i < P::H; ++i) e[k][i] = p[k * (D / 2) + i];
+            else if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(e[k]) = ldg_stream16(p + k * (D / 2));
+            else *reinterpret_cast<uint2 *>(e[k]) = ldg_stream8(p + k * (D / 2));
+        }
+    }
+    __device__ __forceinline__ P values() const {
+        P r;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < P::H; ++i) {
+                if constexpr (std::is_same<T, float>::value) r.x[k][i] = e[k][i];
+                else if constexpr (std::is_same<T, __half>::value) r.x[k][i] = __half2float(e[k][i]);
+                else r.x[k][i] = __bfloat162float(e[k][i]);
+            }
+        return r;
+    }
+    // keeps the compiler from carrying what it computed from 16-bit elements past this point
+    __device__ __forceinline__ void forget() {
+        uint32_t *w = reinterpret_cast<uint32_t *>(e);
+        asm volatile("" : "+r"(w[0]), "+r"(w[1]), "+r"(w[2]), "+r"(w[3]));
     }
 };
 
@@ -109,11 +111,12 @@ __device__ __forceinline__ uint32_t moved_code(uint32_t c, float ratio) {
 template <typename T, int D, bool VEC>
 __device__ __forceinline__ void append_rows(const T *src, int64_t tok_ld, const float *cs, bool turn, int s0, int s1,
                                             uint8_t *codes, float *scale, int lane) {
-    typedef Piece<T, D> P;
+    typedef Piece<D> P;
     constexpr int H = P::H, RP = 32 / P::LR, NP = KV_BLOCK / RP;   // rows of a pass, passes
     const int l = lane % P::LR, sub = lane / P::LR;
     const float s_old = s0 > 0 ? *scale : 0.f;
-    P x[NP];
+    constexpr bool AGAIN = sizeof(T) == 2;                         // rotated for the magnitude and again for the codes
+    Raw<T, D> x[NP];
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
         const int r = s0 + i * RP + sub;
@@ -125,9 +128,14 @@ __device__ __forceinline__ void append_rows(const T *src, int64_t tok_ld, const 
     for (int i = 0; i < NP; ++i) {
         const int r = s0 + i * RP + sub;
         if (s0 + i * RP >= s1) break;   // uniform over the warp
-        if (turn && r < s1) x[i].rotate(cs + (r - s0) * D, l);
+        P y = x[i].values();
+        if (turn && r < s1) y.rotate(cs + (r - s0) * D, l);
 #pragma unroll
-        for (int k = 0; k < H; ++k) top = max_nan(max_nan(top, fabsf(x[i].x[0][k])), fabsf(x[i].x[1][k]));
+        for (int k = 0; k < H; ++k) top = max_nan(max_nan(top, fabsf(y.x[0][k])), fabsf(y.x[1][k]));
+        if constexpr (AGAIN) x[i].forget();
+        else
+#pragma unroll
+            for (int k = 0; k < 2 * H; ++k) x[i].e[k / H][k % H] = y.x[k / H][k % H];
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -149,17 +157,15 @@ __device__ __forceinline__ void append_rows(const T *src, int64_t tok_ld, const 
     for (int i = 0; i < NP; ++i) {
         const int r = s0 + i * RP + sub;
         if (r < s1) {
+            P all = x[i].values();
+            if (AGAIN && turn) all.rotate(cs + (r - s0) * D, l);
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const float *y = x[i].x[k];
+                const float *y = all.x[k];
                 uint8_t *p = codes + r * D + k * (D / 2) + H * l;
                 const uint32_t lo = pack_bytes(code_bits(y[0], inv), code_bits(y[1], inv));
-                if constexpr (H == 4) {
-                    const uint32_t hi = pack_bytes(code_bits(y[2], inv), code_bits(y[3], inv));
-                    *reinterpret_cast<uint32_t *>(p) = bad ? 0x80808080u : __byte_perm(lo, hi, 0x5410u);
-                } else {
-                    *reinterpret_cast<uint16_t *>(p) = bad ? 0x8080u : (uint16_t)lo;
-                }
+                const uint32_t hi = pack_bytes(code_bits(y[2], inv), code_bits(y[3], inv));
+                *reinterpret_cast<uint32_t *>(p) = bad ? 0x80808080u : __byte_perm(lo, hi, 0x5410u);
             }
         }
     }
@@ -171,10 +177,10 @@ __device__ __forceinline__ void append_rows(const T *src, int64_t tok_ld, const 
 template <typename T, int D, bool VEC>
 __device__ __forceinline__ void turn_rows(const T *src, int64_t tok_ld, const float *cs, bool turn, int rows, int placed, T *out,
                                           int64_t out_ld, int lane) {
-    typedef Piece<T, D> P;
+    typedef Piece<D> P;
     constexpr int RP = 32 / P::LR, NP = KV_BLOCK / RP;
     const int l = lane % P::LR, sub = lane / P::LR;
-    P x[NP];
+    Raw<T, D> x[NP];
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
         x[i].zero();
@@ -183,13 +189,20 @@ __device__ __forceinline__ void turn_rows(const T *src, int64_t tok_ld, const fl
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
         const int r = i * RP + sub;
-        if (turn && r < placed) x[i].rotate(cs + r * D, l);
-        if (r < rows) x[i].store(out + r * out_ld + P::H * l);
+        P y = x[i].values();
+        if (turn && r < placed) y.rotate(cs + r * D, l);
+        if (r < rows)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                kv_store4(out + r * out_ld + k * (D / 2) + P::H * l, make_float4(y.x[k][0], y.x[k][1], y.x[k][2], y.x[k][3]));
     }
 }
 
+// CTAs of an SM: what the rows in flight leave registers for
 template <typename T, int D, bool VEC>
-__global__ void __launch_bounds__(32 * APPEND_WARPS, 5) k_kv_append(const __grid_constant__ AppendArgs a) {
+constexpr int append_ctas() { return D * sizeof(T) >= 512 ? (VEC ? 5 : 4) : (VEC ? 7 : 5); }
+template <typename T, int D, bool VEC>
+__global__ void __launch_bounds__(32 * APPEND_WARPS, append_ctas<T, D, VEC>()) k_kv_append(const __grid_constant__ AppendArgs a) {
     __shared__ __align__(16) float cs[KV_BLOCK * D];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int64_t base;
@@ -232,9 +245,10 @@ __global__ void __launch_bounds__(32 * APPEND_WARPS, 5) k_kv_append(const __grid
 
 // --------------------------------------------------------------------------------------------------------- read
 // Values of tokens [first[b], kv_len[b]) of every sequence, of `layers` layers: row row_start[b] + i is token
-// first[b] + i.  A thread takes eight dims of one row of one head, U layers in flight; rows without a page read as zero.
-// Bytes: D codes in, D values out per row and head; 192 rows of 63 tokens, 28 layers, 2 heads of 128 to bf16 (174 MB in, 347 MB
-// out) take 87 us, 6.0 TB/s.
+// first[b] + i.  A thread takes sixteen dims of one row of one head, so that finding the row weighs half as much, U layers in
+// flight; rows without a page read as zero.  HBM bounds it, D codes in and D values out per row and head: 192 rows of 63 tokens,
+// 28 layers, 2 heads of 128 to bf16 (174 MB in, 347 MB out) take 86 us, 6.1 TB/s; 11,247 tokens, one layer, 8 heads (69 MB)
+// 11.4 us (17.2 with eight dims, 64-bit divisions and integer conversions).
 struct ReadArgs {
     KvView c;                     // layer 0 of the call; q_start holds row_start, n_tokens the rows
     const int32_t *first;
@@ -244,36 +258,40 @@ struct ReadArgs {
 };
 
 __device__ __forceinline__ void read8(uint2 w, float s, float4 &lo, float4 &hi) {
-    auto f = [&](uint32_t u, int i) { return __fmul_rn((float)((int)((u >> (8 * i)) & 255u) - 128), s); };
+    // 2^23 + code as a float, less 2^23 + 128: exact
+    auto f = [&](uint32_t u, int i) { return __fmul_rn(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440 + i)) - 8388736.f, s); };
     lo = make_float4(f(w.x, 0), f(w.x, 1), f(w.x, 2), f(w.x, 3));
     hi = make_float4(f(w.y, 0), f(w.y, 1), f(w.y, 2), f(w.y, 3));
 }
 
+// A thread takes two pieces of 8 values of a row, D / 2 apart, in U layers at a time
 template <typename T, int D, int U>
 __global__ void __launch_bounds__(256) k_kv_read(const __grid_constant__ ReadArgs a) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t row = i / (a.c.heads * (D / 8));
+    constexpr int P = 2, LR = D / 8 / P;   // lanes of a row
+    const uint32_t pair = blockIdx.x * (256 / LR) + threadIdx.x / LR, row = pair / a.c.heads;
     if (row >= a.c.n_tokens) return;
-    const int rest = (int)(i - row * (a.c.heads * (D / 8))), h = rest / (D / 8), d = rest % (D / 8) * 8;
+    const int h = (int)(pair - row * a.c.heads), d = threadIdx.x % LR * 8;
     int64_t base;
     const int b = kv_find(a.c.q_start, a.c.batch, a.c.n_tokens, 1, 1, 0, row, base);
-    const int pos = a.first[b] + (int)(row - base);
-    const bool in = base <= row && row < a.c.q_start[b + 1] && pos >= 0 && pos < a.c.len(b);
+    const int pos = a.first[b] + (int)((int64_t)row - base);
+    const bool in = base <= row && (int64_t)row < a.c.q_start[b + 1] && pos >= 0 && pos < a.c.len(b);
     const int page = in ? a.c.page_of(b, pos) : -1;
     const int64_t at = page >= 0 ? a.c.block(page, h, pos) : 0;
-    const int64_t src = (at * KV_BLOCK + (pos & 15)) * D + d, dst = (row * a.c.heads + h) * D + d, layer_out = (int64_t)a.c.n_tokens * a.c.heads * D;
+    const int64_t src = (at * KV_BLOCK + (pos & 15)) * D + d, dst = ((int64_t)row * a.c.heads + h) * D + d, layer_out = (int64_t)a.c.n_tokens * a.c.heads * D;
     for (int l0 = blockIdx.y; l0 < a.layers; l0 += U * gridDim.y) {
-        uint2 w[U][2];
+        uint2 w[U][2][P];
         float s[U][2];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int l = l0 + u * gridDim.y;
 #pragma unroll
             for (int kind = 0; kind < 2; ++kind) {
-                w[u][kind] = make_uint2(0x80808080u, 0x80808080u);
+#pragma unroll
+                for (int k = 0; k < P; ++k) w[u][kind][k] = make_uint2(0x80808080u, 0x80808080u);
                 s[u][kind] = 0.f;
                 if (page >= 0 && l < a.layers) {
-                    w[u][kind] = ldg_stream8((kind ? a.c.v : a.c.k) + l * a.layer_codes + src);
+#pragma unroll
+                    for (int k = 0; k < P; ++k) w[u][kind][k] = ldg_stream8((kind ? a.c.v : a.c.k) + l * a.layer_codes + src + k * (D / P));
                     s[u][kind] = (kind ? a.c.vs : a.c.ks)[l * a.layer_scales + at];
                 }
             }
@@ -283,20 +301,22 @@ __global__ void __launch_bounds__(256) k_kv_read(const __grid_constant__ ReadArg
             const int l = l0 + u * gridDim.y;
             if (l < a.layers)
 #pragma unroll
-                for (int kind = 0; kind < 2; ++kind) {
-                    float4 lo, hi;
-                    read8(w[u][kind], s[u][kind], lo, hi);
-                    T *out = static_cast<T *>(kind ? a.v : a.k) + l * layer_out + dst;
-                    if constexpr (sizeof(T) == 2) {
-                        uint4 r;
-                        kv_store4(reinterpret_cast<T *>(&r), lo);
-                        kv_store4(reinterpret_cast<T *>(&r) + 4, hi);
-                        __stcs(reinterpret_cast<uint4 *>(out), r);
-                    } else {
-                        kv_store4(out, lo);
-                        kv_store4(out + 4, hi);
+                for (int kind = 0; kind < 2; ++kind)
+#pragma unroll
+                    for (int k = 0; k < P; ++k) {
+                        float4 lo, hi;
+                        read8(w[u][kind][k], s[u][kind], lo, hi);
+                        T *out = static_cast<T *>(kind ? a.v : a.k) + l * layer_out + dst + k * (D / P);
+                        if constexpr (sizeof(T) == 2) {
+                            uint4 r;
+                            kv_store4(reinterpret_cast<T *>(&r), lo);
+                            kv_store4(reinterpret_cast<T *>(&r) + 4, hi);
+                            __stcs(reinterpret_cast<uint4 *>(out), r);
+                        } else {
+                            kv_store4(out, lo);
+                            kv_store4(out + 4, hi);
+                        }
                     }
-                }
         }
     }
 }
@@ -431,10 +451,9 @@ static int launched(const char *who) {
 
 static size_t dtype_bytes(int t) { return t == V3G_F32 ? 4 : 2; }
 
-// 8-byte loads of rows: the base and both strides keep that alignment
+// loads of four elements: the base and both strides keep that alignment
 static bool rows_vec(const v3g_rows_t &r, int dtype) {
-    const int64_t n = 8 / (int64_t)dtype_bytes(dtype);
-    return aligned_to(r.data, 8) && r.tok_stride % n == 0 && r.head_stride % n == 0;
+    return aligned_to(r.data, 4 * dtype_bytes(dtype)) && r.tok_stride % 4 == 0 && r.head_stride % 4 == 0;
 }
 
 template <typename T>
@@ -450,13 +469,12 @@ static void launch_append(const AppendArgs &a, int D, dim3 grid, cudaStream_t st
 
 template <typename T>
 static void launch_read(const ReadArgs &a, int D, dim3 grid, cudaStream_t st) {
-    // a thread with one layer keeps few registers
     if ((int)grid.y >= a.layers) {
         if (D == 64) k_kv_read<T, 64, 1><<<grid, 256, 0, st>>>(a);
         else k_kv_read<T, 128, 1><<<grid, 256, 0, st>>>(a);
     } else {
-        if (D == 64) k_kv_read<T, 64, 4><<<grid, 256, 0, st>>>(a);
-        else k_kv_read<T, 128, 4><<<grid, 256, 0, st>>>(a);
+        if (D == 64) k_kv_read<T, 64, 2><<<grid, 256, 0, st>>>(a);
+        else k_kv_read<T, 128, 2><<<grid, 256, 0, st>>>(a);
     }
 }
 
@@ -504,9 +522,10 @@ extern "C" int v3g_kv_append(const v3g_kv_cache_t *cache, uint32_t layer, const 
     a.status = dev_status;
     const uint32_t items = batch->n_tokens / KV_BLOCK + 2 * batch->batch;
     // A block's heads are shared out over CTAs while the blocks are few (8 sequences of up to 200 tokens, 32/8 heads: one CTA a
-    // block 15.5 us, shared out 10.0 us); past one pass of the warps over the heads there is nothing left to share.
+    // block 15.5 us, shared out 10.0 us), and further so that the last round of CTAs is a small part of all (11,247 bf16 tokens: 32
+    // CTAs an SM in all 46.5 us, 8 of them 56.4); past one pass of the warps over the heads there is nothing left to share.
     const uint32_t passes = (2 * cache->n_kv_heads + (q ? n_q_heads : 0) + APPEND_WARPS - 1) / APPEND_WARPS;
-    uint32_t ny = (148 * 8 + items - 1) / items;
+    uint32_t ny = (148 * 32 + items - 1) / items;
     ny = ny > passes ? passes : ny;
     const dim3 grid(items, ny);
     const cudaStream_t st = (cudaStream_t)stream;
@@ -534,11 +553,11 @@ extern "C" int v3g_kv_read(const v3g_kv_cache_t *cache, uint32_t layer, uint32_t
     a.layers = (int)n_layers;
     a.k = k_out;
     a.v = v_out;
-    const int64_t threads = (int64_t)batch->n_tokens * cache->n_kv_heads * (cache->head_dim / 8);
-    const int64_t gx = (threads + 255) / 256;
-    if (gx > 0x7FFFFFFF) return v3g_fail(V3G_E_LIMIT, "v3g_kv_read: too many values");
+    const int64_t rows = (int64_t)batch->n_tokens * cache->n_kv_heads;
+    if (rows > 0x7FFFFFFF) return v3g_fail(V3G_E_LIMIT, "v3g_kv_read: too many values");
     // a thread that takes several layers looks its page up once; few rows spread their layers over the GPU
-    int64_t gy = 8192 / gx;
+    const int64_t gx = (rows * (cache->head_dim / 16) + 255) / 256;
+    int64_t gy = 4096 / gx;
     gy = gy < 1 ? 1 : (gy > n_layers ? n_layers : gy);
     const dim3 grid((uint32_t)gx, (uint32_t)gy);
     const cudaStream_t st = (cudaStream_t)stream;
