@@ -201,6 +201,34 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
     const int per = (all + shares - 1) / shares, jlo = min(share * per, all), nk = min(per, all - jlo);
     auto key0 = [&](int j) { return (j + jlo < sb ? j + jlo : j + jlo - sb + ws) * PF_KEYS; };
 
+    // The softmax warps' 32 query rows each, LPR lanes to a row so that reads are whole lines, on their way while the barriers
+    // are set up
+    constexpr int LPR = D / 8, RPI = 32 / LPR;
+    const int row_w = 32 * warp, pc = lane % LPR, pr = lane / LPR;   // the warp's first row; this lane's piece, its row in a pass
+    uint4 xq[LPR];
+    // f(pass, row, its token, its head in the group), for this lane's rows
+    auto rows_of = [&](auto f) {
+        const int dt = RPI / a.group, dg = RPI - dt * a.group;
+        int tk = (r0 + row_w + pr) / a.group, g = r0 + row_w + pr - tk * a.group;
+#pragma unroll
+        for (int i = 0; i < LPR; ++i) {
+            f(i, row_w + i * RPI + pr, tk, g);
+            tk += dt, g += dg;
+            if (g >= a.group) ++tk, g -= a.group;
+        }
+    };
+    if (warp < 8)
+        rows_of([&](int i, int rr, int tk, int g) {
+            xq[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (rr < rn) {
+                const T *src = static_cast<const T *>(a.q) + (int64_t)(first + tk) * a.q_tok + (int64_t)(h * a.group + g) * a.q_head + 8 * pc;
+                if (a.q_vec8) xq[i] = ldg_stream16(src);
+                else
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) reinterpret_cast<T *>(&xq[i])[e] = src[e];
+            }
+        });
+
     const uint32_t bars = tc::smem_addr(smem + SM::BAR);
     // barrier slots
     auto QFULL = bars;
@@ -253,33 +281,16 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
         const int qh = h * a.group + r - tok * a.group;
         const uint32_t lane_tm = tmem + ((uint32_t)(32 * (warp & 3)) << 16), tS = lane_tm + 128u * tile, tO = lane_tm + 256u + 128u * tile;
         if (tile < tiles) {
-            // The warp's 32 query rows, LPR lanes to a row so that reads are whole lines: a power of two brings a row into fp16 (the
-            // sign of the scale with it), in 128-byte swizzled halves
-            constexpr int LPR = D / 8, RPI = 32 / LPR;
-            const int row_w = 128 * tile + 32 * (warp & 3);   // the warp's first row in the CTA
-            const int pc = lane % LPR, pr = lane / LPR;       // this lane's piece, and its row in a pass
+            // a power of two brings a row into fp16 (the sign of the scale with it), in 128-byte swizzled halves
             float *qfac = reinterpret_cast<float *>(smem + SM::QF);
             uint8_t *piece = smem + SM::Q + tile * SM::OP + (pc >> 3) * 16384;   // rows of 128 bytes, piece pc & 7
             {
-                uint4 x[LPR];
-#pragma unroll
-                for (int i = 0; i < LPR; ++i) {
-                    const int rr = row_w + i * RPI + pr, tk = (r0 + rr) / a.group, hd = h * a.group + r0 + rr - tk * a.group;
-                    x[i] = make_uint4(0u, 0u, 0u, 0u);
-                    if (rr < rn) {
-                        const T *src = static_cast<const T *>(a.q) + (int64_t)(first + tk) * a.q_tok + (int64_t)hd * a.q_head + 8 * pc;
-                        if (a.q_vec8) x[i] = ldg_stream16(src);
-                        else
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) reinterpret_cast<T *>(&x[i])[e] = src[e];
-                    }
-                }
 #pragma unroll
                 for (int i = 0; i < LPR; ++i) {
                     float y[8], top = 0.f;
 #pragma unroll
                     for (int e = 0; e < 8; e += 4) {
-                        const float4 v = kv_load4<T>(reinterpret_cast<const T *>(&x[i]) + e, true);
+                        const float4 v = kv_load4<T>(reinterpret_cast<const T *>(&xq[i]) + e, true);
                         y[e] = v.x, y[e + 1] = v.y, y[e + 2] = v.z, y[e + 3] = v.w;
                         top = fmaxf(fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
                     }
@@ -461,14 +472,12 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
                     }
                 }
                 __syncwarp();
-#pragma unroll 4
-                for (int i = 0; i < LPR; ++i) {
-                    const int rl = 32 * (warp & 3) + i * RPI + pr, rr = 128 * tile + rl, tk = (r0 + rr) / a.group;
+                rows_of([&](int, int rr, int tk, int g) {
+                    const int rl = rr & 127;
                     if (rr < rn)
-                        *reinterpret_cast<uint4 *>(static_cast<T *>(a.out) +
-                                                   ((int64_t)(first + tk) * a.c.heads * a.group + h * a.group + r0 + rr - tk * a.group) * D + 8 * pc) =
+                        *reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + ((int64_t)(first + tk) * a.c.heads * a.group + h * a.group + g) * D + 8 * pc) =
                             *reinterpret_cast<const uint4 *>(piece + rl * 128 + (((pc & 7) ^ (rl & 7)) << 4));
-                }
+                });
             }
             if (live && ok) {
                 if (shares > 1) a.part_ml[part] = make_float2(m, l);
