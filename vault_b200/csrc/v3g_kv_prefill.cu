@@ -16,13 +16,18 @@
 // O += P' V.  A tile's issuer runs PV(u), QK(u + 2): while these run, the tile's softmax works on the other buffer, so neither
 // waits for a round trip.  tcgen05 operations of one thread run in order, so QK(u + 2) may overwrite P'(u).  Each tile has
 // an issuer in another quarter of the SM, because an issuing warp slows the softmax warps of its quarter (one issuer for
-// both tiles: 718 us for the 8,192-token prompt, 32/8 heads; two: 693).  The offset m of a row's exponents is its maximum when m was set, plus 3; it stays until a score passes it
-// by 11 (P' is then below 2^15).  Only then the warp rescales its O in tensor memory, after a wait for PV(u - 1): with a
-// margin of 8 from the maximum itself, some row of the 32 did so at every second step on scores of standard deviation 3.
+// both tiles: 718 us for the 8,192-token prompt, 32/8 heads; two: 693).  The offset m of a row's exponents is its maximum
+// when m was set, plus 3; it stays until a score passes it by 11 (P' is then below 2^15).  Only then the warp rescales its O
+// in tensor memory, after a wait for PV(u - 1): with a margin of 8 from the maximum itself, some row of the 32 did so at every
+// second step on scores of standard deviation 3.
 //
 // K scales multiply the scores; a V scale vs enters the exponent, P' = 2^(s - m + log2(vs / ref)), ref a power of two
-// that follows the largest vs (the same for the whole CTA), and the row sum takes P' ref / vs.  vs / ref is held at or above 2^-40, where P' rounds to
-// zero in fp16 whatever p is: a block with scale 0 adds nothing to O and its full weight to the sum.
+// that follows the largest vs (the same for the whole CTA), and the row sum takes P' ref / vs.  vs / ref is held at or above
+// 2^-40, where P' rounds to zero in fp16 whatever p is: a block with scale 0 adds nothing to O and its full weight to the sum.
+//
+// 8,192 tokens, 32/8 heads of 128, every earlier key: 591 us, 930 TFLOP/s (517 us in a burst, before the clock falls); 4,608
+// tokens under a window of 1,024, 12/2 heads: 67 us, of which each of the two rounds of CTAs spends a quarter on its start and
+// end.
 #include <atomic>
 #include <cfloat>
 
