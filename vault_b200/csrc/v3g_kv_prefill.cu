@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
             }
             const float qf = qfac[128 * tile + row];
             const int p = live ? p0 + tok : -1;
-            float m = -INFINITY, l = 0.f;
+            float m = -INFINITY, l = 0.f, lr = 0.f;   // lr: the sum as the rounded P' have it (fp16 outputs)
             // Warps w of the two tiles share a quarter of the SM and its exponential unit, so they take turns at it (named
             // barriers 1 + w and 5 + w, equal step counts): together they took 1,250 clocks for 64 keys each, in turn 750.
             bool had_turn = false, gave_turn = false;
@@ -380,6 +380,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
                     const float f = pf_ex2(m - (mx + 3.f));
                     m = mx + 3.f;
                     l *= f;
+                    lr *= f;
                     al *= f;
                     change = true;
                 }
@@ -417,6 +418,22 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
                         }
                         float sum, odd;
                         f2_unpack(sum2, sum, odd);
+                        // fp16 outputs show what P' loses when it is rounded, so they are divided by the sum of the rounded P', whose
+                        // error is in part the same (one key that outweighs the others: all of it).  Not where vs / ref is small: there
+                        // P' may be 0.
+                        if constexpr (std::is_same<T, __half>::value) {
+                            float s0 = sum, s1 = odd;
+                            if (wv[i] >= -4.f) {
+                                s0 = s1 = 0.f;
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) {
+                                    const float2 r = __half22float2(*reinterpret_cast<const __half2 *>(&pk[8 * h2 + e]));
+                                    s0 += r.x;
+                                    s1 += r.y;
+                                }
+                            }
+                            lr = fmaf(s0 + s1, iw[i], lr);
+                        }
                         l = fmaf(sum + odd, iw[i], l);
                     }
                     tmem_st16(tS + 64 * half + 16 * c, pk);
@@ -442,7 +459,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
                 ok = pf_wait(OFULL(tile), 0);
                 tc::tc_fence_after();
                 inv = places[(nk - 1) & (PF_RING - 1)].ref;
-                if (shares == 1) inv = l == 0.f ? 0.f : inv / l;
+                if constexpr (std::is_same<T, __half>::value) inv = lr == 0.f ? 0.f : (shares == 1 ? inv / lr : inv * (l / lr));
+                else if (shares == 1) inv = l == 0.f ? 0.f : inv / l;
             }
             const int64_t part = out_row * a.part_stride + share;
             if (ok && shares > 1 && nk > 0) {   // (an empty share has no accumulator)
