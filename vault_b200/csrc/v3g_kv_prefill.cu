@@ -397,10 +397,12 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
                     }
                 }
                 const float mu = m == -INFINITY ? 0.f : m;
+                uint32_t pa[32];
+                float exact[4];
                 my_turn();
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    uint32_t pk[16];
+                    uint32_t *pk = pa + 16 * c;
 #pragma unroll
                     for (int h2 = 0; h2 < 2; ++h2) {
                         const int i = 2 * c + h2;
@@ -418,22 +420,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
                         }
                         float sum, odd;
                         f2_unpack(sum2, sum, odd);
-                        // fp16 outputs show what P' loses when it is rounded, so they are divided by the sum of the rounded P', whose
-                        // error is in part the same (one key that outweighs the others: all of it).  Not where vs / ref is small: there
-                        // P' may be 0.
-                        if constexpr (std::is_same<T, __half>::value) {
-                            float s0 = sum, s1 = odd;
-                            if (wv[i] >= -4.f) {
-                                s0 = s1 = 0.f;
-#pragma unroll
-                                for (int e = 0; e < 8; ++e) {
-                                    const float2 r = __half22float2(*reinterpret_cast<const __half2 *>(&pk[8 * h2 + e]));
-                                    s0 += r.x;
-                                    s1 += r.y;
-                                }
-                            }
-                            lr = fmaf(s0 + s1, iw[i], lr);
-                        }
+                        if constexpr (std::is_same<T, __half>::value) exact[i] = sum + odd;
                         l = fmaf(sum + odd, iw[i], l);
                     }
                     tmem_st16(tS + 64 * half + 16 * c, pk);
@@ -443,6 +430,24 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
                 tc::tc_fence_before();
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(PFULL(tile, half));
+                // fp16 outputs show what P' loses when it is rounded, so they are divided by the sum of the rounded P', whose error is
+                // in part the same (one key that outweighs the others: all of it).  Not where vs / ref is small: there P' may be 0.
+                if constexpr (std::is_same<T, __half>::value) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float s0 = exact[i], s1 = 0.f;
+                        if (wv[i] >= -4.f) {
+                            uint64_t r2 = 0;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const float2 r = __half22float2(*reinterpret_cast<const __half2 *>(&pa[8 * i + e]));
+                                r2 = f2_add(r2, f2_pack(r.x, r.y));
+                            }
+                            f2_unpack(r2, s0, s1);
+                        }
+                        lr = fmaf(s0 + s1, iw[i], lr);
+                    }
+                }
             };
             if (tile == 1) turn(1 + (warp & 3), false);
             for (int u = 0; u < 2 * nk; ++u) {
