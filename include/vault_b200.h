@@ -318,7 +318,8 @@ V3G_API int v3g_kv_read(const v3g_kv_cache_t *cache, uint32_t layer, uint32_t n_
  * count and length of a sequence as far as the host knows them (0: unknown): they choose kernels and splits, never
  * results' validity.  *dev_status (may be NULL) gets V3G_STATUS_TIMEOUT if a bounded wait inside a kernel ran out (the
  * output is then invalid).  dev_work: v3g_kv_attention_work_size bytes of device memory, 256-byte aligned, with no content
- * kept between calls. */
+ * kept between calls.  A call queues several kernels: threads that share a workspace queue their calls one after the
+ * other (under a lock), on one stream. */
 V3G_API size_t v3g_kv_attention_work_size(const v3g_kv_cache_t *cache, const v3g_kv_batch_t *batch, uint32_t n_q_heads,
                                           uint32_t max_q, uint32_t max_kv, uint32_t window, uint32_t n_sink);
 V3G_API int v3g_kv_attention(const v3g_kv_cache_t *cache, uint32_t layer, const v3g_kv_batch_t *batch, int dtype, const v3g_rows_t *q,
@@ -340,7 +341,7 @@ V3G_API int v3g_kv_reorder(const v3g_kv_cache_t *cache, const v3g_kv_batch_t *ba
  * continuation: eos_id at its own score.  Continuations scored NaN or -inf are never chosen; slots left over get token
  * eos_id (0 when eos_id < 0), parent = their own beam, score -inf and count as finished.  NaN logits are skipped.
  * Outputs [groups][beams]; finished_out: the parent's flag, or token == eos_id.  dev_work:
- * v3g_beam_select_work_size bytes, 256-byte aligned. */
+ * v3g_beam_select_work_size bytes, 256-byte aligned, shared between threads as v3g_kv_attention's may be. */
 V3G_API size_t v3g_beam_select_work_size(uint32_t groups, uint32_t beams, uint32_t vocab);
 V3G_API int v3g_beam_select(const void *dev_logits, int dtype, uint32_t groups, uint32_t beams, uint32_t vocab, uint64_t ld,
                             const float *dev_scores, const uint8_t *dev_finished, int32_t eos_id, int32_t *tokens, int32_t *parents,

@@ -18,6 +18,7 @@ host; all device work is the C ABI's (include/vault_b200.h).  No result depends 
 from __future__ import annotations
 
 import ctypes as C
+import threading
 from typing import Optional, Tuple
 
 import torch
@@ -53,11 +54,14 @@ _capturing = torch._C._cuda_isCurrentStreamCapturing
 
 
 class _Workspaces:
-    """Device workspaces, one for each stream that has used them: a stream runs its calls in order, so they can share one.
-    They grow and are kept until their owner goes.  A captured call has one of its own, in the graph's memory."""
+    """Device workspaces, one for each stream that has used them: a stream runs its kernels in order, so its calls can share
+    one.  A call queues several kernels that hand their results on in it and lets other Python threads run meanwhile, so it
+    is queued under a lock: no other thread's kernels come between its own.  Workspaces grow and are kept until their owner
+    goes.  A captured call has one of its own, in the graph's memory."""
 
     def __init__(self):
         self.by_stream = {}
+        self.lock = threading.RLock()   # a finalizer that runs inside may make a call of its own
 
     def run(self, device, size, call) -> int:
         """call(workspace, its bytes, stream) on torch's current stream of `device`, which becomes the current device for
@@ -71,14 +75,15 @@ class _Workspaces:
         if _capturing():
             t = torch.empty(size(), dtype=torch.uint8, device=device)
             return call(t.data_ptr(), t.numel(), stream)
-        held = self.by_stream.get((index, stream))
-        if held is not None:
-            rc = call(held[0], held[1], stream)
-            if rc != _lib.V3G_E_SIZE:
-                return rc
-        t = torch.empty(max(size(), 1 << 16), dtype=torch.uint8, device=device)
-        self.by_stream[(index, stream)] = (t.data_ptr(), t.numel(), t)
-        return call(t.data_ptr(), t.numel(), stream)
+        with self.lock:
+            held = self.by_stream.get((index, stream))
+            if held is not None:
+                rc = call(held[0], held[1], stream)
+                if rc != _lib.V3G_E_SIZE:
+                    return rc
+            t = torch.empty(max(size(), 1 << 16), dtype=torch.uint8, device=device)
+            self.by_stream[(index, stream)] = (t.data_ptr(), t.numel(), t)
+            return call(t.data_ptr(), t.numel(), stream)
 
 
 _beam_work = _Workspaces()
