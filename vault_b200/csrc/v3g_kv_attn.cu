@@ -449,8 +449,9 @@ __global__ void __launch_bounds__(128) k_kv_join(const __grid_constant__ KvAttnA
         const int n = a.c.tokens(b, first);
         if (tok >= first && tok < first + n) shares = n * a.group > a.max_rows ? a.pf_splits : a.splits;
     }
-    if (WR == 4 && shares <= 1) return;            // no sequence's row, or a finished one
+    // Every CTA waits, one without work too: this grid's end stands for the end of the kernels before it.
     griddep_wait();
+    if (WR == 4 && shares <= 1) return;            // no sequence's row, or a finished one
     const float2 *ml = a.part_ml + row * a.part_stride;
     float mx = -INFINITY, ls = 0.f, o[W];
 #pragma unroll
