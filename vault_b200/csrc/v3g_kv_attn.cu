@@ -12,10 +12,12 @@
 //   the head dims are taken in that order (the contraction does not care), so no shared memory is used.  Codes become
 //   fp16 integers exactly (byte permute to 1024 + c, minus 1152).  fp16 queries enter as they are, bf16 queries as fp16
 //   after an exact power of two per row that puts the largest magnitude in [2^13, 2^14).
-// * The K scale of the block multiplies the scores, the V scale the probabilities: P' = p vs / ref with ref a power of
-//   two that follows the largest V scale seen, so P' keeps fp16's 11 bits whatever the scales are; for fp16 outputs it
-//   enters as two fp16 parts, since the rounding of one would be as large as that of the output itself.  Sums, maxima
-//   and the accumulators are fp32.  The maximum is raised only when a score exceeds it by 8 (P' then stays below 2^12).
+// * The K scale of the block multiplies the scores, the V scale enters the exponent of the operand: P' = 2^(s + log2 vs - M)
+//   with an offset M of the row's own, which follows the largest of its terms p vs as m follows its largest score.  So P'
+//   keeps fp16's 11 bits whatever the scales are, and no block that the row does not see, or gives no weight, costs it any.
+//   For fp16 outputs P' enters as two fp16 parts, since the rounding of one would be as large as that of the output itself.
+//   Sums, maxima and the accumulators are fp32.  m and M are raised only when a score or a term exceeds them by 8 (P' then
+//   stays below 2^8).
 // * O^T[d, row] = V^T P'^T: V's bytes of four keys are interleaved into fragments, P' is transposed with movmatrix.
 //   Splits of one row are joined by a second kernel in split order, so results do not depend on timing.
 //
@@ -179,18 +181,18 @@ __global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 2) k_kv_decode(c
         }
         // lane i looks up the i-th of the warp's next 32 blocks: its page, then its place and scales
         int64_t my_at, at;
-        float my_ks, my_vs;
+        float my_ks, my_lv;                                                  // K scale, log2 of the V scale
         auto position = [&](int base) {
             const int vi = base + DEC_WARPS * lane;
             return vi < hi ? (vi < sb ? vi : vi - sb + ws) * KV_BLOCK : -1;
         };
         auto place = [&](int pos, int pg) {
             my_at = -1;
-            my_ks = my_vs = 0.f;
+            my_ks = my_lv = 0.f;
             if (pg >= 0) {
                 my_at = a.c.block(pg, h, pos);
                 my_ks = a.c.ks[my_at];
-                my_vs = a.c.vs[my_at];
+                my_lv = log2f(a.c.vs[my_at]);
             }
         };
         Bytes<16> kr[NCH][2];
@@ -215,7 +217,7 @@ __global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 2) k_kv_decode(c
         const int pos0 = position(lo + warp), pg0 = a.c.page_of(b, pos0);   // on its way while the queries are laid out
         // queries: row g of each n tile, dims 64 c + 16 t .. + 15
         uint32_t qf[NT][NCH][8];
-        float qs[NT][2], m[NT][2], l[NT][2];
+        float qs[NT][2], m[NT][2], M[NT][2], l[NT][2];
         int rpos[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -245,7 +247,7 @@ __global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 2) k_kv_decode(c
                 qs[nt][i] = __shfl_sync(0xffffffffu, fi, (2 * t + i) * 4);
                 const int rr = 8 * nt + 2 * t + i;
                 rpos[nt][i] = rr < rn ? p0 + (r0 + rr) / a.group : -1;
-                m[nt][i] = -INFINITY;
+                m[nt][i] = M[nt][i] = -INFINITY;
                 l[nt][i] = 0.f;
             }
         }
@@ -253,7 +255,7 @@ __global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 2) k_kv_decode(c
         at = __shfl_sync(0xffffffffu, my_at, 0);
         load_k(at);
         load_v(at);
-        float acc[MT][NT][4], ref = 0.f, inv_ref = 0.f;
+        float acc[MT][NT][4];
 #pragma unroll
         for (int j = 0; j < MT; ++j)
 #pragma unroll
@@ -272,7 +274,7 @@ __global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 2) k_kv_decode(c
             }
             for (int it = 0; it < cnt; ++it) {
                 const int64_t next = it + 1 < cnt ? __shfl_sync(0xffffffffu, my_at, it + 1) : -1;
-                const float ks = __shfl_sync(0xffffffffu, my_ks, it), vs = __shfl_sync(0xffffffffu, my_vs, it);
+                const float ks = __shfl_sync(0xffffffffu, my_ks, it), lv = __shfl_sync(0xffffffffu, my_lv, it);
                 if (at < 0) {   // no page: no key is visible
                     load_k(next);
                     load_v(next);
@@ -307,7 +309,8 @@ __global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 2) k_kv_decode(c
                             if (!kv_sees(a, rpos[nt][i], j0 + g)) s[nt][i] = -INFINITY;
                             if (!kv_sees(a, rpos[nt][i], j0 + g + 8)) s[nt][2 + i] = -INFINITY;
                         }
-                        raise |= fmaxf(s[nt][i], s[nt][2 + i]) > m[nt][i] + 8.f;
+                        const float mx = fmaxf(s[nt][i], s[nt][2 + i]);
+                        raise |= mx > m[nt][i] + 8.f || mx + lv > M[nt][i] + 8.f;
                     }
                 if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
@@ -318,10 +321,11 @@ __global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 2) k_kv_decode(c
                             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                            const float t = fmaxf(mx + lv, M[nt][i]), al = ex2(M[nt][i] - (t == -INFINITY ? 0.f : t));
                             mx = fmaxf(mx, m[nt][i]);
-                            const float al = ex2(m[nt][i] - (mx == -INFINITY ? 0.f : mx));
+                            l[nt][i] *= ex2(m[nt][i] - (mx == -INFINITY ? 0.f : mx));
                             m[nt][i] = mx;
-                            l[nt][i] *= al;
+                            M[nt][i] = t;
 #pragma unroll
                             for (int j = 0; j < MT; ++j) {
                                 acc[j][nt][i] *= al;
@@ -329,28 +333,16 @@ __global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 2) k_kv_decode(c
                             }
                         }
                 }
-                if (vs > 16.f * ref) {   // uniform over the warp
-                    const float nr = kv_scale_ref(vs), al = ref / nr;
-                    ref = nr;
-                    inv_ref = 1.f / nr;
-#pragma unroll
-                    for (int j = 0; j < MT; ++j)
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) acc[j][nt][i] *= al;
-                }
-                const float w = vs * inv_ref;
                 uint32_t pb[NT][2], pl[NT][2];   // P' as fp16, and for fp16 outputs what that rounding left
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     float pw[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float mi = m[nt][i & 1];
-                        const float p = ex2(s[nt][i] - (mi == -INFINITY ? 0.f : mi));
-                        l[nt][i & 1] += p;
-                        pw[i] = s[nt][i] == -INFINITY ? 0.f : p * w;   // a hidden key counts for nothing, whatever its block's scale
+                        const float mi = m[nt][i & 1], ti = M[nt][i & 1];
+                        l[nt][i & 1] += ex2(s[nt][i] - (mi == -INFINITY ? 0.f : mi));
+                        const float p = ex2((s[nt][i] - (ti == -INFINITY ? 0.f : ti)) + lv);
+                        pw[i] = s[nt][i] == -INFINITY ? 0.f : p;   // a hidden key counts for nothing, whatever its block's scale
                     }
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
@@ -399,7 +391,7 @@ __global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 2) k_kv_decode(c
                 float mx = sm_m[0][r];
 #pragma unroll
                 for (int w = 1; w < DEC_WARPS; ++w) mx = fmaxf(mx, sm_m[w][r]);
-                const float f = exp2f(m[nt][i] - (mx == -INFINITY ? 0.f : mx)) * ref;
+                const float f = exp2f(M[nt][i] - (mx == -INFINITY ? 0.f : mx));   // from units of 2^M to the maximum's
 #pragma unroll
                 for (int j = 0; j < MT; ++j)
                     *reinterpret_cast<float2 *>(&sm_o[warp][r][VB * g + 2 * j]) = make_float2(acc[j][nt][i] * f, acc[j][nt][2 + i] * f);

@@ -59,12 +59,6 @@ __device__ __forceinline__ int kv_row_exponent(float top) {
     return min(13 - e, 100);
 }
 
-// the power of two at or above a V scale, inside a range whose inverse is a normal number
-__device__ __forceinline__ float kv_scale_ref(float vs) {
-    const uint32_t e = ((__float_as_uint(vs) + 0x7FFFFFu) >> 23) & 255u;
-    return __uint_as_float(min(max(e, 7u), 247u) << 23);
-}
-
 constexpr int PF_ROWS = 256;   // rows of a many-row CTA
 
 // the many-row kernel over every sequence of at least min_rows rows (v3g_kv_prefill.cu)

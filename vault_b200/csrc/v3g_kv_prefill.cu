@@ -17,13 +17,15 @@
 // waits for a round trip.  tcgen05 operations of one thread run in order, so QK(u + 2) may overwrite P'(u).  Each tile has
 // an issuer in another quarter of the SM, because an issuing warp slows the softmax warps of its quarter (one issuer for
 // both tiles: 718 us for the 8,192-token prompt, 32/8 heads; two: 693).  The offset m of a row's exponents is its maximum
-// when m was set, plus 3; it stays until a score passes it by 11 (P' is then below 2^15).  Only then the warp rescales its O
+// when m was set, plus 3; it stays until a score passes it by 11 (P' is then below 2^11).  Only then the warp rescales its O
 // in tensor memory, after a wait for PV(u - 1): with a margin of 8 from the maximum itself, some row of the 32 did so at every
 // second step on scores of standard deviation 3.
 //
-// K scales multiply the scores; a V scale vs enters the exponent, P' = 2^(s - m + log2(vs / ref)), ref a power of two
-// that follows the largest vs (the same for the whole CTA), and the row sum takes P' ref / vs.  vs / ref is held at or above
-// 2^-40, where P' rounds to zero in fp16 whatever p is: a block with scale 0 adds nothing to O and its full weight to the sum.
+// K scales multiply the scores; a V scale vs enters the exponent, P' = 2^(s + log2 vs - M), with a second offset M of the
+// row's own that follows the largest of its terms p vs as m follows its largest score, so that no block which the row does
+// not see, or gives no weight, can push its P' into the range where fp16 has fewer bits.  O stands in units of 2^M, the row
+// sum takes P' 2^(M - m) / vs.  P' is held at or above 2^(s - m - 40), where it rounds to zero in fp16 whatever s is: a block
+// with scale 0 adds nothing to O and its full weight to the sum.
 //
 // 8,192 tokens, 32/8 heads of 128, every earlier key: 591 us, 930 TFLOP/s (517 us in a burst, before the clock falls); 4,608
 // tokens under a window of 1,024, 12/2 heads: 67 us, of which each of the two rounds of CTAs spends a quarter on its start and
@@ -51,12 +53,11 @@ struct PfSmem {
 };
 
 struct alignas(16) PfPlaces {   // of one key tile, per 16-key block
-    float ks[8], w[8], iw[8];    // K scale, log2 of vs / ref, ref / vs (both with vs / ref held at 2^-40 or above)
+    float ks[8], lv[8], iv[8];   // K scale, log2 of vs, 1 / vs
     int64_t at[8];               // index of the block in the layer
     int k0;                      // first key
     uint32_t valid, whole;       // bit i: block i has a page and some row sees it; bit 2 tile + half: every key of the half is visible
-    float al, ref;               // what a change of ref multiplies the accumulators by, ref
-    uint32_t pad[3];
+    uint32_t pad[5];
 };
 static_assert(sizeof(PfPlaces) == 192, "ring slot");
 
@@ -313,7 +314,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
             }
             const float qf = qfac[128 * tile + row];
             const int p = live ? p0 + tok : -1;
-            float m = -INFINITY, l = 0.f, lr = 0.f;   // lr: the sum as the rounded P' have it (fp16 outputs)
+            float m = -INFINITY, M = -INFINITY, l = 0.f, lr = 0.f;   // lr: the sum as the rounded P' have it (fp16 outputs)
+            float root = 0.f;   // of 2^(M - m): as two factors it stays in range; 0 while there is no M
             // Warps w of the two tiles share a quarter of the SM and its exponential unit, so they take turns at it (named
             // barriers 1 + w and 5 + w, equal step counts): together they took 1,250 clocks for 64 keys each, in turn 750.
             bool had_turn = false, gave_turn = false;
@@ -338,14 +340,13 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
                 tmem_ld64(tS + 64 * half, s);
                 // the tile's scales were written before the K that the scores come from
                 const PfPlaces &at = places[j & (PF_RING - 1)];
-                const float4 k4 = *reinterpret_cast<const float4 *>(at.ks + 4 * half), w4 = *reinterpret_cast<const float4 *>(at.w + 4 * half),
-                             i4 = *reinterpret_cast<const float4 *>(at.iw + 4 * half);
+                const float4 k4 = *reinterpret_cast<const float4 *>(at.ks + 4 * half), w4 = *reinterpret_cast<const float4 *>(at.lv + 4 * half),
+                             i4 = *reinterpret_cast<const float4 *>(at.iv + 4 * half);
                 float f[4] = {k4.x * qf, k4.y * qf, k4.z * qf, k4.w * qf};
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (f[i] < 0x1p-100f) f[i] = 0x1p-100f;   // hidden keys' -inf stays -inf in a block of scale 0; a NaN stays one
                 float wv[4] = {w4.x, w4.y, w4.z, w4.w}, iw[4] = {i4.x, i4.y, i4.z, i4.w};
-                const float al_ref = half ? 1.f : at.al;
                 const bool whole = at.whole >> (2 * tile + half) & 1u;
                 tmem_ld64_done(s);
                 if (!whole) {   // hide keys; a block that the row does not see at all loses its scales
@@ -366,25 +367,29 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
                             }
                     }
                 }
-                float mx = -INFINITY;
+                float mx = -INFINITY, tx = -INFINITY;   // largest score, largest term
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     float g = __uint_as_float(s[16 * i]);
 #pragma unroll
                     for (int e = 1; e < 15; e += 2) g = max3(g, __uint_as_float(s[16 * i + e]), __uint_as_float(s[16 * i + e + 1]));
-                    mx = fmaxf(mx, fmaxf(g, __uint_as_float(s[16 * i + 15])) * f[i]);
+                    g = fmaxf(g, __uint_as_float(s[16 * i + 15])) * f[i];
+                    mx = fmaxf(mx, g);
+                    tx = fmaxf(tx, g + wv[i]);
                 }
-                float al = al_ref;
-                bool change = al_ref != 1.f;
-                if (mx > m + 11.f) {
-                    const float f = pf_ex2(m - (mx + 3.f));
-                    m = mx + 3.f;
+                float al = 1.f;
+                if (mx > m + 11.f || tx > M + 11.f) {
+                    const float m1 = fmaxf(m, mx + 3.f), M1 = fmaxf(M, tx + 3.f), f = pf_ex2(m - m1);
                     l *= f;
                     lr *= f;
-                    al *= f;
-                    change = true;
+                    m = m1;
+                    if (M1 > -INFINITY) {
+                        al = pf_ex2(M - M1);
+                        M = M1;
+                        root = pf_ex2(0.5f * (M - m));
+                    }
                 }
-                if (__any_sync(0xffffffffu, change) && u > 0) {   // O as it stands after the step before this one
+                if (__any_sync(0xffffffffu, al != 1.f) && u > 0) {   // O as it stands after the step before this one
                     if (!(ok = pf_wait(ODONE(tile), (u - 1) & 1))) return;
                     tc::tc_fence_after();
 #pragma unroll 1
@@ -396,7 +401,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
                         tmem_st16(tO + 16 * c, o);
                     }
                 }
-                const float mu = m == -INFINITY ? 0.f : m;
+                const float mu = m == -INFINITY ? 0.f : m, Mu = M == -INFINITY ? 0.f : M, least = -40.f - mu;
+                bool weigh[4];   // fp16 outputs: the sum of the rounded P' takes part
                 uint32_t pa[32];
                 float exact[4];
                 my_turn();
@@ -406,7 +412,10 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
 #pragma unroll
                     for (int h2 = 0; h2 < 2; ++h2) {
                         const int i = 2 * c + h2;
-                        const float cw = wv[i] - mu;
+                        float cw = wv[i] - Mu;
+                        weigh[i] = cw >= -4.f - mu;
+                        iw[i] = root * iw[i] * root;
+                        if (cw < least) cw = least, iw[i] = 0x1p40f;   // a NaN stays one
                         const uint64_t f2 = f2_pack(f[i], f[i]), c2 = f2_pack(cw, cw);
                         uint64_t sum2 = 0;   // two zeros
 #pragma unroll
@@ -431,12 +440,13 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(PFULL(tile, half));
                 // fp16 outputs show what P' loses when it is rounded, so they are divided by the sum of the rounded P', whose error is
-                // in part the same (one key that outweighs the others: all of it).  Not where vs / ref is small: there P' may be 0.
+                // in part the same (one key that outweighs the others: all of it).  Not where vs is small beside the row's others: there
+                // P' may be 0.
                 if constexpr (std::is_same<T, __half>::value) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         float s0 = exact[i], s1 = 0.f;
-                        if (wv[i] >= -4.f) {
+                        if (weigh[i]) {
                             uint64_t r2 = 0;
 #pragma unroll
                             for (int e = 0; e < 8; ++e) {
@@ -463,9 +473,10 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
             if (nk > 0 && ok) {
                 ok = pf_wait(OFULL(tile), 0);
                 tc::tc_fence_after();
-                inv = places[(nk - 1) & (PF_RING - 1)].ref;
-                if constexpr (std::is_same<T, __half>::value) inv = lr == 0.f ? 0.f : (shares == 1 ? inv / lr : inv * (l / lr));
-                else if (shares == 1) inv = l == 0.f ? 0.f : inv / l;
+                // O to units of 2^m, over the sum where this CTA has all of it
+                float sum = shares == 1 ? l : 1.f;
+                if constexpr (std::is_same<T, __half>::value) sum = shares == 1 ? lr : lr / l;
+                inv = l == 0.f ? 0.f : root / sum * root;
             }
             const int64_t part = out_row * a.part_stride + share;
             if (ok && shares > 1 && nk > 0) {   // (an empty share has no accumulator)
@@ -570,7 +581,6 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
         if (warp == 14) {   // ------------------------------------------------------ pages, some tiles ahead
             // first and last position of each tile's rows
             const int lo1 = p0 + (r0 + 128) / a.group, hi0 = tiles > 1 ? p0 + (r0 + 127) / a.group : phi;
-            float e = -126.f;   // log2 of ref
             for (int j = 0; j < nk && ok; ++j) {
                 const int s = j & (PF_RING - 1), k0 = key0(j), kb = k0 + 16 * lane;
                 int pg = -1;
@@ -584,14 +594,6 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
                     ks = a.c.ks[at];
                     vs = a.c.vs[at];
                 }
-                const float lv = log2f(vs), top = warp_max(lane < 8 ? lv : -INFINITY);
-                float al = 1.f;
-                if (top > e + 4.f) {
-                    const float up = fminf(fmaxf(ceilf(top), -120.f), 120.f);
-                    al = pf_ex2(e - up);
-                    e = up;
-                }
-                const float ref = pf_ex2(e), w = lv - e;
                 uint32_t whole = 0;
                 if (lane < 4) {
                     const int t = lane >> 1, k = k0 + 64 * (lane & 1), lo = t ? lo1 : plo, hi = t ? phi : hi0;
@@ -601,16 +603,14 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
                 if (j >= PF_AHEAD && !(ok = pf_wait(ATEMPTY((j - PF_AHEAD) & (PF_RING - 1)), ((j - PF_AHEAD) / PF_RING) & 1))) break;
                 if (lane < 8) {
                     places[s].ks[lane] = ks;
-                    places[s].w[lane] = w < -40.f ? -40.f : w;   // a NaN stays one
-                    places[s].iw[lane] = fminf(ref / vs, 0x1p40f);
+                    places[s].lv[lane] = log2f(vs);
+                    places[s].iv[lane] = 1.f / vs;
                     places[s].at[lane] = at;
                 }
                 if (lane == 8) {
                     places[s].k0 = k0;
                     places[s].valid = valid;
                     places[s].whole = whole;
-                    places[s].al = al;
-                    places[s].ref = ref;
                 }
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(ATFULL(s));
