@@ -335,8 +335,8 @@ V3G_API int v3g_kv_attention(const v3g_kv_cache_t *cache, uint32_t layer, const 
 V3G_API int v3g_kv_reorder(const v3g_kv_cache_t *cache, const v3g_kv_batch_t *batch, uint32_t beams, const int32_t *dev_parents,
                            const int32_t *dev_dst_page, int32_t *table_out, uint64_t table_out_ld, int32_t *dev_status, void *stream);
 /* One step of beam search: of every group's beams x vocab continuations, scored (logit - logsumexp of the beam's
- * logits) + scores[beam], the `beams` best in descending order; equal scores go to the lower beam * vocab + token
- * (different logits of one beam that round to the same score may also come in the order of the logits).
+ * logits) + scores[beam], the `beams` best in descending order; equal scores go to the lower beam * vocab + token.  Scores are
+ * fp32 (the last bits of a logsumexp depend on the number of rows, which decides how they are divided).
  * logits [groups * beams] rows ld elements apart (dtype any).  A finished beam (finished may be NULL) has one
  * continuation: eos_id at its own score.  Continuations scored NaN or -inf are never chosen; slots left over get token
  * eos_id (0 when eos_id < 0), parent = their own beam, score -inf and count as finished.  NaN logits are skipped.

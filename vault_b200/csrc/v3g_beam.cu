@@ -5,14 +5,18 @@
 // The logits are read once (4 bytes and an exponential per element: HBM bounds it).  Inside a beam the order of the
 // scores is the order of the logits, so the first kernel needs no lse: a CTA streams a slice of one beam's logits, each
 // thread keeping the maximum and the sum of exponentials of its own, and writes the slice's `beams` best as 64-bit keys
-// (value, then lower index).  The second kernel joins the sums of a beam and selects among the slices' best, reading only
-// those of the slices whose maximum can be among the answers.  Both selections are exact: the `beams`-th largest of 64 group
-// maxima bounds the answer from below; the few threads whose maximum reaches it have their logits read again, and what is
-// at or above it is collected and ranked by counting; where too much is (long ties), `beams` rounds of a block maximum take
-// its place.
+// (value, then lower index) and the largest logit that it leaves out.  The second kernel joins the sums of a beam and selects
+// among the slices' best, reading only those of the slices whose maximum can be among the answers.  Both selections are exact:
+// the `beams`-th largest of 64 group maxima bounds the answer from below; the few threads whose maximum reaches it have their
+// logits read again, and what is at or above it is collected and ranked by counting; where too much is (long ties), `beams`
+// rounds of a block maximum take its place.
 //
-// 48 x 8 beams over 151,936 logits (233 MB) take 43 us in fp32 (slices 41, 5.7 TB/s; the join, 6 alone, starts under them) and
-// 35 us in bf16, where loads and powers of a CTA alternate; one request of 4 beams 6.6 us.
+// Equal scores go to the lower index, but different logits may round to one score, and a slice chose by logit.  What it left
+// out scores at most what the last place is worth, so only places of that score can be wrong, and only if a left-out logit has
+// it too.  Then those places are given out again, over the logits themselves in the order of their indices.
+//
+// 48 x 8 beams over 151,936 logits (233 MB) take 44 us in fp32 (5.3 TB/s; the join starts under the slices) and
+// 35 us in bf16, where loads and powers of a CTA alternate; one request of 4 beams 7.0 us.
 #include <cfloat>
 
 #include "v3g_internal.h"
@@ -36,7 +40,7 @@ struct BeamShared {
     u64 buf[BEAM_BUF];
     u64 red[BEAM_THREADS / 32];
     float4 group[BEAM_GROUPS / 4];
-    float bound;
+    float bound, next;           // next: what the best leave out
     int count, listed;
 };
 
@@ -136,7 +140,7 @@ __device__ __forceinline__ float beam_ex2(float x) {
 constexpr int BEAM_EPT = 32, BEAM_STEP = BEAM_THREADS * BEAM_EPT;
 template <typename T>
 __global__ void __launch_bounds__(BEAM_THREADS, 4) k_beam_slice(const T *logits, int64_t ld, int vocab, int slice, int beams, bool vec, u64 *keys,
-                                                               float2 *sums) {
+                                                               float4 *sums) {
     __shared__ BeamShared sm;
     __shared__ float red[BEAM_THREADS / 32];
     __shared__ uint32_t list[BEAM_THREADS];
@@ -196,7 +200,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 4) k_beam_slice(const T *logits,
         sum = sum * power(mine, m) + add;
         mine = m;
     }
-    const float bound = beam_bound(sm, mine, beams);
+    const float bound = beam_bound(sm, mine, beams + 1);
     const float *group = reinterpret_cast<const float *>(sm.group);
     float top = fmaxf(group[lane], group[lane + 32]);
     top = warp_max(top);                                          // the slice's maximum
@@ -210,7 +214,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 4) k_beam_slice(const T *logits,
     __syncthreads();
     const int listed = sm.listed;
     beam_best(
-        sm, beams, float_key(bound),
+        sm, beams + 1, float_key(bound),
         [&](auto f) {
             for (int k = tid / BEAM_EPT; k < listed; k += BEAM_THREADS / BEAM_EPT) {
                 const uint32_t l = list[k];
@@ -222,35 +226,42 @@ __global__ void __launch_bounds__(BEAM_THREADS, 4) k_beam_slice(const T *logits,
                 }
             }
         },
-        [&](int rank, u64 k) { keys[at * beams + rank] = k; });
+        [&](int rank, u64 k) {
+            if (rank < beams) keys[at * beams + rank] = k;
+            else sm.next = k ? key_float((uint32_t)(k >> 32)) : -INFINITY;
+        });
+    __syncthreads();
     if (tid == 0) {   // red was written before beam_best's barrier
         sum = red[0];
         for (int w = 1; w < BEAM_THREADS / 32; ++w) sum += red[w];
-        sums[at] = make_float2(top, sum);
+        sums[at] = make_float4(top, sum, sm.next, 0.f);
     }
 }
 
 struct BeamArgs {
+    const void *logits;
+    int64_t ld;
     const u64 *keys;    // the slices' best, largest first
-    const float2 *sums;
+    const float4 *sums; // their largest logit, sum, and the largest logit that is not among the best
     const float *scores;
     const uint8_t *finished;
-    int beams, slices, vocab, eos;
+    int beams, slice, slices, vocab, eos;
     int32_t *tokens, *parents;
     float *scores_out;
     uint8_t *finished_out;
 };
 
+template <typename T>
 __global__ void __launch_bounds__(BEAM_THREADS) k_beam_join(const __grid_constant__ BeamArgs a) {
     __shared__ BeamShared sm;
     __shared__ u64 only[V3G_BEAM_MAX];
-    __shared__ float lse[V3G_BEAM_MAX], run[V3G_BEAM_MAX];
+    __shared__ float lse[V3G_BEAM_MAX], run[V3G_BEAM_MAX], given[V3G_BEAM_MAX];
     __shared__ bool done[V3G_BEAM_MAX];
-    __shared__ int list[BEAM_LIST];
+    __shared__ int list[BEAM_LIST], found[BEAM_THREADS / 32];
     griddep_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, K = a.beams, n = a.slices * K;
     const int64_t g0 = (int64_t)blockIdx.x * K;
-    const float2 *sums = a.sums + g0 * a.slices;
+    const float4 *sums = a.sums + g0 * a.slices;
     const u64 *keys = a.keys + g0 * a.slices * K;
     const bool few = n * K <= 4 * BEAM_THREADS;   // every key fits the threads' registers
     u64 ahead[4];
@@ -259,7 +270,7 @@ __global__ void __launch_bounds__(BEAM_THREADS) k_beam_join(const __grid_constan
         for (int i = 0; i < 4; ++i) ahead[i] = tid + BEAM_THREADS * i < n * K ? keys[tid + BEAM_THREADS * i] : 0ull;
     // a warp takes a beam: its logsumexp
     for (int k = warp; k < K; k += BEAM_THREADS / 32) {
-        const float2 *p = sums + (int64_t)k * a.slices;
+        const float4 *p = sums + (int64_t)k * a.slices;
         const float run_k = a.scores[g0 + k];
         const bool done_k = a.finished && a.finished[g0 + k];
         float m = -INFINITY;
@@ -267,7 +278,7 @@ __global__ void __launch_bounds__(BEAM_THREADS) k_beam_join(const __grid_constan
         m = warp_max(m);
         float s = 0.f;
         for (int i = lane; i < a.slices; i += 32) {
-            const float2 v = p[i];
+            const float4 v = p[i];
             if (v.x > -INFINITY) s += v.y * beam_ex2((v.x - m) * 1.44269504f);
         }
         s = m + logf(warp_sum(s));
@@ -290,7 +301,12 @@ __global__ void __launch_bounds__(BEAM_THREADS) k_beam_join(const __grid_constan
     // consecutive slices go to different groups of the bound: often one beam alone has candidates
     const int mine = tid % (BEAM_THREADS / BEAM_GROUPS) * BEAM_GROUPS + tid / (BEAM_THREADS / BEAM_GROUPS);
     float top = tid < K && only[tid] ? run[tid] : -INFINITY;
-    for (int i = mine; i < n; i += BEAM_THREADS) top = fmaxf(top, score(i / a.slices, sums[i].x));
+    float left = -INFINITY;   // the best score that a slice left out
+    for (int i = mine; i < n; i += BEAM_THREADS) {
+        const float4 v = sums[i];
+        top = fmaxf(top, score(i / a.slices, v.x));
+        left = fmaxf(left, score(i / a.slices, v.z));
+    }
     const float bound = beam_bound(sm, top, K), lo = fmaxf(bound, -FLT_MAX);
     if (!few && top >= lo)
         for (int i = mine; i < n; i += BEAM_THREADS)
@@ -316,15 +332,19 @@ __global__ void __launch_bounds__(BEAM_THREADS) k_beam_join(const __grid_constan
         }
         if (tid < K && only[tid]) f(only[tid]);
     };
+    auto put = [&](int rank, int parent, int token, float y) {
+        const int64_t at = g0 + rank;
+        a.tokens[at] = token;
+        a.parents[at] = parent;
+        a.scores_out[at] = y;
+        a.finished_out[at] = done[parent] || token == a.eos;
+    };
     beam_best(sm, K, float_key(bound), each, [&](int rank, u64 k) {
         const int64_t at = g0 + rank;
+        given[rank] = k ? key_float((uint32_t)(k >> 32)) : INFINITY;   // an empty place: nothing was left out
         if (k) {
             const uint32_t flat = 0xFFFFFFFFu - (uint32_t)k;
-            const int parent = (int)(flat / (uint32_t)a.vocab), token = (int)(flat % (uint32_t)a.vocab);
-            a.tokens[at] = token;
-            a.parents[at] = parent;
-            a.scores_out[at] = key_float((uint32_t)(k >> 32));
-            a.finished_out[at] = done[parent] || token == a.eos;
+            put(rank, (int)(flat / (uint32_t)a.vocab), (int)(flat % (uint32_t)a.vocab), given[rank]);
         } else {
             a.tokens[at] = a.eos < 0 ? 0 : a.eos;
             a.parents[at] = rank;
@@ -332,6 +352,48 @@ __global__ void __launch_bounds__(BEAM_THREADS) k_beam_join(const __grid_constan
             a.finished_out[at] = 1;
         }
     });
+    __syncthreads();
+    const float last = given[K - 1];
+    if (!__syncthreads_or(left >= last)) return;
+    // The places worth `last`, to the lowest indices that have this score.  A thread looks at PER consecutive logits at a time.
+    constexpr int PER = 16;
+    int rank = 0;
+    while (given[rank] > last) ++rank;
+    for (int k = 0; k < K && rank < K; ++k) {
+        if (done[k]) {
+            if (only[k] && run[k] == last) {
+                if (tid == 0) put(rank, k, a.eos, last);
+                ++rank;
+            }
+            continue;
+        }
+        const T *p = static_cast<const T *>(a.logits) + (g0 + k) * a.ld;
+        for (int s = 0; s < a.slices && rank < K; ++s) {
+            if (!(score(k, sums[k * a.slices + s].x) >= last)) continue;
+            const int end = min((s + 1) * a.slice, a.vocab);
+            for (int i0 = s * a.slice; i0 < end && rank < K; i0 += BEAM_THREADS * PER) {
+                const int first = i0 + tid * PER;
+                uint32_t has = 0;
+                for (int e = 0; e < PER; ++e)
+                    if (first + e < end && score(k, beam_value(p[first + e])) == last) has |= 1u << e;
+                int upto = __popc(has);
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int y = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += y;
+                }
+                if (lane == 31) found[warp] = upto;
+                __syncthreads();
+                int at = rank + upto - __popc(has);
+                for (int w = 0; w < BEAM_THREADS / 32; ++w) {
+                    at += w < warp ? found[w] : 0;
+                    rank += found[w];
+                }
+                for (; has && at < K; has &= has - 1) put(at++, k, first + __ffs(has) - 1, last);
+                __syncthreads();
+            }
+        }
+    }
 }
 
 struct BeamPlan {
@@ -348,17 +410,23 @@ static BeamPlan beam_plan(uint64_t rows, uint32_t beams, uint32_t vocab) {
     const uint64_t each = (steps + want - 1) / want;
     p.slice = (int)(each * BEAM_STEP);
     p.slices = (int)((steps + each - 1) / each);
-    p.keys = (rows * p.slices * sizeof(float2) + 255) & ~(size_t)255;
+    p.keys = (rows * p.slices * sizeof(float4) + 255) & ~(size_t)255;
     p.bytes = p.keys + rows * p.slices * beams * sizeof(u64);
     return p;
 }
 
 template <typename T>
 static cudaError_t launch_slices(const void *logits, int64_t ld, int vocab, int beams, const BeamPlan &p, uint32_t rows, u64 *keys,
-                                 float2 *sums, cudaStream_t st) {
+                                 float4 *sums, cudaStream_t st) {
     const bool vec = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && ld * sizeof(T) % 16 == 0;
     return launch_k(false, k_beam_slice<T>, dim3(p.slices, rows), BEAM_THREADS, 0, st, static_cast<const T *>(logits), ld, vocab, p.slice,
                     beams, vec, keys, sums);
+}
+
+template <typename T>
+static cudaError_t launch_beam(const BeamArgs &a, const BeamPlan &p, uint32_t groups, u64 *keys, float4 *sums, cudaStream_t st) {
+    const cudaError_t e = launch_slices<T>(a.logits, a.ld, a.vocab, a.beams, p, groups * a.beams, keys, sums, st);
+    return e == cudaSuccess ? launch_k(true, k_beam_join<T>, dim3(groups), BEAM_THREADS, 0, st, a) : e;
 }
 
 }  // namespace v3g
@@ -389,13 +457,16 @@ extern "C" int v3g_beam_select(const void *dev_logits, int dtype, uint32_t group
     if (!dev_work || work_bytes < p.bytes) return v3g_fail(V3G_E_SIZE, "v3g_beam_select: workspace too small");
     if (reinterpret_cast<uintptr_t>(dev_work) % 256) return v3g_fail(V3G_E_ALIGN, "v3g_beam_select: the workspace needs 256-byte alignment");
     BeamArgs a = {};
-    float2 *sums = static_cast<float2 *>(dev_work);
+    float4 *sums = static_cast<float4 *>(dev_work);
     u64 *keys = reinterpret_cast<u64 *>(static_cast<uint8_t *>(dev_work) + p.keys);
+    a.logits = dev_logits;
+    a.ld = (int64_t)ld;
     a.keys = keys;
     a.sums = sums;
     a.scores = dev_scores;
     a.finished = dev_finished;
     a.beams = (int)beams;
+    a.slice = p.slice;
     a.slices = p.slices;
     a.vocab = (int)vocab;
     a.eos = eos_id;
@@ -405,9 +476,8 @@ extern "C" int v3g_beam_select(const void *dev_logits, int dtype, uint32_t group
     a.finished_out = finished_out;
     const cudaStream_t st = (cudaStream_t)stream;
     cudaError_t e;
-    if (dtype == V3G_F32) e = launch_slices<float>(dev_logits, (int64_t)ld, (int)vocab, (int)beams, p, rows, keys, sums, st);
-    else if (dtype == V3G_F16) e = launch_slices<__half>(dev_logits, (int64_t)ld, (int)vocab, (int)beams, p, rows, keys, sums, st);
-    else e = launch_slices<__nv_bfloat16>(dev_logits, (int64_t)ld, (int)vocab, (int)beams, p, rows, keys, sums, st);
-    if (e == cudaSuccess) e = launch_k(true, k_beam_join, dim3(groups), BEAM_THREADS, 0, st, a);
+    if (dtype == V3G_F32) e = launch_beam<float>(a, p, groups, keys, sums, st);
+    else if (dtype == V3G_F16) e = launch_beam<__half>(a, p, groups, keys, sums, st);
+    else e = launch_beam<__nv_bfloat16>(a, p, groups, keys, sums, st);
     return e == cudaSuccess ? V3G_OK : v3g_fail(V3G_E_CUDA, std::string("v3g_beam_select: ") + cudaGetErrorString(e));
 }

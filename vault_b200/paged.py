@@ -300,7 +300,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: Optional[t
     """One step of beam search: logits [groups, beams, vocab] (fp32, fp16 or bf16), scores [groups, beams] fp32 (-inf: no
     beam yet), finished [groups, beams] uint8.  Of each group's continuations, scored log_softmax(logits) + scores, the
     `beams` best in descending order: (tokens, parents, scores, finished), each [groups, beams].  A finished beam goes on
-    with eos_id alone, at its own score; equal scores go to the lower (beam, token); continuations at -inf or NaN are
+    with eos_id alone, at its own score; equal (fp32) scores go to the lower (beam, token); continuations at -inf or NaN are
     never chosen, and slots left over come back finished, with score -inf."""
     dt = _DTYPES.get(logits.dtype)
     if dt is None or logits.dim() != 3 or not logits.is_cuda or logits.numel() == 0:
