@@ -272,7 +272,8 @@ V3G_API int v3g_argmax_noalloc(const float *dev_logits, uint32_t rows, uint32_t 
  *
  * A batch names its sequences by device arrays.  Token i of sequence b (packed index q_start[b] + i, of
  * n_b = q_start[b + 1] - q_start[b]) stands at position kv_len[b] - n_b + i, so kv_len counts the batch's tokens too
- * and the same arrays serve the append and the attention that follows.  Sequences without tokens are allowed.
+ * and the same arrays serve the append and the attention that follows.  Sequences without tokens are allowed, and packed
+ * rows that belong to no sequence (a step of fixed size that is not full): their queries and outputs become zero.
  * Position p of sequence b lives in page page_table[b * table_ld + p / page]; an entry outside [0, n_pages) is no
  * page: nothing is stored there and attention sees no key there.  The arrays are not read on the host; whatever they
  * hold, no kernel leaves the cache's and the batch's bounds. */
@@ -314,10 +315,10 @@ V3G_API int v3g_kv_read(const v3g_kv_cache_t *cache, uint32_t layer, uint32_t n_
 /* Attention of the batch's query rows (dtype V3G_F16 or V3G_BF16) over `layer`: out [n_tokens][n_q_heads][head_dim] of
  * the same type, lse [n_tokens][n_q_heads] fp32 (natural logarithm of the sum of exponentials; may be NULL).  Query
  * heads h n_q_heads / n_kv_heads .. share KV head h.  A token at position p sees keys j <= p with j > p - window or
- * j < n_sink (window 0: all).  A row that sees no key gives zeros and lse -inf.  max_q and max_kv are the largest token
- * count and length of a sequence as far as the host knows them (0: unknown): they choose kernels and splits, never
- * results' validity.  *dev_status (may be NULL) gets V3G_STATUS_TIMEOUT if a bounded wait inside a kernel ran out (the
- * output is then invalid).  dev_work: v3g_kv_attention_work_size bytes of device memory, 256-byte aligned, with no content
+ * j < n_sink (window 0: all).  A row that sees no key, or belongs to no sequence,
+ * gives zeros and lse -inf.  max_q and max_kv are the largest token count and length of a sequence as far as the host
+ * knows them (0: unknown): they choose kernels and splits, never results' validity.  *dev_status (may be NULL) gets
+ * V3G_STATUS_TIMEOUT if a bounded wait inside a kernel ran out (the output is then invalid).  dev_work: v3g_kv_attention_work_size bytes of device memory, 256-byte aligned, with no content
  * kept between calls.  A call queues several kernels: threads that share a workspace queue their calls one after the
  * other (under a lock), on one stream. */
 V3G_API size_t v3g_kv_attention_work_size(const v3g_kv_cache_t *cache, const v3g_kv_batch_t *batch, uint32_t n_q_heads,

@@ -212,7 +212,16 @@ __global__ void __launch_bounds__(32 * APPEND_WARPS, append_ctas<T, D, VEC>()) k
     const int p0 = a.c.end(b) - n;                                        // position of the first new token
     const int blk = (p0 >> 4) + (int)(blockIdx.x - base);                 // arithmetic shift: p0 may be negative
     const int lo = max(blk * KV_BLOCK, p0), hi = min(blk * KV_BLOCK + KV_BLOCK, p0 + n);
-    if (lo >= hi) return;
+    if (lo >= hi) {
+        // past the last sequence's blocks: the queries of no sequence (the grid has one such CTA at least)
+        const int idle = (int)(blockIdx.x - base) - (n > 0 ? ((p0 + n - 1) >> 4) - (p0 >> 4) + 1 : 0);
+        if (a.q && b == a.c.batch - 1 && idle >= 0) {
+            const int64_t cta = (int64_t)idle * gridDim.y + blockIdx.y, ctas = (int64_t)(gridDim.x - blockIdx.x + idle) * gridDim.y;
+            kv_clear_loose<T, D>(a.c, static_cast<T *>(a.q_out), nullptr, a.q_heads, cta * (32 * APPEND_WARPS) + threadIdx.x,
+                                 ctas * (32 * APPEND_WARPS));
+        }
+        return;
+    }
     const int t0 = first + (lo - p0), nt = hi - lo;                       // the block's packed tokens
     const int s0 = lo - blk * KV_BLOCK;
     const bool turn = a.rope != nullptr;
@@ -520,7 +529,7 @@ extern "C" int v3g_kv_append(const v3g_kv_cache_t *cache, uint32_t layer, const 
     a.rope = rope;
     a.rope_rows = (int)rope_rows;
     a.status = dev_status;
-    const uint32_t items = batch->n_tokens / KV_BLOCK + 2 * batch->batch;
+    const uint32_t items = batch->n_tokens / KV_BLOCK + 2 * batch->batch + 1;
     // A block's heads are shared out over CTAs while the blocks are few (8 sequences of up to 200 tokens, 32/8 heads: one CTA a
     // block 15.5 us, shared out 10.0 us), and further so that the last round of CTAs is a small part of all (11,247 bf16 tokens: 32
     // CTAs an SM in all 46.5 us, 8 of them 56.4); past one pass of the warps over the heads there is nothing left to share.

@@ -39,6 +39,12 @@ struct KvView {
         first = min(max(q_start[b], 0), n_tokens);
         return max(min(q_start[b + 1], n_tokens) - first, 0);
     }
+    // packed rows that belong to no sequence, before the first and after the last: how many; row(i): the i-th of them
+    __device__ __forceinline__ int loose(int &before, int &after) const {
+        before = min(max(q_start[0], 0), n_tokens);
+        after = min(max(q_start[batch], 0), n_tokens);
+        return before + n_tokens - after;
+    }
     // page that holds position pos of sequence b, -1 where there is none
     __device__ __forceinline__ int page_of(int b, int pos) const {
         const int i = pos >> page_shift;
@@ -100,6 +106,20 @@ __device__ __forceinline__ void kv_store4(__half *p, float4 x) {
 __device__ __forceinline__ void kv_store4(__nv_bfloat16 *p, float4 x) {
     const __nv_bfloat162 a = __floats2bfloat162_rn(x.x, x.y), b = __floats2bfloat162_rn(x.z, x.w);
     *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+}
+
+// Zeros to the rows of out [n_tokens][heads][D] that belong to no sequence, and -inf to their lse (may be null): the share of
+// worker `w` of `workers`.
+template <typename T, int D>
+__device__ __forceinline__ void kv_clear_loose(const KvView &c, T *out, float *lse, int heads, int64_t w, int64_t workers) {
+    constexpr int PIECES = D * sizeof(T) / 16;
+    int before, after;
+    const int rows = c.loose(before, after);
+    for (int64_t i = w; i < (int64_t)rows * heads * PIECES; i += workers) {
+        const int64_t head = i / PIECES, at = head + (head < (int64_t)before * heads ? 0 : (int64_t)(after - before) * heads);
+        reinterpret_cast<uint4 *>(out + at * D)[i % PIECES] = make_uint4(0u, 0u, 0u, 0u);
+        if (lse && i % PIECES == 0) lse[at] = -INFINITY;
+    }
 }
 
 // host: argument checks shared by the entry points; fills the kernels' view of `layer`

@@ -140,6 +140,10 @@ __global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 2) k_kv_decode(c
     const int rt0 = idx % a.row_tiles;
     idx /= a.row_tiles;
     int h, b, split, shares = a.splits;
+    auto clear = [&]() {
+        kv_clear_loose<T, D>(a.c, static_cast<T *>(a.out), a.lse, a.c.heads * a.group, (int64_t)blockIdx.x * (32 * DEC_WARPS) + threadIdx.x,
+                             (int64_t)gridDim.x * (32 * DEC_WARPS));
+    };
     griddep_launch();
     if (a.units) {
         h = idx % a.c.heads;
@@ -149,7 +153,10 @@ __global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 2) k_kv_decode(c
         }
         __syncthreads();
         b = sm_share[0], split = sm_share[1], shares = sm_share[2];
-        if (b < 0) return;
+        if (b < 0) {
+            clear();
+            return;
+        }
     } else {
         split = idx % a.splits;
         idx /= a.splits;
@@ -422,6 +429,7 @@ __global__ void __launch_bounds__(32 * DEC_WARPS, NT == 1 ? 4 : 2) k_kv_decode(c
         }
         __syncthreads();
     }
+    clear();
 }
 
 // Joins the shares of a row: WR warps take every WR-th share each, in order, and are added in order.  Latency bounds it (5 us
@@ -561,7 +569,7 @@ static KvAttnPlan kv_plan(const v3g_kv_cache_t *c, const v3g_kv_batch_t *b, uint
         uint64_t s = 148 / live;
         s = s > most ? most : s;
         s = s > room ? room : s;
-        p.pf_items = (int)items;
+        p.pf_items = (int)items + 1;   // one that is never a sequence's
         p.pf_splits = s < 1 ? 1 : (s > 128 ? 128 : (int)s);
     }
     p.part_stride = p.splits > p.pf_splits ? p.splits : p.pf_splits;

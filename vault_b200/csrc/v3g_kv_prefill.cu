@@ -195,7 +195,12 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
     const int n = a.c.tokens(b, first);
     const int64_t off = (item - base) * PF_ROWS;
     if (off < 0 || off >= (int64_t)n * a.group || n * a.group < min_rows) {
+        // past the last sequence's units (one for each head at least): the rows of no sequence, unless the few-row kernel runs
+        const int64_t idle = item - base - ((int64_t)n * a.group + PF_ROWS - 1) / PF_ROWS, per = (int64_t)a.c.heads * shares;
         if (a.after_few) griddep_wait();
+        else if (b == a.c.batch - 1 && idle >= 0)
+            kv_clear_loose<T, D>(a.c, static_cast<T *>(a.out), a.lse, a.c.heads * a.group,
+                                 (idle * per + h * shares + share) * PF_THREADS + threadIdx.x, (a.pf_items - item + idle) * per * PF_THREADS);
         return;
     }
     const int r0 = (int)off, rn = min(n * a.group - r0, PF_ROWS), tiles = rn > 128 ? 2 : 1;

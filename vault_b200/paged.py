@@ -10,8 +10,8 @@ The operators a serving loop needs around its projections, for batches of sequen
     page_table = cache.reorder(page_table, kv_len, parents)
 
 Tokens are packed: rows q_start[b] .. q_start[b + 1] - 1 belong to sequence b and stand at its last positions, kv_len[b]
-counting them.  page_table[b, i] is the page of tokens i * page .. (i + 1) * page - 1 of sequence b, negative where there
-is none.  Index tensors are int32 on the cache's device.  Calls run on torch's current stream and read no tensor on the
+counting them; rows past q_start[-1] belong to none and come out as zeros.  page_table[b, i] is the page of tokens
+i * page .. (i + 1) * page - 1 of sequence b, negative where there is none.  Index tensors are int32 on the cache's device.  Calls run on torch's current stream and read no tensor on the
 host; all device work is the C ABI's (include/vault_b200.h).  No result depends on the order in which blocks run.
 """
 
