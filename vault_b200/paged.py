@@ -136,10 +136,13 @@ class PagedKVCache:
         return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale))
 
     def check(self) -> None:
-        """Synchronize and raise if a token or a beam had no place (V3G_STATUS_BOUNDS) since the last check."""
+        """Wait for the device, every stream of it, and raise if a token or a beam had no place (V3G_STATUS_BOUNDS) since the
+        last check."""
+        torch.cuda.synchronize(self.device)   # the read below waits for the current stream alone
         bits = int(self.status_word.item())
         if bits:
             self.status_word.zero_()
+            torch.cuda.synchronize(self.device)   # what other streams run from here on is not wiped
             raise RuntimeError(f"device status bits {bits:#x}: " +
                                ("a token without a page or a rotation row was dropped, or a beam's parent or page does not exist"
                                 if bits & _lib.V3G_STATUS_BOUNDS else "a kernel gave up waiting, its output is invalid"))
