@@ -320,6 +320,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: Optional[t
     if finished is not None and (finished.dtype not in (torch.uint8, torch.bool) or finished.shape != rows or
                                  finished.device != dev or not finished.is_contiguous()):
         raise ValueError("finished must be a contiguous uint8 [groups, beams] tensor on the logits' device")
+    eos_id = min(max(eos_id, -1), 0x7FFFFFFF)   # as 32 bits: none at all, or past every vocabulary, which the engine refuses
     L = _lib.lib()
     best = torch.empty_like(scores)
     tokens = torch.empty_like(scores, dtype=torch.int32)
