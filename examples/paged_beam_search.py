@@ -70,6 +70,8 @@ def beam_search(dec: PagedDecoder, prompts: List[List[int]], beams: int, steps: 
     """The best `beams` continuations of every prompt: tokens [prompts, beams, steps] and their log-probabilities
     [prompts, beams], best first.  Each beam owns a column of pages; full pages are shared between the beams that descend
     from the same one."""
+    if not prompts or not all(prompts):
+        raise ValueError("every prompt needs a token to go on from")
     dev, groups, page = dec.cache.device, len(prompts), dec.cache.page
     rows, longest = groups * beams, max(len(p) for p in prompts)
     cols = -(-(longest + steps) // page)
