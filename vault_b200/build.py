@@ -7,6 +7,7 @@ The library is a plain C-ABI .so (include/vault_b200.h) built in-tree so it ship
 from __future__ import annotations
 
 import os
+import re
 import subprocess
 import sys
 
@@ -21,8 +22,11 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-shared", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
-    "--expt-relaxed-constexpr", "-Xptxas", "-warn-spills",
+    "--expt-relaxed-constexpr", "-Xptxas", "-warn-spills,-v",
 ]
+# Registers a thread of the kernels whose warps trade them: a launch has to bring what the warps' shares add up to, so such a
+# kernel refuses to run with another number, and a compiler that allots one is to be noticed here.
+REGISTERS = {"k_kv_prefill": 128}
 
 
 def _stale() -> bool:
@@ -33,13 +37,34 @@ def _stale() -> bool:
     return any(os.path.getmtime(p) > t for p in deps)
 
 
+def check_registers(log: str) -> None:
+    """Raise unless ptxas's report has every kernel of REGISTERS, each instance with its number."""
+    found, kernel = {k: set() for k in REGISTERS}, None
+    for line in log.splitlines():
+        entry = re.search(r"Compiling entry function '(\w+)'", line)
+        if entry:
+            kernel = next((k for k in REGISTERS if k in entry.group(1)), None)
+        used = re.search(r"Used (\d+) registers", line)
+        if used and kernel:
+            found[kernel].add(int(used.group(1)))
+            kernel = None
+    for k, want in REGISTERS.items():
+        if found[k] != {want}:
+            raise RuntimeError(f"{k} needs {want} registers a thread, ptxas allotted {sorted(found[k]) or 'none'}")
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     if not force and not _stale():
         return LIB
     cmd = [NVCC, *FLAGS, "-I", os.path.join(REPO, "include"), *[os.path.join(CSRC, s) for s in SOURCES], "-o", LIB + ".tmp"]
     if verbose:
         print(" ".join(cmd), flush=True)
-    subprocess.run(cmd, check=True)
+    run = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    report = re.compile(r"ptxas info|\s+\d+ bytes stack frame")
+    said = run.stdout if run.returncode else "".join(x for x in run.stdout.splitlines(True) if not report.match(x))
+    sys.stderr.write(said)
+    run.check_returncode()
+    check_registers(run.stdout)
     os.replace(LIB + ".tmp", LIB)
     return LIB
 
