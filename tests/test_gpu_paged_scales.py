@@ -152,3 +152,21 @@ def test_zero_scales_that_take_the_weight(new, dtype):
     parts[3].zero_()
     out, lse = _attend(parts, bt, q, 0, 0)
     assert bool((out == 0).all()) and bool(((lse.double() - want_lse).abs() <= tol_lse).all())
+
+
+@pytest.mark.parametrize("new", [1, 40, 140])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_values_do_not_reach_lse(new, bad, dtype):
+    """V scales that are no number: the rows that see them have no output, and the lse they have without them."""
+    d = 64
+    bt = ref.Batch([new], [100], 16, seed=new)
+    parts = ref.random_cache(1, bt.n_pages, 1, 16, d, seed=3, scale=0.02)
+    q = torch.randn(new, 2, d, generator=torch.Generator().manual_seed(3)).to(dtype)
+    _, want, _, tol = ref.attention(q, parts, 0, bt, 0, 0, d ** -0.5)
+    for j in (20, 100 + new - 1):
+        pg, blk = _block(bt, j)
+        parts[3][0, pg, :, blk] = bad
+        out, lse = _attend(parts, bt, q, 0, 0)
+        sees = torch.arange(100, 100 + new) >= j - j % 16
+        assert bool(((lse.double() - want).abs() <= tol).all()) and not bool(out[sees].isfinite().any())

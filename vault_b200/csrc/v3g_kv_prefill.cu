@@ -25,7 +25,8 @@
 // row's own that follows the largest of its terms p vs as m follows its largest score, so that no block which the row does
 // not see, or gives no weight, can push its P' into the range where fp16 has fewer bits.  O stands in units of 2^M, the row
 // sum takes P' 2^(M - m) / vs.  P' is held at or above 2^(s - m - 40), where it rounds to zero in fp16 whatever s is: a block
-// with scale 0 adds nothing to O and its full weight to the sum.
+// with scale 0 adds nothing to O and its full weight to the sum.  So does one whose V scale is NaN or infinite, since V is no
+// matter of the sum; the warp that looks up the scales notes which rows see such a block, and those have no output.
 //
 // 8,192 tokens, 32/8 heads of 128, every earlier key: 591 us, 930 TFLOP/s (517 us in a burst, before the clock falls); 4,608
 // tokens under a window of 1,024, 12/2 heads: 67 us, of which each of the two rounds of CTAs spends a quarter on its start and
@@ -255,6 +256,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
     auto ATEMPTY = [&](int s) { return bars + 8u * (29 + s); };
     const uint32_t DRAIN = bars + 8u * 37;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + SM::BAR + 8 * 38);
+    uint32_t *spoilt = tmem_slot + 2;   // a bit for each row: it sees a V scale that is NaN or infinite
     PfPlaces *places = reinterpret_cast<PfPlaces *>(smem + SM::SC);
     if (threadIdx.x == 0) {
         tc::mbar_init(QFULL, 4 * tiles);
@@ -275,6 +277,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
             tc::mbar_init(ATEMPTY(s), 4);
         }
         tc::mbar_init(DRAIN, tiles);
+        for (int i = 0; i < PF_ROWS / 32; ++i) spoilt[i] = 0u;
         tc::mbar_fence_init();
     }
     if (warp == 12) tc::tmem_alloc(tc::smem_addr(tmem_slot), 512);
@@ -420,7 +423,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
                         float cw = wv[i] - Mu;
                         weigh[i] = cw >= -4.f - mu;
                         iw[i] = root * iw[i] * root;
-                        if (cw < least) cw = least, iw[i] = 0x1p40f;   // a NaN stays one
+                        if (cw < least) cw = least, iw[i] = 0x1p40f;
                         const uint64_t f2 = f2_pack(f[i], f[i]), c2 = f2_pack(cw, cw);
                         uint64_t sum2 = 0;   // two zeros
 #pragma unroll
@@ -482,6 +485,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
                 float sum = shares == 1 ? l : 1.f;
                 if constexpr (std::is_same<T, __half>::value) sum = shares == 1 ? lr : lr / l;
                 inv = l == 0.f ? 0.f : root / sum * root;
+                if (spoilt[warp] >> lane & 1u) inv = NAN;
             }
             const int64_t part = out_row * a.part_stride + share;
             if (ok && shares > 1 && nk > 0) {   // (an empty share has no accumulator)
@@ -599,6 +603,13 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
                     ks = a.c.ks[at];
                     vs = a.c.vs[at];
                 }
+                const bool proper = vs <= FLT_MAX;
+                for (uint32_t bad = __ballot_sync(0xffffffffu, !proper); bad; bad &= bad - 1)
+#pragma unroll 1
+                    for (int w = 0; w < PF_ROWS / 32; ++w) {
+                        const uint32_t see = __ballot_sync(0xffffffffu, pf_mask(a, p0 + (r0 + 32 * w + lane) / a.group, k0 + 16 * (__ffs(bad) - 1), 1u));
+                        if (lane == 0) spoilt[w] |= see;
+                    }
                 uint32_t whole = 0;
                 if (lane < 4) {
                     const int t = lane >> 1, k = k0 + 64 * (lane & 1), lo = t ? lo1 : plo, hi = t ? phi : hi0;
@@ -608,7 +619,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_kv_prefill(const __grid_const
                 if (j >= PF_AHEAD && !(ok = pf_wait(ATEMPTY((j - PF_AHEAD) & (PF_RING - 1)), ((j - PF_AHEAD) / PF_RING) & 1))) break;
                 if (lane < 8) {
                     places[s].ks[lane] = ks;
-                    places[s].lv[lane] = log2f(vs);
+                    places[s].lv[lane] = proper ? log2f(vs) : -INFINITY;
                     places[s].iv[lane] = 1.f / vs;
                     places[s].at[lane] = at;
                 }
