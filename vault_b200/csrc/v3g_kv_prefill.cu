@@ -28,8 +28,8 @@
 // with scale 0 adds nothing to O and its full weight to the sum.  So does one whose V scale is NaN or infinite, since V is no
 // matter of the sum; the warp that looks up the scales notes which rows see such a block, and those have no output.
 //
-// 8,192 tokens, 32/8 heads of 128, every earlier key: 591 us, 930 TFLOP/s (517 us in a burst, before the clock falls); 4,608
-// tokens under a window of 1,024, 12/2 heads: 67 us, of which each of the two rounds of CTAs spends a quarter on its start and
+// 8,192 tokens, 32/8 heads of 128, every earlier key: 602 us, 913 TFLOP/s (530 us in a burst, before the clock falls); 4,608
+// tokens under a window of 1,024, 12/2 heads: 68 us, of which each of the two rounds of CTAs spends a quarter on its start and
 // end.
 #include <atomic>
 #include <cfloat>
